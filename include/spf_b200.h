@@ -33,6 +33,8 @@ extern "C" {
 
 #define SPF_MAX_BLOCKS 8192
 #define SPF_MAX_HEADS 256
+#define SPF_MAX_REQUESTS 4096       /* requests of one paged batch */
+#define SPF_MAX_KEYS (1 << 30)      /* tokens of one sequence */
 
 typedef enum spf_status {
   SPF_OK = 0,
@@ -50,6 +52,10 @@ typedef enum spf_status {
 #define SPF_HEAD_QUERY_AWARE 1
 #define SPF_HEAD_PIVOT 2
 #define SPF_HEAD_SHARED 4
+
+/* element types of the paged and windowed operators */
+#define SPF_BF16 0
+#define SPF_FP16 1
 
 const char* spf_status_string(int status);
 /* cudaGetErrorString of the last launch error seen by this library on this thread. */
@@ -257,6 +263,84 @@ int spf_decode_attention(const void* q, int64_t q_stride_h,
                          int n_keys, int n_q_heads, int n_kv_heads, int head_dim,
                          double softmax_scale, void* out, void* scratch, int64_t scratch_bytes,
                          void* stream);
+
+/* ---------------------------------------------------------------- paged cache: plan of a step
+ * (No counterpart in the reference, whose decode step reads a contiguous cache; this group and the next
+ * serve batches of requests whose K/V lie in pages of page_size tokens, page_size in {16,32,64,128,256}.)
+ * Request r has cached_len[r] tokens in the cache and brings new_len[r] more (negative counts as 0); row r of
+ * block_table [n_requests][table_stride >= table_width] lists its pages, the first
+ * ceil(cached_len / page_size) entries being its own.  The pages it lacks come from the free ring - ids
+ * free_ring[(head + i) % ring_capacity], i < count, with ring_state = {head, count}; a caller returns
+ * pages by writing them behind the last and raising count - in the order of the requests:
+ *   - a request is REFUSED when its sequence would not fit table_width (or SPF_MAX_KEYS), when its rows
+ *     would end behind n_rows, or when the pages that it and the requests before it lack (those refused
+ *     for the first two reasons not counted) exceed the ring's count; nobody overtakes for pages, but a
+ *     request that needs no new page is not held up;
+ *   - block_table gets the new ids; nothing else in it changes.
+ * Outputs: cu_new [R + 1] (first packed row of each request, at most n_rows; refused requests keep their
+ * rows), seq_len [R] (cached + new, 0 if refused), refused [R] (0 / 1), ring_state_out {head, count},
+ * and per packed row of the n_rows: slot_map (page * page_size + offset, -1 for rows of refused requests,
+ * of negative page ids and behind the last request) and positions (place in the sequence; 0 behind the
+ * last request).  Any output may be the buffer of the input it follows (seq_len = cached_len,
+ * ring_state_out = ring_state).  n_requests <= SPF_MAX_REQUESTS.
+ */
+int spf_paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_requests, int page_size,
+                   int32_t* block_table, int64_t table_stride, int table_width,
+                   const int32_t* free_ring, int ring_capacity, const int32_t* ring_state,
+                   int32_t* ring_state_out, int32_t* cu_new, int32_t* seq_len, int64_t* slot_map,
+                   int32_t* positions, int32_t* refused, int n_rows, void* stream);
+
+/* spf_paged_write: rows k, v [n_rows][Hkv][D] (16-bit elements of either type) into the slots of
+ * k_cache, v_cache [n_pages][page_size][Hkv][D], all with the given strides in elements (multiples of 8; D
+ * contiguous; a cache stored head-major is the same with other strides).  Rows whose slot lies outside
+ * [0, n_pages * page_size) are skipped.  Slots of one call must differ: of two rows with the same slot
+ * either may be found there, in whole or in part.
+ */
+int spf_paged_write(const void* k, int64_t k_stride_n, int64_t k_stride_h,
+                    const void* v, int64_t v_stride_n, int64_t v_stride_h,
+                    const int64_t* slot_map, int n_rows, int n_kv_heads, int head_dim,
+                    void* k_cache, int64_t k_stride_page, int64_t k_stride_token, int64_t k_stride_head,
+                    void* v_cache, int64_t v_stride_page, int64_t v_stride_token, int64_t v_stride_head,
+                    int n_pages, int page_size, void* stream);
+
+/* ---------------------------------------------------------------- attention over a paged cache
+ * The new tokens of every request (a chunk of a prompt, or one token) against its whole sequence in the
+ * cache, their own keys included: row cu_new[r] + i stands at position p = seq_len[r] - new_r + i, with
+ * new_r = cu_new[r + 1] - cu_new[r], and sees the keys j <= p with  j > p - window  or  j < sinks  (window
+ * 0: all j <= p) whose page id lies in [0, n_pages); keys behind table_width * page_size and keys of other
+ * ids are absent.  out = softmax(softmax_scale * q k^T) v with fp32 scores, statistics and accumulation; the
+ * weights are rounded to the inputs' type before the product with V.  A row that sees nothing (a refused
+ * request: seq_len 0) gives zeros.  Rows behind cu_new[R] are left as they were.
+ *   q: [n_rows][H][D], out: [n_rows][H][D] contiguous; caches as for spf_paged_write; dtype of all: SPF_BF16
+ *   or SPF_FP16.  max_new: an upper bound of new_r, read on the host; it selects the kernel, and rows of a
+ *   request past it need not be computed.  cu_new and seq_len are clipped to the batch on the device.
+ *   Keys that a request does not see are not read, or not used, whatever they hold (NaN included), except that
+ *   a NaN or infinity in a VALUE row that some token of a chunk sees can reach the chunk's other tokens.
+ *   scratch: spf_paged_scratch_bytes() bytes, 16-byte aligned, overwritten; calls that may run at the same
+ *   time need their own.
+ */
+int64_t spf_paged_scratch_bytes(int max_new, int n_q_heads, int n_kv_heads, int head_dim);
+int spf_paged_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, int n_rows, int n_q_heads,
+                        const void* k_cache, int64_t k_stride_page, int64_t k_stride_token, int64_t k_stride_head,
+                        const void* v_cache, int64_t v_stride_page, int64_t v_stride_token, int64_t v_stride_head,
+                        int n_pages, int page_size, int n_kv_heads, int head_dim, int dtype,
+                        const int32_t* block_table, int64_t table_stride, int table_width,
+                        const int32_t* cu_new, const int32_t* seq_len, int n_requests, int max_new,
+                        double softmax_scale, int window, int sinks, void* out,
+                        void* scratch, int64_t scratch_bytes, void* stream);
+
+/* ---------------------------------------------------------------- sliding window with sinks
+ * The same attention for one sequence in contiguous views: q [n_new][H][D] are the last n_new of n_keys
+ * tokens, k, v [n_keys][Hkv][D].  window >= 1 counts the query's own token; the first `sinks` tokens stay
+ * visible; window 0 is plain causal attention.  n_new = n_keys is a prompt, n_new = 1 a decode step.
+ * scratch: spf_paged_scratch_bytes(n_new, ...) bytes.
+ */
+int spf_window_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                         const void* k, int64_t k_stride_n, int64_t k_stride_h,
+                         const void* v, int64_t v_stride_n, int64_t v_stride_h,
+                         int n_new, int n_keys, int n_q_heads, int n_kv_heads, int head_dim, int dtype,
+                         double softmax_scale, int window, int sinks, void* out,
+                         void* scratch, int64_t scratch_bytes, void* stream);
 
 /* ---------------------------------------------------------------- bounded device-side waits
  * The tcgen05 kernels never spin without a limit: a wait (on an mbarrier) that has been spinning for

@@ -5,6 +5,8 @@
 #include <cstring>
 
 #include "spf_internal.cuh"
+#include "spf_paged.cuh"
+#include "spf_ragged.cuh"
 
 namespace spf {
 static thread_local cudaError_t g_last_error = cudaSuccess;
@@ -335,6 +337,151 @@ int spf_decode_attention(const void* q, int64_t q_stride_h, const void* k, int64
   p.splits = decode_splits(n_keys, n_q_heads, n_kv_heads);
   p.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   return decode_attention(p, head_dim, static_cast<cudaStream_t>(stream));
+}
+
+// log2 of a supported page size, or -1
+static int page_shift_of(int page_size) {
+  for (int s = 4; s <= 8; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+
+int spf_paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_requests, int page_size,
+                   int32_t* block_table, int64_t table_stride, int table_width, const int32_t* free_ring,
+                   int ring_capacity, const int32_t* ring_state, int32_t* ring_state_out, int32_t* cu_new,
+                   int32_t* seq_len, int64_t* slot_map, int32_t* positions, int32_t* refused, int n_rows, void* stream) {
+  if (!cached_len || !new_len || !block_table || !free_ring || !ring_state || !ring_state_out || !cu_new || !seq_len ||
+      !refused || (n_rows > 0 && (!slot_map || !positions)))
+    return SPF_ERR_NULL;
+  if (page_shift_of(page_size) < 0) return SPF_ERR_SHAPE;
+  if (n_requests <= 0 || n_rows < 0 || table_width <= 0 || table_stride < table_width || ring_capacity <= 0)
+    return SPF_ERR_RANGE;
+  if (n_requests > SPF_MAX_REQUESTS) return SPF_ERR_TOO_LARGE;
+  PlanParams p;
+  p.cached_len = cached_len; p.new_len = new_len; p.n_requests = n_requests; p.page_shift = page_shift_of(page_size);
+  p.table = block_table; p.table_stride = table_stride; p.table_width = table_width;
+  p.ring = free_ring; p.ring_capacity = ring_capacity; p.ring_state = ring_state; p.ring_state_out = ring_state_out;
+  p.cu_new = cu_new; p.seq_len = seq_len; p.slot_map = slot_map; p.positions = positions; p.refused = refused;
+  p.n_rows = n_rows;
+  return launch_paged_plan(p, static_cast<cudaStream_t>(stream));
+}
+
+int spf_paged_write(const void* k, int64_t k_stride_n, int64_t k_stride_h, const void* v, int64_t v_stride_n,
+                    int64_t v_stride_h, const int64_t* slot_map, int n_rows, int n_kv_heads, int head_dim,
+                    void* k_cache, int64_t k_stride_page, int64_t k_stride_token, int64_t k_stride_head,
+                    void* v_cache, int64_t v_stride_page, int64_t v_stride_token, int64_t v_stride_head, int n_pages,
+                    int page_size, void* stream) {
+  if (n_rows == 0) return SPF_OK;
+  if (!k || !v || !slot_map || !k_cache || !v_cache) return SPF_ERR_NULL;
+  const int shift = page_shift_of(page_size);
+  if (!supported_head_dim(head_dim) || n_kv_heads <= 0 || shift < 0) return SPF_ERR_SHAPE;
+  if (n_rows < 0 || n_pages <= 0) return SPF_ERR_RANGE;
+  if (n_kv_heads > SPF_MAX_HEADS) return SPF_ERR_TOO_LARGE;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache) || !strides_ok(k_stride_n, k_stride_h) ||
+      !strides_ok(v_stride_n, v_stride_h) || !strides_ok(k_stride_page, k_stride_token) || k_stride_head % 8 ||
+      !strides_ok(v_stride_page, v_stride_token) || v_stride_head % 8)
+    return SPF_ERR_ALIGN;
+  WriteParams p;
+  p.k = WriteTensor{static_cast<const uint16_t*>(k), k_stride_n, k_stride_h, static_cast<uint16_t*>(k_cache),
+                    k_stride_page, k_stride_token, k_stride_head};
+  p.v = WriteTensor{static_cast<const uint16_t*>(v), v_stride_n, v_stride_h, static_cast<uint16_t*>(v_cache),
+                    v_stride_page, v_stride_token, v_stride_head};
+  p.slot_map = slot_map; p.n_slots = int64_t(n_pages) << shift;
+  p.n_rows = n_rows; p.n_kv_heads = n_kv_heads; p.chunk_shift = head_dim == 128 ? 4 : 3; p.page_shift = shift;
+  return launch_paged_write(p, static_cast<cudaStream_t>(stream));
+}
+
+// what the two attention entry points check alike
+static int check_ragged(int n_q_heads, int n_kv_heads, int head_dim, int dtype, double softmax_scale, int window, int sinks) {
+  if (!supported_head_dim(head_dim) || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads) return SPF_ERR_SHAPE;
+  if (n_q_heads > SPF_MAX_HEADS) return SPF_ERR_TOO_LARGE;
+  if ((dtype != SPF_BF16 && dtype != SPF_FP16) || !std::isfinite(softmax_scale) || softmax_scale <= 0.0 || window < 0 || sinks < 0)
+    return SPF_ERR_RANGE;
+  return SPF_OK;
+}
+
+// how the work of a call is cut (tile_rows, units, CTAs); the scratch follows from it
+static void ragged_config(RaggedParams& p) { ragged_rows_config(p); }
+
+static int run_ragged(RaggedParams& p, int head_dim, int64_t scratch_bytes, cudaStream_t st) {
+  if (scratch_bytes < ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim)) return SPF_ERR_RANGE;
+  int rc = ragged_schedule(p, st);
+  if (rc == SPF_OK) rc = ragged_rows_attention(p, head_dim, st);
+  if (rc == SPF_OK) rc = ragged_merge(p, head_dim, st);
+  return rc;
+}
+
+int64_t spf_paged_scratch_bytes(int max_new, int n_q_heads, int n_kv_heads, int head_dim) {
+  if (max_new <= 0 || check_ragged(n_q_heads, n_kv_heads, head_dim, SPF_BF16, 1.0, 0, 0) != SPF_OK) return 0;
+  RaggedParams p;
+  p.group = n_q_heads / n_kv_heads;
+  ragged_config(p);
+  return ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim);
+}
+
+int spf_paged_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, int n_rows, int n_q_heads,
+                        const void* k_cache, int64_t k_stride_page, int64_t k_stride_token, int64_t k_stride_head,
+                        const void* v_cache, int64_t v_stride_page, int64_t v_stride_token, int64_t v_stride_head,
+                        int n_pages, int page_size, int n_kv_heads, int head_dim, int dtype, const int32_t* block_table,
+                        int64_t table_stride, int table_width, const int32_t* cu_new, const int32_t* seq_len,
+                        int n_requests, int max_new, double softmax_scale, int window, int sinks, void* out,
+                        void* scratch, int64_t scratch_bytes, void* stream) {
+  if (n_rows == 0) return SPF_OK;
+  if (!q || !k_cache || !v_cache || !block_table || !cu_new || !seq_len || !out || !scratch) return SPF_ERR_NULL;
+  const int rc = check_ragged(n_q_heads, n_kv_heads, head_dim, dtype, softmax_scale, window, sinks);
+  if (rc) return rc;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return SPF_ERR_SHAPE;
+  if (n_rows < 0 || n_pages <= 0 || n_requests <= 0 || max_new <= 0 || table_width <= 0 || table_stride < table_width)
+    return SPF_ERR_RANGE;
+  if (n_requests > SPF_MAX_REQUESTS || (int64_t(table_width) << shift) > SPF_MAX_KEYS || n_rows > SPF_MAX_KEYS)
+    return SPF_ERR_TOO_LARGE;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(scratch) ||
+      !strides_ok(q_stride_n, q_stride_h) || !strides_ok(k_stride_page, k_stride_token) || k_stride_head % 8 ||
+      !strides_ok(v_stride_page, v_stride_token) || v_stride_head % 8)
+    return SPF_ERR_ALIGN;
+  RaggedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q; p.q_sn = q_stride_n; p.q_sh = q_stride_h;
+  p.k = k_cache; p.k_sp = k_stride_page; p.k_st = k_stride_token; p.k_sh = k_stride_head;
+  p.v = v_cache; p.v_sp = v_stride_page; p.v_st = v_stride_token; p.v_sh = v_stride_head;
+  p.out = out; p.table = block_table; p.table_stride = table_stride; p.table_width = table_width;
+  p.n_pages = n_pages; p.page_shift = shift;
+  p.cu = cu_new; p.seq = seq_len; p.n_requests = n_requests; p.n_rows = n_rows;
+  p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads; p.group = n_q_heads / n_kv_heads;
+  p.window = window < SPF_MAX_KEYS ? window : 0; p.sinks = sinks < SPF_MAX_KEYS ? sinks : SPF_MAX_KEYS;
+  p.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  p.fp16 = dtype == SPF_FP16; p.scratch = static_cast<char*>(scratch);
+  ragged_config(p);
+  return run_ragged(p, head_dim, scratch_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int spf_window_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k, int64_t k_stride_n,
+                         int64_t k_stride_h, const void* v, int64_t v_stride_n, int64_t v_stride_h, int n_new,
+                         int n_keys, int n_q_heads, int n_kv_heads, int head_dim, int dtype, double softmax_scale,
+                         int window, int sinks, void* out, void* scratch, int64_t scratch_bytes, void* stream) {
+  if (n_new == 0) return SPF_OK;
+  if (!q || !k || !v || !out || !scratch) return SPF_ERR_NULL;
+  const int rc = check_ragged(n_q_heads, n_kv_heads, head_dim, dtype, softmax_scale, window, sinks);
+  if (rc) return rc;
+  if (n_new < 0 || n_keys < n_new) return SPF_ERR_RANGE;
+  if (n_keys > SPF_MAX_KEYS) return SPF_ERR_TOO_LARGE;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(scratch) ||
+      !strides_ok(q_stride_n, q_stride_h) || !strides_ok(k_stride_n, k_stride_h) || !strides_ok(v_stride_n, v_stride_h))
+    return SPF_ERR_ALIGN;
+  RaggedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q; p.q_sn = q_stride_n; p.q_sh = q_stride_h;
+  p.k = k; p.k_st = k_stride_n; p.k_sh = k_stride_h;
+  p.v = v; p.v_st = v_stride_n; p.v_sh = v_stride_h;
+  p.out = out; p.n_pages = 1;
+  p.n_requests = 1; p.n_rows = n_new; p.seq_one = n_keys;
+  p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads; p.group = n_q_heads / n_kv_heads;
+  p.window = window < SPF_MAX_KEYS ? window : 0; p.sinks = sinks < SPF_MAX_KEYS ? sinks : SPF_MAX_KEYS;
+  p.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  p.fp16 = dtype == SPF_FP16; p.scratch = static_cast<char*>(scratch);
+  ragged_config(p);
+  return run_ragged(p, head_dim, scratch_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int spf_device_timeouts(void) {

@@ -1,0 +1,415 @@
+// Ragged attention over a paged or contiguous KV cache (see spf_ragged.cuh): the schedule, the kernel for
+// items of up to 16 rows, and the kernel that joins broken items.
+#include "spf_mma.cuh"
+#include "spf_ragged.cuh"
+
+namespace spf {
+
+// ---------------------------------------------------------------- schedule
+// Every block sums the units of every request (a warp per request, its lanes over the tiles), scans the
+// sums, and each of its warps finds the start of one CTA: request by binary search, head by division, tile
+// by a scan over the tiles.
+constexpr int SCH_NT = 1024, SCH_WARPS = SCH_NT / 32;
+
+__device__ __forceinline__ long long warp_sum_ll(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+__global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedParams p) {
+  __shared__ long long upto[SPF_MAX_REQUESTS];   // inclusive sums over the requests
+  __shared__ long long wsum[SCH_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = p.n_kv_heads * p.head_chunks;
+  for (int r = warp; r < p.n_requests; r += SCH_WARPS) {
+    const RaggedReq q = ragged_req(p, r);
+    const int tiles = ragged_tiles(p, q.n);
+    long long s = 0;
+    for (int t = lane; t < tiles; t += 32) s += ragged_span(p, q, t).total;
+    s = warp_sum_ll(s);
+    if (lane == 0) upto[r] = s * heads;
+  }
+  __syncthreads();
+  long long carry = 0;
+  for (int r0 = 0; r0 < p.n_requests; r0 += SCH_NT) {
+    const int r = r0 + threadIdx.x;
+    long long v = warp_scan_ll(r < p.n_requests ? upto[r] : 0, lane);
+    if (lane == 31) wsum[warp] = v;
+    __syncthreads();
+    if (warp == 0) wsum[lane] = warp_scan_ll(wsum[lane], lane);
+    __syncthreads();
+    if (warp > 0) v += wsum[warp - 1];
+    if (r < p.n_requests) upto[r] = v + carry;
+    carry += wsum[SCH_WARPS - 1];
+    __syncthreads();
+  }
+  const int c = blockIdx.x * SCH_WARPS + warp;
+  if (c >= p.n_ctas) return;
+  const long long all = carry, per = max((all + p.n_ctas - 1) / p.n_ctas, 1ll), u = per * c;
+  RaggedStart s = {};
+  if (u < all) {
+    int lo = 0, hi = p.n_requests - 1;   // first request whose inclusive sum is above u
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (upto[mid] > u) hi = mid; else lo = mid + 1;
+    }
+    const long long before = lo > 0 ? upto[lo - 1] : 0;
+    const long long a_head = (upto[lo] - before) / heads;
+    const RaggedReq q = ragged_req(p, lo);
+    const int tiles = ragged_tiles(p, q.n);
+    s.req = lo;
+    s.head = int((u - before) / a_head);
+    long long rem = (u - before) - a_head * s.head;
+    for (int t0 = 0; t0 < tiles; t0 += 32) {
+      const int cost = t0 + lane < tiles ? ragged_span(p, q, t0 + lane).total : 0;
+      const long long inc = warp_scan_ll(cost, lane);
+      const unsigned above = __ballot_sync(0xffffffffu, inc > rem);
+      if (above) {
+        const int at = __ffs(above) - 1;
+        s.tile = t0 + at;
+        s.item_units = __shfl_sync(0xffffffffu, cost, at);
+        s.first = int(rem - __shfl_sync(0xffffffffu, inc - cost, at));
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, inc, 31);
+    }
+    s.units = int(min(per, all - u));
+  }
+  if (lane == 0) reinterpret_cast<RaggedStart*>(p.scratch)[c] = s;
+}
+
+int ragged_schedule(const RaggedParams& p, cudaStream_t st) {
+  ragged_schedule_kernel<<<ceil_div(p.n_ctas, SCH_WARPS), SCH_NT, 0, st>>>(p);
+  return check_launch();
+}
+
+// ---------------------------------------------------------------- join of broken items
+// Block (c, y): CTA c's start lies inside an item; if c is the first such CTA of that item, the pieces of
+// CTAs c - 1 (its second slot) and c, c + 1, ... (their first slots) are that item's.  A warp owns rows.
+constexpr int MRG_NT = 256;
+
+template <int D, bool FP16>
+__global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams p) {
+  constexpr int PER = D / 32;
+  const RaggedStart* starts = reinterpret_cast<const RaggedStart*>(p.scratch);
+  const int c = blockIdx.x + 1;
+  const RaggedStart s = starts[c];
+  if (s.units == 0 || s.first == 0) return;
+  const int per = starts[0].units;             // every CTA but the last runs through equally many
+  if (s.first > per) return;                   // an earlier CTA starts inside this item too
+  const int last = c + (s.item_units - s.first + per - 1) / per - 1;
+  const RaggedReq q = ragged_req(p, s.req);
+  const int kvh = s.head / p.head_chunks, h0 = (s.head % p.head_chunks) * p.chunk_heads;
+  const int heads = min(p.chunk_heads, p.group - h0);
+  const int rows = min(p.tile_tokens, q.n - s.tile * p.tile_tokens) * heads;
+  const int64_t stride = ragged_partial_floats(p.tile_rows, D);
+  const float* parts = reinterpret_cast<const float*>(p.scratch + ragged_starts_bytes(p.n_ctas));
+  auto part = [&](int i) { return parts + (i < 0 ? 2 * int64_t(c - 1) + 1 : 2 * int64_t(c + i)) * stride; };
+  const int n = last - c + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int row = blockIdx.y * (MRG_NT / 32) + warp; row < rows; row += gridDim.y * (MRG_NT / 32)) {
+    float top = -INFINITY;
+    for (int i = lane - 1; i < n; i += 32) top = fmaxf(top, part(i)[row]);
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int i = -1; i < n; ++i) {
+      const float* x = part(i);
+      const float w = exp2f(x[row] - ref);
+      sum += x[p.tile_rows + row] * w;
+      const float* o = x + 2 * p.tile_rows + row * D + lane * PER;
+#pragma unroll
+      for (int e = 0; e < PER; e += 2) {
+        const float2 t = *reinterpret_cast<const float2*>(o + e);
+        acc[e] += t.x * w; acc[e + 1] += t.y * w;
+      }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const int64_t tok = q.row0 + s.tile * p.tile_tokens + row / heads;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) +
+                    (tok * p.n_q_heads + kvh * p.group + h0 + row % heads) * D + lane * PER);
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) dst[e >> 1] = pack_half2<FP16>(acc[e] * inv, acc[e + 1] * inv);
+  }
+}
+
+int ragged_merge(const RaggedParams& p, int head_dim, cudaStream_t st) {
+  if (p.n_ctas < 2) return SPF_OK;
+  const dim3 grid(p.n_ctas - 1, ceil_div(p.tile_rows, MRG_NT / 32));
+  if (head_dim == 128) {
+    if (p.fp16) ragged_merge_kernel<128, true><<<grid, MRG_NT, 0, st>>>(p);
+    else ragged_merge_kernel<128, false><<<grid, MRG_NT, 0, st>>>(p);
+  } else {
+    if (p.fp16) ragged_merge_kernel<64, true><<<grid, MRG_NT, 0, st>>>(p);
+    else ragged_merge_kernel<64, false><<<grid, MRG_NT, 0, st>>>(p);
+  }
+  return check_launch();
+}
+
+// ---------------------------------------------------------------- items of up to 16 rows
+// The rows of an item are the 16 rows of mma.sync m16n8k16 tiles.  A unit is 64 keys, 16 per warp; every
+// warp streams its tiles through a private ring of cp.async stages and keeps its own running maximum, sum
+// and output; the warps meet when the CTA's part of the item ends.
+constexpr int RR_NT = 128, RR_NW = RR_NT / 32, RR_TT = 16, RR_STAGES = 3, RR_ROWS = 16;
+
+template <int D>
+constexpr int rr_smem_bytes() { return RR_NW * RR_STAGES * 2 * RR_TT * D * 2; }
+
+template <bool FP16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (FP16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    mma_bf16_16816(d, a, b0, b1);
+  }
+}
+
+template <int D, bool FP16>
+__global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p) {
+  constexpr int CH = D / 8, TILE_B = RR_TT * D * 2;
+  extern __shared__ __align__(128) uint8_t rsm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = smem_u32(rsm) + warp * (RR_STAGES * 2 * TILE_B);
+  const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
+  const RaggedStart start = reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
+  int left = start.units, req = start.req, head = start.head, tile = start.tile, first = start.first;
+  if (left == 0) return;
+  RaggedReq q = ragged_req(p, req);
+
+  while (true) {
+    const RaggedSpan span = ragged_span(p, q, tile);
+    const int units = min(left, span.total - first);
+    const int kvh = head / p.head_chunks, h0 = (head % p.head_chunks) * p.chunk_heads;
+    const int heads = min(p.chunk_heads, p.group - h0);
+    const int tok0 = tile * p.tile_tokens, rows = min(p.tile_tokens, q.n - tok0) * heads;
+    const int pos0 = q.seq - q.n + tok0;
+    const uint16_t* kb = static_cast<const uint16_t*>(p.k) + kvh * p.k_sh;
+    const uint16_t* vb = static_cast<const uint16_t*>(p.v) + kvh * p.v_sh;
+    const int32_t* table = p.table ? p.table + req * p.table_stride : nullptr;
+
+    // the item's query rows as A fragments (rows past its end are zero)
+    uint32_t qa[D / 16][4];
+    const int t_r0 = r0 / heads, t_r1 = r1 / heads;
+    {
+      const uint16_t* qb = static_cast<const uint16_t*>(p.q) + (int64_t(q.row0) + tok0) * p.q_sn +
+                           int64_t(kvh * p.group + h0) * p.q_sh + cq;
+      const uint16_t* q0 = qb + t_r0 * p.q_sn + (r0 - t_r0 * heads) * p.q_sh;
+      const uint16_t* q1 = qb + t_r1 * p.q_sn + (r1 - t_r1 * heads) * p.q_sh;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qa[ks][0] = r0 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16)) : 0u;
+        qa[ks][1] = r1 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16)) : 0u;
+        qa[ks][2] = r0 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16 + 8)) : 0u;
+        qa[ks][3] = r1 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16 + 8)) : 0u;
+      }
+    }
+    // row r sees keys <= hi that are >= lo or < sinks (rows past the item's end: none)
+    const int hi0 = r0 < rows ? pos0 + t_r0 : -1, hi1 = r1 < rows ? pos0 + t_r1 : -1;
+    const int lo0 = p.window > 0 ? hi0 - p.window + 1 : 0, lo1 = p.window > 0 ? hi1 - p.window + 1 : 0;
+    // keys in [all_lo, all_hi] are seen by every row of the item
+    const int all_hi = pos0, all_lo = p.window > 0 ? pos0 + p.tile_tokens - p.window : 0;
+    const int any_lo = p.window > 0 ? pos0 - p.window + 1 : 0;   // keys below it that are no sinks are seen by no row
+
+    // step u of this warp: 16 keys from key0(u); their page, -1 if absent
+    auto key0 = [&](int u) {
+      const int s = first + u, unit = s < span.sink_units ? s : span.win_first + s - span.sink_units;
+      return unit * (RR_TT * RR_NW) + warp * RR_TT;
+    };
+    auto page_of = [&](int u) -> int {
+      if (u >= units) return -1;
+      const int k0 = key0(u);
+      if (k0 >= span.keys) return -1;
+      if (!table) return 0;
+      const int pg = __ldg(table + (k0 >> p.page_shift));
+      return pg >= 0 && pg < p.n_pages ? pg : -1;
+    };
+    auto issue = [&](int u, int page, int stage) {
+      if (u < units) {
+        const int k0 = key0(u), valid = page >= 0 ? span.keys - k0 : 0;
+        const int in_page = table ? k0 & ((1 << p.page_shift) - 1) : k0;
+        const uint32_t ks = ring + stage * (2 * TILE_B), vs = ks + TILE_B;
+        const uint16_t* kp = kb + (valid > 0 ? page * p.k_sp + in_page * p.k_st : 0);
+        const uint16_t* vp = vb + (valid > 0 ? page * p.v_sp + in_page * p.v_st : 0);
+#pragma unroll
+        for (int i = lane; i < RR_TT * CH; i += 32) {
+          const int row = i / CH, ch = i % CH;
+          // keys that no row of the item sees are not read: whatever they hold, 0 times it must stay 0
+          const bool ok = row < valid && (k0 + row >= any_lo || k0 + row < p.sinks);
+          cp_async16(ks + tile_off<D>(row, ch), kp + (ok ? row * p.k_st + ch * 8 : 0), ok);
+          cp_async16(vs + tile_off<D>(row, ch), vp + (ok ? row * p.v_st + ch * 8 : 0), ok);
+        }
+      }
+      cp_async_commit();
+    };
+
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float o[D / 8][4];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+
+    // page ids run one step ahead of the copies that need them
+    int pg_a = page_of(0), pg_b = page_of(1), pg_c = page_of(2);
+    issue(0, pg_a, 0);
+    issue(1, pg_b, 1);
+    int stage = 0;
+    for (int u = 0; u < units; ++u) {
+      const int page = pg_a, pg_next = page_of(u + 3);
+      int pre = stage + 2; if (pre >= RR_STAGES) pre -= RR_STAGES;
+      issue(u + 2, pg_c, pre);
+      pg_a = pg_b; pg_b = pg_c; pg_c = pg_next;
+      cp_async_wait<2>();
+      __syncwarp();
+      if (page >= 0) {
+        const int k0 = key0(u);
+        const uint32_t ks_base = ring + stage * (2 * TILE_B), vs_base = ks_base + TILE_B;
+        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t b[4];
+          ldmatrix_x4(b, ks_base + tile_off<D>((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+          mma_16816<FP16>(s[0], qa[ks], b[0], b[1]);
+          mma_16816<FP16>(s[1], qa[ks], b[2], b[3]);
+        }
+        if (k0 >= all_lo && k0 + RR_TT - 1 <= all_hi) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][e] *= p.scale_log2;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = k0 + j * 8 + cq + (e & 1);
+              const int hi = e < 2 ? hi0 : hi1, lo = e < 2 ? lo0 : lo1;
+              s[j][e] = key <= hi && (key >= lo || key < p.sinks) && key < span.keys ? s[j][e] * p.scale_log2 : -INFINITY;
+            }
+        }
+        float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1)); x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet: all weights are 0
+        const float a0 = exp2f(m0 - f0), a1 = exp2f(m1 - f1);
+        m0 = n0; m1 = n1;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[j][0] = exp2f(s[j][0] - f0); s[j][1] = exp2f(s[j][1] - f0);
+          s[j][2] = exp2f(s[j][2] - f1); s[j][3] = exp2f(s[j][3] - f1);
+        }
+        l0 = l0 * a0 + (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
+        l1 = l1 * a1 + (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
+        // the weights are rounded to the inputs' type for the product, their sum is taken before that
+        const uint32_t pa[4] = {pack_half2<FP16>(s[0][0], s[0][1]), pack_half2<FP16>(s[0][2], s[0][3]),
+                                pack_half2<FP16>(s[1][0], s[1][1]), pack_half2<FP16>(s[1][2], s[1][3])};
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) { o[j][0] *= a0; o[j][1] *= a0; o[j][2] *= a1; o[j][3] *= a1; }
+#pragma unroll
+        for (int jj = 0; jj < D / 16; ++jj) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, vs_base + tile_off<D>((lane & 7) + (((lane >> 3) & 1) << 3), jj * 2 + (lane >> 4)));
+          mma_16816<FP16>(o[jj * 2], pa, b[0], b[1]);
+          mma_16816<FP16>(o[jj * 2 + 1], pa, b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (++stage == RR_STAGES) stage = 0;
+    }
+    cp_async_wait<0>();
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    __syncthreads();
+
+    // join the warps through shared memory (the rings are drained)
+    constexpr int WSTRIDE = 16 * D + 32;
+    float* wbuf = reinterpret_cast<float*>(rsm) + warp * WSTRIDE;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      *reinterpret_cast<float2*>(wbuf + r0 * D + j * 8 + cq) = make_float2(o[j][0], o[j][1]);
+      *reinterpret_cast<float2*>(wbuf + r1 * D + j * 8 + cq) = make_float2(o[j][2], o[j][3]);
+    }
+    if ((lane & 3) == 0) {
+      wbuf[16 * D + r0] = m0; wbuf[16 * D + r1] = m1;
+      wbuf[16 * D + 16 + r0] = l0; wbuf[16 * D + 16 + r1] = l1;
+    }
+    __syncthreads();
+    const float* all = reinterpret_cast<const float*>(rsm);
+    const bool whole = units == span.total;
+    float* part = reinterpret_cast<float*>(p.scratch + ragged_starts_bytes(p.n_ctas)) +
+                  (2 * int64_t(blockIdx.x) + (first == 0 ? 1 : 0)) * ragged_partial_floats(RR_ROWS, D);
+    for (int idx = threadIdx.x; idx < rows * (D / 2); idx += RR_NT) {
+      const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < RR_NW; ++w) top = fmaxf(top, all[w * WSTRIDE + 16 * D + r]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < RR_NW; ++w) {
+        const float sc = exp2f(all[w * WSTRIDE + 16 * D + r] - ref);
+        sum += all[w * WSTRIDE + 16 * D + 16 + r] * sc;
+        const float2 t = *reinterpret_cast<const float2*>(all + w * WSTRIDE + r * D + d);
+        x += t.x * sc; y += t.y * sc;
+      }
+      if (whole) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const int64_t tok = int64_t(q.row0) + tok0 + r / heads;
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) +
+                                     (tok * p.n_q_heads + kvh * p.group + h0 + r % heads) * D + d) =
+            pack_half2<FP16>(x * inv, y * inv);
+      } else {
+        *reinterpret_cast<float2*>(part + 2 * RR_ROWS + r * D + d) = make_float2(x, y);
+        if (d == 0) { part[r] = top; part[RR_ROWS + r] = sum; }
+      }
+    }
+    left -= units;
+    if (left == 0) return;
+    first = 0;
+    if (!ragged_next(p, req, head, tile, q)) return;
+    __syncthreads();   // the buffers become rings again
+  }
+}
+
+// Two CTAs per SM: 96 KiB of rings each at D = 128.
+void ragged_rows_config(RaggedParams& p) {
+  p.tile_rows = RR_ROWS;
+  p.head_chunks = ceil_div(p.group, RR_ROWS);
+  p.chunk_heads = ceil_div(p.group, p.head_chunks);
+  p.tile_tokens = RR_ROWS / p.chunk_heads;
+  p.unit_keys = RR_TT * RR_NW;
+  p.n_ctas = 2 * 148;
+}
+
+template <int D, bool FP16>
+static int launch_rows(const RaggedParams& p, cudaStream_t st) {
+  constexpr int SMEM = rr_smem_bytes<D>();
+  static_assert(SMEM >= RR_NW * (16 * D + 32) * 4, "the join of the warps must fit in the rings");
+  const cudaError_t e = cudaFuncSetAttribute(ragged_rows_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
+  ragged_rows_kernel<D, FP16><<<p.n_ctas, RR_NT, SMEM, st>>>(p);
+  return check_launch();
+}
+
+int ragged_rows_attention(const RaggedParams& p, int head_dim, cudaStream_t st) {
+  if (head_dim == 128) return p.fp16 ? launch_rows<128, true>(p, st) : launch_rows<128, false>(p, st);
+  return p.fp16 ? launch_rows<64, true>(p, st) : launch_rows<64, false>(p, st);
+}
+
+}  // namespace spf

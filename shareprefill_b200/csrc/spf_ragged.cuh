@@ -1,0 +1,114 @@
+// Attention of ragged batches of query rows over a paged (or contiguous) KV cache: what the kernels of
+// this family share.  Request r brings n_r new tokens that stand at positions seq_r - n_r ... seq_r - 1
+// of its sequence; the query at position p sees the keys
+//     j <= p   and   (no window,  j > p - window,  or  j < sinks)   and   j's page is present,
+// o = softmax(scale * q k^T) v over the seen keys, zeros if there is none.
+//
+// Work is cut twice.  An ITEM is a tile of packed query rows (tile_tokens consecutive tokens x the query
+// heads that share a KV head, row = token * heads + head) of one request and one KV head; its cost is the
+// number of UNITS (unit_keys consecutive keys) that any of its rows sees.  All units of all items form
+// one line, which is cut into equal pieces, one per CTA: a CTA runs through the end of one item, whole
+// items, and the start of another.  Whole items are written to the output, the two broken ones leave
+// their partial (max, sum, unnormalised output) behind and a second kernel joins them.  The load is even
+// whatever the lengths are, nothing about them is needed on the host, and the scratch is two tiles per CTA.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "spf_internal.cuh"
+
+namespace spf {
+
+struct RaggedParams {
+  const void* q; int64_t q_sn, q_sh;
+  const void* k; int64_t k_sp, k_st, k_sh;   // strides of a page, a token of a page, a KV head
+  const void* v; int64_t v_sp, v_st, v_sh;
+  void* out;                                 // [n_rows][H][D]
+  const int32_t* table; int64_t table_stride;  // [R][table_width]; nullptr: contiguous keys (one request)
+  int table_width, n_pages, page_shift;
+  const int32_t* cu; const int32_t* seq;     // [R + 1], [R]; nullptr: one request of n_rows tokens, seq_one keys
+  int n_requests, n_rows, seq_one;
+  int n_q_heads, n_kv_heads, group;
+  int window, sinks;                         // window 0: none
+  float scale_log2;
+  int fp16;
+  // how the work is cut
+  int head_chunks, chunk_heads;              // a KV head's group as head_chunks pieces of at most chunk_heads heads
+  int tile_rows, tile_tokens, unit_keys, n_ctas;
+  char* scratch;
+};
+
+// where a CTA starts (written by the schedule kernel); units: what it runs through, 0 if it has no work
+struct RaggedStart { int req, head, tile, first, units, item_units, pad0, pad1; };
+
+// units of one item: [0, sink_units) and then [win_first, win_first + total - sink_units)
+struct RaggedSpan { int total, sink_units, win_first, keys; };   // keys: exclusive end of the keys in view
+
+__host__ __device__ inline int ragged_starts_bytes(int n_ctas) { return (n_ctas * int(sizeof(RaggedStart)) + 255) & ~255; }
+__host__ __device__ inline int64_t ragged_partial_floats(int tile_rows, int head_dim) { return int64_t(tile_rows) * (head_dim + 2); }
+inline int64_t ragged_scratch_bytes(int n_ctas, int tile_rows, int head_dim) {
+  return ragged_starts_bytes(n_ctas) + 2 * n_ctas * ragged_partial_floats(tile_rows, head_dim) * 4;
+}
+
+#ifdef __CUDACC__
+struct RaggedReq { int row0, n, seq; };   // first packed row, new tokens, sequence length (whatever the arrays hold, rows stay in the batch)
+
+__device__ __forceinline__ RaggedReq ragged_req(const RaggedParams& p, int r) {
+  RaggedReq q;
+  if (p.cu == nullptr) {
+    q.row0 = 0; q.n = p.n_rows; q.seq = p.seq_one;
+  } else {
+    const int a = min(max(__ldg(p.cu + r), 0), p.n_rows), b = min(max(__ldg(p.cu + r + 1), a), p.n_rows);
+    q.row0 = a; q.n = b - a; q.seq = min(max(__ldg(p.seq + r), 0), SPF_MAX_KEYS);
+  }
+  return q;
+}
+
+__device__ __forceinline__ RaggedSpan ragged_span(const RaggedParams& p, const RaggedReq& q, int tile) {
+  const int t0 = tile * p.tile_tokens, t1 = min(t0 + p.tile_tokens, q.n);
+  const int first_pos = q.seq - q.n + t0;
+  int64_t end = q.seq - q.n + t1;
+  if (p.table != nullptr) end = min(end, int64_t(p.table_width) << p.page_shift);
+  RaggedSpan s;
+  s.keys = int(max(end, int64_t(0)));
+  const int low = p.window > 0 ? max(first_pos - p.window + 1, 0) : 0;
+  const int end_unit = (s.keys + p.unit_keys - 1) / p.unit_keys;
+  s.win_first = min(low / p.unit_keys, end_unit);
+  s.sink_units = min(p.sinks / p.unit_keys + (p.sinks % p.unit_keys != 0), s.win_first);
+  s.total = max(s.sink_units + end_unit - s.win_first, 1);   // an item that sees nothing still has zeros to write
+  return s;
+}
+
+__device__ __forceinline__ int ragged_tiles(const RaggedParams& p, int n) { return (n + p.tile_tokens - 1) / p.tile_tokens; }
+
+// the item after (req, head, tile); false behind the last one
+__device__ __forceinline__ bool ragged_next(const RaggedParams& p, int& req, int& head, int& tile, RaggedReq& q) {
+  if (++tile < ragged_tiles(p, q.n)) return true;
+  tile = 0;
+  if (++head < p.n_kv_heads * p.head_chunks) return true;
+  head = 0;
+  while (++req < p.n_requests) {
+    q = ragged_req(p, req);
+    if (q.n > 0) return true;
+  }
+  return false;
+}
+
+template <bool FP16>
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  if (FP16) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+#endif  // __CUDACC__
+
+int ragged_schedule(const RaggedParams& p, cudaStream_t st);
+int ragged_merge(const RaggedParams& p, int head_dim, cudaStream_t st);
+// up to 16 packed rows an item: bandwidth bound (single tokens); also what TMA cannot describe
+void ragged_rows_config(RaggedParams& p);
+int ragged_rows_attention(const RaggedParams& p, int head_dim, cudaStream_t st);
+
+}  // namespace spf

@@ -1,0 +1,378 @@
+"""Paged cache and windowed attention on the GPU against the 64-bit statements of tests/paged_reference.py."""
+import random
+
+import pytest
+import torch
+
+import paged_reference as R
+from shareprefill_b200 import native
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------ plan
+def _random_plan(seed, requests, page, spare, ctx, new, pad, width_cut=0, short_rows=0):
+    rng = random.Random(seed)
+    cached = [rng.choice([0, 1, page - 1, page, page + 1, rng.randint(0, ctx)]) for _ in range(requests)]
+    fresh = [rng.choice([0, 1, 1, page, rng.randint(0, new)]) for _ in range(requests)]
+    held = [-(-c // page) for c in cached]
+    width = max(-(-(c + n) // page) for c, n in zip(cached, fresh)) + 1 - width_cut
+    width = max(width, max(held), 1)
+    ids = list(range(sum(held) + spare))
+    rng.shuffle(ids)
+    table, at = [], 0
+    for h in held:
+        table.append(ids[at:at + h] + [-7] * (width - h))
+        at += h
+    head = rng.randrange(len(ids) or 1)
+    ring = [-9] * max(len(ids), 1)
+    for i, x in enumerate(ids[at:]):
+        ring[(head + i) % len(ring)] = x
+    return cached, fresh, table, width, ring, head, spare, max(0, sum(fresh) + pad - short_rows)
+
+
+@pytest.mark.parametrize("seed,requests,page,spare,ctx,new,pad,width_cut,short_rows", [
+    (1, 1, 16, 4, 40, 3, 0, 0, 0), (2, 7, 16, 200, 300, 70, 5, 0, 0), (3, 33, 32, 9, 500, 200, 0, 0, 0),
+    (4, 64, 64, 0, 900, 100, 3, 0, 0), (5, 513, 16, 700, 700, 60, 11, 2, 0), (6, 1500, 256, 500, 5000, 20, 0, 0, 300),
+    (7, 4096, 16, 9000, 100, 40, 1, 1, 17), (8, 3, 128, 50, 40, 9000, 0, 0, 0),
+])
+def test_plan_equals_the_statement(seed, requests, page, spare, ctx, new, pad, width_cut, short_rows):
+    cached, fresh, table, width, ring, head, count, n_rows = _random_plan(seed, requests, page, spare, ctx, new, pad,
+                                                                          width_cut, short_rows)
+    want = R.plan(cached, fresh, table, width, ring, head, count, n_rows, page)
+    t = _ints(table)
+    got = native.paged_plan(_ints(cached), _ints(fresh), t, _ints(ring), _ints([head, count]), n_rows, page)
+    assert t.tolist() == want["table"]
+    for name in ("cu_new", "seq_len", "refused", "slot_map", "positions", "ring_state"):
+        assert getattr(got, name).tolist() == want[name], name
+    # once more over its own result: the entries are found again, not taken anew
+    again = native.paged_plan(_ints(cached), _ints(fresh), t, _ints(ring), _ints([head, count]), n_rows, page)
+    assert t.tolist() == want["table"] and again.slot_map.tolist() == want["slot_map"]
+
+
+def test_plan_in_place_state_odd_lengths_and_padded_table_rows():
+    page, cap = 16, 10
+    ring, state = _ints(list(range(100, 100 + cap))), _ints([8, 5])
+    table = torch.full((3, 9), -1, dtype=torch.int32, device="cuda")[:, :6]      # rows further apart than wide
+    cached, fresh = _ints([-4, 0, 16]), _ints([17, -3, 1])
+    table[2, 0] = 55
+    p = native.paged_plan(cached, fresh, table, ring, state, 20, page, ring_state_out=state)
+    want = R.plan([-4, 0, 16], [17, -3, 1], [[-1] * 6, [-1] * 6, [55] + [-1] * 5], 6, list(range(100, 110)), 8, 5, 20, page)
+    assert p.ring_state.data_ptr() == state.data_ptr() and state.tolist() == want["ring_state"] == [1, 2]
+    assert table.tolist() == want["table"] and p.slot_map.tolist() == want["slot_map"]
+    assert p.seq_len.tolist() == [17, 0, 17] and p.refused.tolist() == [0, 0, 0]
+
+
+def test_plan_with_extreme_lengths_refuses_and_stays_inside():
+    page, top = 16, 2 ** 31 - 1
+    table = torch.full((4, 3), -1, dtype=torch.int32, device="cuda")
+    ring, state = _ints(list(range(8))), _ints([2 ** 31 - 1, 2 ** 31 - 1])       # head and count past the ring
+    p = native.paged_plan(_ints([top, 0, top, 3]), _ints([1, top, top, 2]), table, ring, state, 5, page)
+    assert p.refused.tolist() == [1, 1, 1, 1]      # the rows of the last lie behind the batch
+    assert p.cu_new.tolist() == [0, 1, 5, 5, 5] and p.slot_map.tolist() == [-1] * 5
+    assert bool((table == -1).all())
+
+
+# ----------------------------------------------------------------------------------------- write
+@pytest.mark.parametrize("rows,kv_heads,dim,page,dtype,layout", [
+    (1, 1, 64, 16, BF16, "token"), (37, 8, 128, 16, FP16, "head"), (1000, 4, 128, 64, BF16, "joined"),
+    (257, 3, 64, 256, FP16, "token"), (5000, 8, 128, 32, BF16, "token"),
+])
+def test_write_puts_rows_in_their_slots_and_nothing_else(rows, kv_heads, dim, page, dtype, layout):
+    g = torch.Generator().manual_seed(rows)
+    lengths = [rows]
+    pool = R.Pool(lengths, page, kv_heads, dim, dtype, g, layout)
+    k_cache, v_cache = pool.cuda()
+    k_cache.fill_(3.0), v_cache.fill_(4.0)
+    k = torch.randn(rows, kv_heads + 2, dim, generator=g).to(dtype).cuda()[:, 1:-1]     # strided rows
+    v = torch.randn(kv_heads, rows, dim, generator=g).to(dtype).cuda().transpose(0, 1)
+    n_slots = k_cache.shape[0] * page
+    slots = torch.randperm(n_slots, generator=g)[:rows]
+    bad = torch.rand(rows, generator=g) < 0.1
+    slots[bad] = torch.tensor([-1, n_slots, n_slots + 5, -2 ** 40, 2 ** 62])[torch.randint(0, 5, (int(bad.sum()),), generator=g)]
+    want_k, want_v = k_cache.clone(), v_cache.clone()
+    keep = slots[~bad].cuda()
+    want_k[keep // page, keep % page] = k[~bad.cuda()]
+    want_v[keep // page, keep % page] = v[~bad.cuda()]
+    native.paged_write(k, v, slots.cuda(), k_cache, v_cache)
+    assert torch.equal(k_cache, want_k) and torch.equal(v_cache, want_v)
+
+
+# ------------------------------------------------------------------------------------- attention
+CASES = [
+    # (cached, new) per request, page, heads, kv heads, head size, type, window, sinks, cache layout
+    ([(0, 1)], 16, 32, 8, 128, BF16, 0, 0, "token"),
+    ([(15, 1), (16, 1), (0, 1), (700, 1), (63, 1)], 16, 32, 8, 128, BF16, 0, 0, "head"),
+    ([(2000, 1), (31, 1)], 32, 28, 4, 128, FP16, 0, 0, "token"),
+    ([(900, 1), (5, 1), (130, 1)], 64, 64, 8, 64, BF16, 100, 4, "joined"),
+    ([(900, 1), (5, 1)], 256, 8, 2, 128, BF16, 1, 0, "token"),
+    ([(777, 1), (300, 1)], 16, 16, 1, 128, FP16, 33, 200, "token"),
+    ([(100, 4), (0, 3), (47, 1), (200, 2)], 16, 8, 2, 128, BF16, 0, 0, "token"),
+    ([(0, 130)], 16, 8, 2, 64, BF16, 0, 0, "token"),
+    ([(0, 1), (0, 0), (500, 77), (3, 0), (64, 64)], 64, 8, 2, 128, BF16, 0, 0, "head"),
+    ([(1000, 300), (0, 257), (33, 1)], 128, 14, 2, 128, FP16, 0, 0, "joined"),
+    ([(1000, 300), (0, 257), (33, 1), (5, 40)], 32, 8, 2, 64, FP16, 70, 5, "token"),
+    ([(600, 500)], 16, 4, 4, 128, BF16, 128, 130, "head"),
+    ([(130, 260), (7, 9)], 16, 40, 1, 128, BF16, 0, 0, "token"),        # 40 heads on one KV head
+    ([(50, 3), (0, 20)], 16, 200, 1, 64, BF16, 0, 0, "token"),
+    ([(0, 1000)], 256, 6, 2, 128, BF16, 8, 1, "token"),
+    ([(3000, 64)] + [(i * 37, 1) for i in range(40)], 16, 8, 2, 128, BF16, 0, 0, "token"),
+]
+
+
+def _batch(spec, page, heads, kv_heads, dim, dtype, layout, seed):
+    g = torch.Generator().manual_seed(seed)
+    pool = R.Pool([c + n for c, n in spec], page, kv_heads, dim, dtype, g, layout)
+    cu = [0]
+    for _, n in spec:
+        cu.append(cu[-1] + n)
+    q = (1.5 * torch.randn(cu[-1], heads, dim, generator=g)).to(dtype)
+    return pool, cu, q
+
+
+def _check_batch(got, spec, pool, cu, q, scale, window, sinks, dtype, present=None):
+    for r, (c, n) in enumerate(spec):
+        k, v = pool.rows[r]
+        out, mass = R.attention(q[cu[r]:cu[r + 1]], k, v, c, scale, window, sinks, None if present is None else present[r])
+        if n:
+            R.check(got[cu[r]:cu[r + 1]], out, mass, dtype, c + n, float(v.abs().max()), f"request {r}")
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_paged_attention_matches_the_statement(case):
+    spec, page, heads, kv_heads, dim, dtype, window, sinks, layout = CASES[case]
+    pool, cu, q = _batch(spec, page, heads, kv_heads, dim, dtype, layout, 100 + case)
+    k, v = pool.cuda()
+    scale = dim ** -0.5
+    got = native.paged_attention(q.cuda(), k, v, pool.table.cuda(), _ints(cu), _ints([c + n for c, n in spec]),
+                                 max(n for _, n in spec), scale, window, sinks)
+    _check_batch(got, spec, pool, cu, q, scale, window, sinks, dtype)
+
+
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_rows_without_keys_absent_pages_and_rows_behind_the_batch(new):
+    page, heads, kv_heads, dim, dtype = 16, 8, 2, 128, BF16
+    spec = [(100, new), (200, new), (40, new)]
+    pool, cu, q = _batch(spec, page, heads, kv_heads, dim, dtype, "token", new)
+    k, v = pool.cuda()
+    # request 0 loses pages 1 and 4 (ids outside the pool), request 1 is refused, request 2 keeps only absent pages
+    table = pool.table.clone()
+    table[0, 1], table[0, 4] = -3, k.shape[0]
+    table[2] = 2 ** 31 - 1
+    present = torch.ones(100 + new, dtype=torch.bool)
+    present[16:32] = False
+    present[64:80] = False
+    rows = torch.cat([q, q[:5]]).cuda()
+    out = torch.full_like(rows, 7.0)
+    got = native.paged_attention(rows, k, v, table.cuda(), _ints(cu), _ints([100 + new, 0, 40 + new]), new, dim ** -0.5,
+                                 out=out)
+    assert got.data_ptr() == out.data_ptr()
+    _check_batch(got, spec[:1], pool, cu, q, dim ** -0.5, 0, 0, dtype, [present])
+    assert bool((got[cu[1]:cu[3]] == 0).all()), "refused and absent: zeros"
+    assert bool((got[cu[3]:] == 7).all()), "rows behind the batch were touched"
+
+
+def test_offsets_and_lengths_that_lie_are_clipped():
+    page, heads, kv_heads, dim = 16, 8, 2, 64
+    spec = [(30, 2)]
+    pool, cu, q = _batch(spec, page, heads, kv_heads, dim, BF16, "token", 5)
+    k, v = pool.cuda()
+    table = pool.table.cuda().expand(3, -1).contiguous()
+    for cu_bad in ([0, 2, 2, 400], [-9, 2, 2, 2], [0, 2, 2, 1]):
+        got = native.paged_attention(q.cuda(), k, v, table, _ints(cu_bad), _ints([32, 2 ** 31 - 1, -1]), 2, dim ** -0.5)
+        _check_batch(got, spec, pool, cu, q, dim ** -0.5, 0, 0, BF16)
+
+
+@pytest.mark.parametrize("new", [1, 200])
+def test_cache_of_more_than_32_bits_of_elements(new):
+    page, heads, kv_heads, dim = 64, 8, 8, 128
+    n_pages = (2 ** 32 // (page * kv_heads * dim)) + 40
+    if torch.cuda.mem_get_info()[0] < 3 * n_pages * page * kv_heads * dim * 2:
+        pytest.skip("not enough free memory")
+    spec = [(500, new)]
+    pool, cu, q = _batch(spec, page, heads, kv_heads, dim, BF16, "token", 11)
+    k, v = (torch.empty(n_pages, page, kv_heads, dim, dtype=BF16, device="cuda") for _ in range(2))
+    table = torch.full_like(pool.table, -1)
+    for i in range(-(-(500 + new) // page)):
+        table[0, i] = n_pages - 1 - 2 * i
+        k[table[0, i]] = pool.k[pool.table[0, i]].cuda()
+        v[table[0, i]] = pool.v[pool.table[0, i]].cuda()
+    got = native.paged_attention(q.cuda(), k, v, table.cuda(), _ints(cu), _ints([500 + new]), new, dim ** -0.5)
+    _check_batch(got, spec, pool, cu, q, dim ** -0.5, 0, 0, BF16)
+
+
+# ---------------------------------------------------------------------------------------- window
+@pytest.mark.parametrize("new,keys,heads,kv_heads,dim,dtype,window,sinks,layout", [
+    (1, 1, 32, 8, 128, BF16, 4, 0, "token"), (1, 5000, 32, 8, 128, BF16, 1000, 4, "token"),
+    (1, 3001, 28, 4, 64, FP16, 37, 300, "head"), (5, 5, 8, 2, 128, BF16, 2, 1, "token"),
+    (129, 129, 8, 2, 128, FP16, 64, 0, "head"), (1000, 1000, 8, 2, 64, BF16, 256, 4, "token"),
+    (700, 1500, 14, 2, 128, BF16, 300, 140, "token"), (257, 900, 4, 4, 128, BF16, 5000, 3, "head"),
+    (640, 640, 8, 1, 128, BF16, 1, 0, "token"), (300, 1000, 40, 1, 64, FP16, 129, 1, "token"),
+    (513, 513, 8, 2, 128, BF16, 0, 9, "token"), (1500, 1500, 32, 8, 64, BF16, 128, 128, "token"),
+])
+def test_window_attention_matches_the_statement(new, keys, heads, kv_heads, dim, dtype, window, sinks, layout):
+    g = torch.Generator().manual_seed(new + keys)
+    q = (1.5 * torch.randn(new, heads, dim, generator=g)).to(dtype)
+    k, v = (torch.randn(keys, kv_heads, dim, generator=g).to(dtype) for _ in range(2))
+    dq, dk, dv = q.cuda(), k.cuda(), v.cuda()
+    if layout == "head":        # [heads, tokens, D] storage seen token-major
+        dq, dk, dv = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (dq, dk, dv))
+    got = native.window_attention(dq, dk, dv, dim ** -0.5, window, sinks)
+    out, mass = R.attention(q, k, v, keys - new, dim ** -0.5, window, sinks)
+    R.check(got, out, mass, dtype, keys, float(v.abs().max()))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_values_that_no_query_sees_may_be_anything(new):
+    dim, keys, window, sinks = 128, 900, 100, 4
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(new, 8, dim, generator=g).to(BF16)
+    k, v = (torch.randn(keys, 2, dim, generator=g).to(BF16) for _ in range(2))
+    out, mass = R.attention(q, k, v, keys - new, dim ** -0.5, window, sinks)
+    hidden = slice(sinks, keys - new - window + 1)
+    for bad in (float("nan"), float("inf"), torch.finfo(BF16).min):
+        k[hidden], v[hidden] = bad, bad
+        got = native.window_attention(q.cuda(), k.cuda(), v.cuda(), dim ** -0.5, window, sinks)
+        R.check(got, out, mass, BF16, keys, 5.0)
+
+
+@pytest.mark.parametrize("new", [1, 200])
+@pytest.mark.parametrize("gain", [30.0, 1e4])
+def test_peaked_scores_and_expanded_caches(new, gain):
+    # scores far apart (the reference point of the exponentials moves often) and one KV row shared by views
+    dim = 128
+    g = torch.Generator().manual_seed(17)
+    q = (gain * torch.randn(new, 4, dim, generator=g)).to(BF16)
+    k, v = (torch.randn(1000, 1, dim, generator=g).to(BF16) for _ in range(2))
+    out, _ = R.attention(q, k, v, 1000 - new, dim ** -0.5, 0, 0)
+    got = native.window_attention(q.cuda(), k.cuda().expand(-1, 2, -1), v.cuda().expand(-1, 2, -1), dim ** -0.5, 0)
+    # weights differ by e^(score error): 128 products of size gain * 4 sum up with errors of 128 * 2^-24 * their size
+    s_err = 128 * 2.0 ** -24 * gain * 4 * 4 * dim ** 0.5
+    mass = R.attention(q, k, v, 1000 - new, dim ** -0.5, 0, 0)[1]
+    tol = R.tolerance(out, mass, BF16, 1000, 5.0) + 2 * min(s_err, 1.0) * (mass + out.abs())
+    assert bool(((got.double().cpu() - out).abs() <= tol).all())
+
+
+# ---------------------------------------------------------------------------------- run together
+def test_a_serving_loop_plan_write_attend_over_pages():
+    page, heads, kv_heads, dim, dtype, window, sinks = 16, 8, 2, 128, BF16, 60, 3
+    g = torch.Generator().manual_seed(23)
+    steps = [[40, 0, 7], [33, 100, 1], [1, 1, 1], [1, 17, 0], [1, 1, 1], [0, 300, 2]]
+    n_pages = 64
+    shape = (n_pages, page, kv_heads, dim)
+    k_cache, v_cache = (torch.full(shape, float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    table = torch.full((3, 40), -1, dtype=torch.int32, device="cuda")
+    ring, state = torch.randperm(n_pages, generator=g).to(torch.int32).cuda(), _ints([5, n_pages])
+    seq = _ints([0, 0, 0])
+    history = [(torch.empty(0, kv_heads, dim, dtype=dtype),) * 2 for _ in range(3)]
+    for new in steps:
+        rows = sum(new) + 3                                   # a padded batch
+        q = torch.randn(rows, heads, dim, generator=g).to(dtype)
+        k, v = (torch.randn(rows, kv_heads, dim, generator=g).to(dtype) for _ in range(2))
+        plan = native.paged_plan(seq, _ints(new), table, ring, state, rows, page, ring_state_out=state)
+        native.paged_write(k.cuda(), v.cuda(), plan.slot_map, k_cache, v_cache)
+        out = native.paged_attention(q.cuda(), k_cache, v_cache, table, plan.cu_new, plan.seq_len, max(new), dim ** -0.5,
+                                     window, sinks)
+        seq = plan.seq_len
+        at = 0
+        for r, n in enumerate(new):
+            hk, hv = history[r]
+            history[r] = (torch.cat([hk, k[at:at + n]]), torch.cat([hv, v[at:at + n]]))
+            if n:
+                want, mass = R.attention(q[at:at + n], *history[r], len(hk), dim ** -0.5, window, sinks)
+                R.check(out[at:at + n], want, mass, dtype, len(hk) + n, 5.0, f"step {new} request {r}")
+            at += n
+        assert seq.tolist() == [len(h[0]) for h in history] and plan.refused.tolist() == [0, 0, 0]
+    assert state[1].item() == n_pages - sum(-(-len(h[0]) // page) for h in history)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_captured_graphs_replay_with_new_lengths_side_by_side(new):
+    page, heads, kv_heads, dim = 16, 8, 2, 128
+    spec = [(300, new), (77, new)]
+    pool, cu, q = _batch(spec, page, heads, kv_heads, dim, BF16, "token", 31)
+    k, v = pool.cuda()
+    table = pool.table.cuda()
+    graphs = []
+    for _ in range(2):
+        s = dict(q=torch.zeros_like(q).cuda(), cu=_ints([0, 0, 0]), seq=_ints([0, 0]), stream=torch.cuda.Stream())
+        with torch.cuda.stream(s["stream"]):
+            native.paged_attention(s["q"], k, v, table, s["cu"], s["seq"], new, dim ** -0.5)
+        torch.cuda.synchronize()
+        s["graph"] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(s["graph"]):
+            s["out"] = native.paged_attention(s["q"], k, v, table, s["cu"], s["seq"], new, dim ** -0.5)
+        graphs.append(s)
+    for cut in (0, 33):
+        want = []
+        for i, s in enumerate(graphs):
+            lens = [c + n - cut * (i + 1) for c, n in spec]
+            s["q"].copy_(q * (1 + i)), s["cu"].copy_(_ints(cu)), s["seq"].copy_(_ints(lens))
+            want.append([R.attention(q[cu[r]:cu[r + 1]] * (1 + i), *(x[:lens[r]] for x in pool.rows[r]),
+                                     lens[r] - spec[r][1], dim ** -0.5) for r in range(2)])
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s in graphs:
+                with torch.cuda.stream(s["stream"]):
+                    s["graph"].replay()
+        torch.cuda.synchronize()
+        for i, s in enumerate(graphs):
+            for r in range(2):
+                R.check(s["out"][cu[r]:cu[r + 1]], *want[i][r], BF16, 400, 5.0, f"graph {i} request {r} cut {cut}")
+
+
+def test_results_do_not_depend_on_the_run_or_the_stream():
+    pool, cu, q = _batch([(3000, 1), (777, 1), (20, 1)], 16, 32, 8, 128, BF16, "token", 41)
+    k, v = pool.cuda()
+    args = (q.cuda(), k, v, pool.table.cuda(), _ints(cu), _ints([3001, 778, 21]), 1, 128 ** -0.5)
+    first = native.paged_attention(*args)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            again = native.paged_attention(*args)
+        side.synchronize()
+        assert torch.equal(first, again)
+
+
+def test_a_device_that_is_not_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    q = torch.randn(3, 4, 64, device="cuda:1").to(BF16)
+    k = torch.randn(30, 2, 64, device="cuda:1").to(BF16)
+    got = native.window_attention(q, k, k, 0.125, 10)
+    assert got.device == q.device and torch.cuda.current_device() == 0
+
+
+def test_wrong_arguments_are_refused():
+    q = torch.zeros(4, 8, 128, dtype=BF16, device="cuda")
+    c = torch.zeros(6, 16, 2, 128, dtype=BF16, device="cuda")
+    t, cu, seq = _ints([[0, 1], [2, 3]]), _ints([0, 2, 4]), _ints([20, 20])
+    ok = dict(q=q, k_cache=c, v_cache=c, block_table=t, cu_new=cu, seq_len=seq, max_new=2, softmax_scale=0.1)
+    native.paged_attention(ok.pop("q"), **ok)
+    for change in (dict(q=q.half()), dict(k_cache=c.half()), dict(q=q[:, :7]), dict(q=q.float()), dict(cu_new=_ints([0, 4])),
+                   dict(cu_new=cu.long()), dict(seq_len=seq.cpu()), dict(block_table=t[:1]), dict(block_table=t.t()),
+                   dict(max_new=0), dict(softmax_scale=float("nan")), dict(softmax_scale=-1.0), dict(window=-1), dict(sinks=-1),
+                   dict(k_cache=c[:, :10], v_cache=c[:, :10]), dict(k_cache=c[..., :96], v_cache=c[..., :96]),
+                   dict(out=torch.zeros(4, 8, 64, dtype=BF16, device="cuda")), dict(q=q[..., ::2]),
+                   dict(k_cache=c[..., 4:68], v_cache=c[..., 4:68], q=q[..., :64])):
+        with pytest.raises(native.SpfError):
+            native.paged_attention(change.pop("q", q), **{**ok, **change})
+    with pytest.raises(native.SpfError):
+        native.window_attention(q, c[0], c[0][:8], 0.1, 4)
+    with pytest.raises(native.SpfError):
+        native.window_attention(q, c[0, :3], c[0, :3], 0.1, 4)         # more queries than keys
+    with pytest.raises(native.SpfError):
+        native.paged_write(c[0], c[0], torch.zeros(15, dtype=torch.int64, device="cuda"), c, c)
+    with pytest.raises(native.SpfError):
+        native.paged_plan(seq, seq, t, seq, seq, -1, 16)
+    with pytest.raises(native.SpfError):
+        native.paged_plan(seq, seq, t, seq, seq, 40, 24)
+    empty = native.paged_attention(q[:0], c, c, t, _ints([0, 0, 0]), seq, 1, 0.1)
+    assert empty.shape == (0, 8, 128)

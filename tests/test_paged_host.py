@@ -1,0 +1,87 @@
+"""CPU-only checks of the paged and windowed entry points: what the C ABI and the binding refuse before anything is
+launched, and the 64-bit statement of the plan itself."""
+import pytest
+import torch
+
+import paged_reference as R
+from shareprefill_b200 import native
+
+PTR = 1 << 20      # never dereferenced: every call below is refused first
+
+
+def _attention(**kw):
+    a = dict(q=PTR, qn=1024, qh=128, rows=4, heads=8, k=PTR, kp=4096, kt=256, kh=128, v=PTR, vp=4096, vt=256, vh=128, pages=9,
+             page=16, kv=2, dim=128, dtype=0, table=PTR, ts=4, tw=4, cu=PTR, seq=PTR, req=2, most=1, scale=0.1, window=0, sinks=0,
+             out=PTR, scratch=PTR, bytes=1, stream=None)
+    assert set(kw) <= set(a)
+    return native.load().spf_paged_attention(*{**a, **kw}.values())
+
+
+def test_paged_attention_refusals():
+    assert _attention(rows=0) == 0
+    for name in ("q", "k", "v", "table", "cu", "seq", "out", "scratch"):
+        assert _attention(**{name: None}) == -1, name
+    for bad in (dict(dim=96), dict(heads=7), dict(kv=0), dict(page=24), dict(page=8), dict(page=512), dict(page=0)):
+        assert _attention(**bad) == -2, bad
+    for bad in (dict(q=PTR + 8), dict(k=PTR + 2), dict(out=PTR + 4), dict(scratch=PTR + 1), dict(qn=1020), dict(kt=252),
+                dict(vh=4), dict(vp=4097)):
+        assert _attention(**bad) == -3, bad
+    for bad in (dict(dtype=2), dict(dtype=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0),
+                dict(window=-1), dict(sinks=-1), dict(rows=-1), dict(pages=0), dict(req=0), dict(most=0), dict(tw=0), dict(ts=3),
+                dict(bytes=1)):
+        assert _attention(**bad) == -4, bad
+    for bad in (dict(heads=512, kv=2), dict(req=4097), dict(tw=1 << 27, ts=1 << 27), dict(rows=(1 << 30) + 1)):
+        assert _attention(**bad) == -6, bad
+
+
+def test_window_plan_and_write_refusals():
+    lib = native.load()
+
+    def window(new=4, keys=9, dim=128, n=1024, scale=0.1, bytes_=1):
+        return lib.spf_window_attention(PTR, n, 128, PTR, 256, 128, PTR, 256, 128, new, keys, 8, 2, dim, 0, scale, 4, 0, PTR, PTR,
+                                        bytes_, None)
+    assert window(new=0) == 0 and window(new=-1) == -4 and window(new=10) == -4 and window(dim=32) == -2
+    assert window(n=1023) == -3 and window(scale=-1.0) == -4 and window(keys=(1 << 30) + 1) == -6
+    assert window(bytes_=1) == -4       # scratch too small
+
+    def plan(req=2, page=16, ts=4, tw=4, cap=8, rows=4, cached=PTR):
+        return lib.spf_paged_plan(cached, PTR, req, page, PTR, ts, tw, PTR, cap, PTR, PTR, PTR, PTR, PTR, PTR, PTR, rows, None)
+    assert plan(cached=None) == -1 and plan(page=48) == -2 and plan(req=0) == -4 and plan(req=4097) == -6
+    assert plan(ts=3) == -4 and plan(tw=0) == -4 and plan(cap=0) == -4 and plan(rows=-1) == -4
+
+    def write(rows=4, dim=128, page=16, pages=3, slot=PTR, kc=PTR):
+        return lib.spf_paged_write(PTR, 256, 128, PTR, 256, 128, slot, rows, 2, dim, kc, 4096, 256, 128, PTR, 4096, 256, 128,
+                                   pages, page, None)
+    assert write(rows=0) == 0 and write(slot=None) == -1 and write(dim=72) == -2 and write(page=20) == -2
+    assert write(pages=0) == -4 and write(rows=-1) == -4 and write(kc=PTR + 8) == -3
+
+
+def test_scratch_grows_with_the_tile_not_with_the_lengths():
+    lib = native.load()
+    one, many = lib.spf_paged_scratch_bytes(1, 32, 8, 128), lib.spf_paged_scratch_bytes(1 << 20, 32, 8, 128)
+    assert 0 < one <= 16 << 20 and 0 < many <= 64 << 20
+    assert lib.spf_paged_scratch_bytes(0, 32, 8, 128) == 0 and lib.spf_paged_scratch_bytes(1, 32, 5, 128) == 0
+
+
+def test_binding_refuses_cpu_tensors():
+    q, c, i = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: native.paged_attention(q, c, c, i[:, None], i, i, 1, 0.1), lambda: native.window_attention(q, q, q, 0.1, 4),
+                 lambda: native.paged_write(q, q, i.long(), c, c), lambda: native.paged_plan(i, i, i[:, None], i, i, 4, 16)):
+        with pytest.raises(native.SpfError, match="CUDA"):
+            call()
+
+
+def test_statement_of_the_plan():
+    p = R.plan([15, 0, 16], [2, 40, 0], [[4, -1, -1], [-1] * 3, [6, -1, -1]], 3, [9, 8, 7, 5], 3, 3, 44, 16)
+    assert p["table"] == [[4, 5, -1], [-1, -1, -1], [6, -1, -1]]        # the second lacks three pages, two are left
+    assert p["refused"] == [0, 1, 0] and p["seq_len"] == [17, 0, 16] and p["cu_new"] == [0, 2, 42, 42]
+    assert p["slot_map"] == [4 * 16 + 15, 5 * 16] + [-1] * 42 and p["ring_state"] == [0, 2]
+
+
+def test_statement_of_the_attention():
+    q, k = torch.randn(3, 2, 8), torch.randn(5, 1, 8)
+    v = torch.randn(5, 1, 8)
+    out, _ = R.attention(q, k, v, 2, 0.3, window=1)
+    assert torch.allclose(out, v[2:].double().expand(-1, 2, -1))       # a window of one: the token's own value
+    out, _ = R.attention(q, k, v, 2, 0.3, present=torch.zeros(5, dtype=torch.bool))
+    assert bool((out == 0).all())
