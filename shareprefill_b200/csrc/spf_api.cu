@@ -400,13 +400,17 @@ static int check_ragged(int n_q_heads, int n_kv_heads, int head_dim, int dtype, 
   return SPF_OK;
 }
 
-// how the work of a call is cut (tile_rows, units, CTAs); the scratch follows from it
-static void ragged_config(RaggedParams& p) { ragged_rows_config(p); }
+// Items of up to 16 rows go to the bandwidth-bound kernel, more to the tcgen05 one, unless TMA cannot describe the
+// tensors (strides of 0 in expanded views).
+static bool few_rows(int group, int max_new) { return int64_t(group) * max_new <= 16; }
 
-static int run_ragged(RaggedParams& p, int head_dim, int64_t scratch_bytes, cudaStream_t st) {
+static int run_ragged(RaggedParams& p, int max_new, int head_dim, int64_t scratch_bytes, cudaStream_t st) {
+  const bool tc5 = !few_rows(p.group, max_new) && ragged_tc5_describable(p);
+  if (tc5) ragged_tc5_config(p); else ragged_rows_config(p);
+  if (tc5 && timeouts_tripped()) return SPF_ERR_TIMEOUT;
   if (scratch_bytes < ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim)) return SPF_ERR_RANGE;
   int rc = ragged_schedule(p, st);
-  if (rc == SPF_OK) rc = ragged_rows_attention(p, head_dim, st);
+  if (rc == SPF_OK) rc = tc5 ? ragged_tc5_attention(p, head_dim, st) : ragged_rows_attention(p, head_dim, st);
   if (rc == SPF_OK) rc = ragged_merge(p, head_dim, st);
   return rc;
 }
@@ -415,8 +419,12 @@ int64_t spf_paged_scratch_bytes(int max_new, int n_q_heads, int n_kv_heads, int 
   if (max_new <= 0 || check_ragged(n_q_heads, n_kv_heads, head_dim, SPF_BF16, 1.0, 0, 0) != SPF_OK) return 0;
   RaggedParams p;
   p.group = n_q_heads / n_kv_heads;
-  ragged_config(p);
-  return ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim);
+  ragged_rows_config(p);
+  const int64_t rows = ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim);
+  if (few_rows(p.group, max_new)) return rows;
+  ragged_tc5_config(p);
+  const int64_t tc5 = ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim);
+  return tc5 > rows ? tc5 : rows;
 }
 
 int spf_paged_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, int n_rows, int n_q_heads,
@@ -452,8 +460,7 @@ int spf_paged_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, i
   p.window = window < SPF_MAX_KEYS ? window : 0; p.sinks = sinks < SPF_MAX_KEYS ? sinks : SPF_MAX_KEYS;
   p.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   p.fp16 = dtype == SPF_FP16; p.scratch = static_cast<char*>(scratch);
-  ragged_config(p);
-  return run_ragged(p, head_dim, scratch_bytes, static_cast<cudaStream_t>(stream));
+  return run_ragged(p, max_new, head_dim, scratch_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int spf_window_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k, int64_t k_stride_n,
@@ -480,25 +487,24 @@ int spf_window_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, 
   p.window = window < SPF_MAX_KEYS ? window : 0; p.sinks = sinks < SPF_MAX_KEYS ? sinks : SPF_MAX_KEYS;
   p.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   p.fp16 = dtype == SPF_FP16; p.scratch = static_cast<char*>(scratch);
-  ragged_config(p);
-  return run_ragged(p, head_dim, scratch_bytes, static_cast<cudaStream_t>(stream));
+  return run_ragged(p, n_new, head_dim, scratch_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int spf_device_timeouts(void) {
-  const unsigned int n = tc5_timeout_count() + est_tc5_timeout_count();
+  const unsigned int n = tc5_timeout_count() + est_tc5_timeout_count() + ragged_tc5_timeout_count();
   g_known_timeouts.store(n, std::memory_order_relaxed);
   return static_cast<int>(n);
 }
 
 int spf_reset_device_timeouts(void) {
-  if (!tc5_reset_timeouts() || !est_tc5_reset_timeouts()) return SPF_ERR_LAUNCH;
+  if (!tc5_reset_timeouts() || !est_tc5_reset_timeouts() || !ragged_tc5_reset_timeouts()) return SPF_ERR_LAUNCH;
   g_known_timeouts.store(0, std::memory_order_relaxed);
   return SPF_OK;
 }
 
 int spf_set_device_wait_limit_ns(uint64_t ns) {
   if (ns == 0) return SPF_ERR_RANGE;
-  return (tc5_set_wait_limit(ns) && est_tc5_set_wait_limit(ns)) ? SPF_OK : SPF_ERR_LAUNCH;
+  return (tc5_set_wait_limit(ns) && est_tc5_set_wait_limit(ns) && ragged_tc5_set_wait_limit(ns)) ? SPF_OK : SPF_ERR_LAUNCH;
 }
 
 int spf_force_generic_kernels(int attention, int profile) {

@@ -108,15 +108,14 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
   if (s.first > per) return;                   // an earlier CTA starts inside this item too
   const int last = c + (s.item_units - s.first + per - 1) / per - 1;
   const RaggedReq q = ragged_req(p, s.req);
-  const int kvh = s.head / p.head_chunks, h0 = (s.head % p.head_chunks) * p.chunk_heads;
-  const int heads = min(p.chunk_heads, p.group - h0);
-  const int rows = min(p.tile_tokens, q.n - s.tile * p.tile_tokens) * heads;
-  const int64_t stride = ragged_partial_floats(p.tile_rows, D);
-  const float* parts = reinterpret_cast<const float*>(p.scratch + ragged_starts_bytes(p.n_ctas));
-  auto part = [&](int i) { return parts + (i < 0 ? 2 * int64_t(c - 1) + 1 : 2 * int64_t(c + i)) * stride; };
+  const RaggedItem item = ragged_item(p, q, s.head, s.tile);
+  auto part = [&](int i) { return ragged_part(p, i < 0 ? c - 1 : c + i, i < 0 ? 1 : 0, D); };
   const int n = last - c + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int row = blockIdx.y * (MRG_NT / 32) + warp; row < rows; row += gridDim.y * (MRG_NT / 32)) {
+  for (int row = blockIdx.y * (MRG_NT / 32) + warp; row < p.tile_rows; row += gridDim.y * (MRG_NT / 32)) {
+    const int in_stream = row % p.stream_rows, t = in_stream / p.chunk_heads, h = in_stream - t * p.chunk_heads;
+    const int tok = row / p.stream_rows * p.stream_tokens + t;
+    if (t >= p.stream_tokens || tok >= item.n_tok || h >= item.heads) continue;
     float top = -INFINITY;
     for (int i = lane - 1; i < n; i += 32) top = fmaxf(top, part(i)[row]);
     top = warp_max(top);
@@ -137,9 +136,7 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
       }
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    const int64_t tok = q.row0 + s.tile * p.tile_tokens + row / heads;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) +
-                    (tok * p.n_q_heads + kvh * p.group + h0 + row % heads) * D + lane * PER);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D) + lane * PER);
 #pragma unroll
     for (int e = 0; e < PER; e += 2) dst[e >> 1] = pack_half2<FP16>(acc[e] * inv, acc[e + 1] * inv);
   }
@@ -195,32 +192,32 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
   while (true) {
     const RaggedSpan span = ragged_span(p, q, tile);
     const int units = min(left, span.total - first);
-    const int kvh = head / p.head_chunks, h0 = (head % p.head_chunks) * p.chunk_heads;
-    const int heads = min(p.chunk_heads, p.group - h0);
-    const int tok0 = tile * p.tile_tokens, rows = min(p.tile_tokens, q.n - tok0) * heads;
-    const int pos0 = q.seq - q.n + tok0;
+    const RaggedItem item = ragged_item(p, q, head, tile);
+    const int kvh = item.kvh, h0 = item.h0, tok0 = item.tok0, pos0 = item.pos0;
     const uint16_t* kb = static_cast<const uint16_t*>(p.k) + kvh * p.k_sh;
     const uint16_t* vb = static_cast<const uint16_t*>(p.v) + kvh * p.v_sh;
     const int32_t* table = p.table ? p.table + req * p.table_stride : nullptr;
 
     // the item's query rows as A fragments (rows past its end are zero)
     uint32_t qa[D / 16][4];
-    const int t_r0 = r0 / heads, t_r1 = r1 / heads;
+    const int t_r0 = r0 / p.chunk_heads, t_r1 = r1 / p.chunk_heads;
+    const int h_r0 = r0 - t_r0 * p.chunk_heads, h_r1 = r1 - t_r1 * p.chunk_heads;
+    const bool in0 = t_r0 < item.n_tok && h_r0 < item.heads, in1 = t_r1 < item.n_tok && h_r1 < item.heads;
     {
       const uint16_t* qb = static_cast<const uint16_t*>(p.q) + (int64_t(q.row0) + tok0) * p.q_sn +
                            int64_t(kvh * p.group + h0) * p.q_sh + cq;
-      const uint16_t* q0 = qb + t_r0 * p.q_sn + (r0 - t_r0 * heads) * p.q_sh;
-      const uint16_t* q1 = qb + t_r1 * p.q_sn + (r1 - t_r1 * heads) * p.q_sh;
+      const uint16_t* q0 = qb + t_r0 * p.q_sn + h_r0 * p.q_sh;
+      const uint16_t* q1 = qb + t_r1 * p.q_sn + h_r1 * p.q_sh;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        qa[ks][0] = r0 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16)) : 0u;
-        qa[ks][1] = r1 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16)) : 0u;
-        qa[ks][2] = r0 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16 + 8)) : 0u;
-        qa[ks][3] = r1 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16 + 8)) : 0u;
+        qa[ks][0] = in0 ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16)) : 0u;
+        qa[ks][1] = in1 ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16)) : 0u;
+        qa[ks][2] = in0 ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16 + 8)) : 0u;
+        qa[ks][3] = in1 ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16 + 8)) : 0u;
       }
     }
     // row r sees keys <= hi that are >= lo or < sinks (rows past the item's end: none)
-    const int hi0 = r0 < rows ? pos0 + t_r0 : -1, hi1 = r1 < rows ? pos0 + t_r1 : -1;
+    const int hi0 = in0 ? pos0 + t_r0 : -1, hi1 = in1 ? pos0 + t_r1 : -1;
     const int lo0 = p.window > 0 ? hi0 - p.window + 1 : 0, lo1 = p.window > 0 ? hi1 - p.window + 1 : 0;
     // keys in [all_lo, all_hi] are seen by every row of the item
     const int all_hi = pos0, all_lo = p.window > 0 ? pos0 + p.tile_tokens - p.window : 0;
@@ -352,10 +349,10 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     __syncthreads();
     const float* all = reinterpret_cast<const float*>(rsm);
     const bool whole = units == span.total;
-    float* part = reinterpret_cast<float*>(p.scratch + ragged_starts_bytes(p.n_ctas)) +
-                  (2 * int64_t(blockIdx.x) + (first == 0 ? 1 : 0)) * ragged_partial_floats(RR_ROWS, D);
-    for (int idx = threadIdx.x; idx < rows * (D / 2); idx += RR_NT) {
-      const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
+    float* part = ragged_part(p, blockIdx.x, first == 0 ? 1 : 0, D);
+    for (int idx = threadIdx.x; idx < item.n_tok * p.chunk_heads * (D / 2); idx += RR_NT) {
+      const int r = idx / (D / 2), d = (idx % (D / 2)) * 2, t = r / p.chunk_heads, h = r - t * p.chunk_heads;
+      if (h >= item.heads) continue;
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < RR_NW; ++w) top = fmaxf(top, all[w * WSTRIDE + 16 * D + r]);
@@ -370,9 +367,7 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
       }
       if (whole) {
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        const int64_t tok = int64_t(q.row0) + tok0 + r / heads;
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) +
-                                     (tok * p.n_q_heads + kvh * p.group + h0 + r % heads) * D + d) =
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, t, h, D) + d) =
             pack_half2<FP16>(x * inv, y * inv);
       } else {
         *reinterpret_cast<float2*>(part + 2 * RR_ROWS + r * D + d) = make_float2(x, y);
@@ -392,7 +387,8 @@ void ragged_rows_config(RaggedParams& p) {
   p.tile_rows = RR_ROWS;
   p.head_chunks = ceil_div(p.group, RR_ROWS);
   p.chunk_heads = ceil_div(p.group, p.head_chunks);
-  p.tile_tokens = RR_ROWS / p.chunk_heads;
+  p.stream_rows = RR_ROWS;
+  p.tile_tokens = p.stream_tokens = RR_ROWS / p.chunk_heads;
   p.unit_keys = RR_TT * RR_NW;
   p.n_ctas = 2 * 148;
 }

@@ -5,7 +5,7 @@
 // o = softmax(scale * q k^T) v over the seen keys, zeros if there is none.
 //
 // Work is cut twice.  An ITEM is a tile of packed query rows (tile_tokens consecutive tokens x the query
-// heads that share a KV head, row = token * heads + head) of one request and one KV head; its cost is the
+// heads that share a KV head, row = token * chunk_heads + head) of one request and one KV head; its cost is the
 // number of UNITS (unit_keys consecutive keys) that any of its rows sees.  All units of all items form
 // one line, which is cut into equal pieces, one per CTA: a CTA runs through the end of one item, whole
 // items, and the start of another.  Whole items are written to the output, the two broken ones leave
@@ -34,7 +34,8 @@ struct RaggedParams {
   int fp16;
   // how the work is cut
   int head_chunks, chunk_heads;              // a KV head's group as head_chunks pieces of at most chunk_heads heads
-  int tile_rows, tile_tokens, unit_keys, n_ctas;
+  int stream_rows, stream_tokens;            // an item's rows come in streams (one MMA tile each) of stream_tokens tokens
+  int tile_rows, tile_tokens, unit_keys, n_ctas;   // tile_rows / stream_rows streams an item
   char* scratch;
 };
 
@@ -94,6 +95,27 @@ __device__ __forceinline__ bool ragged_next(const RaggedParams& p, int& req, int
   return false;
 }
 
+// an item's place in the tensors
+struct RaggedItem { int kvh, h0, heads, tok0, n_tok, pos0; };   // first head of the chunk (in its group), heads and tokens there are
+__device__ __forceinline__ RaggedItem ragged_item(const RaggedParams& p, const RaggedReq& q, int head, int tile) {
+  RaggedItem t;
+  t.kvh = head / p.head_chunks;
+  t.h0 = (head - t.kvh * p.head_chunks) * p.chunk_heads;
+  t.heads = min(p.chunk_heads, p.group - t.h0);
+  t.tok0 = tile * p.tile_tokens;
+  t.n_tok = min(p.tile_tokens, q.n - t.tok0);
+  t.pos0 = q.seq - q.n + t.tok0;
+  return t;
+}
+// offset of (token of the item, head of the chunk) in `out`, in elements
+__device__ __forceinline__ int64_t ragged_out(const RaggedParams& p, const RaggedReq& q, const RaggedItem& t, int tok, int h, int d) {
+  return ((int64_t(q.row0) + t.tok0 + tok) * p.n_q_heads + t.kvh * p.group + t.h0 + h) * d;
+}
+__device__ __forceinline__ float* ragged_part(const RaggedParams& p, int cta, int which, int d) {
+  return reinterpret_cast<float*>(p.scratch + ragged_starts_bytes(p.n_ctas)) +
+         (2 * int64_t(cta) + which) * ragged_partial_floats(p.tile_rows, d);
+}
+
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   if (FP16) {
@@ -110,5 +132,12 @@ int ragged_merge(const RaggedParams& p, int head_dim, cudaStream_t st);
 // up to 16 packed rows an item: bandwidth bound (single tokens); also what TMA cannot describe
 void ragged_rows_config(RaggedParams& p);
 int ragged_rows_attention(const RaggedParams& p, int head_dim, cudaStream_t st);
+// items of two 128-row MMA tiles on tcgen05 (spf_ragged_tc5.cu); SPF_ERR_SHAPE where TMA cannot describe the tensors
+void ragged_tc5_config(RaggedParams& p);
+bool ragged_tc5_describable(const RaggedParams& p);
+int ragged_tc5_attention(const RaggedParams& p, int head_dim, cudaStream_t st);
+unsigned int ragged_tc5_timeout_count();
+bool ragged_tc5_reset_timeouts();
+bool ragged_tc5_set_wait_limit(unsigned long long ns);
 
 }  // namespace spf

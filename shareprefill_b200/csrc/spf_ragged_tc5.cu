@@ -1,0 +1,597 @@
+// Ragged attention over a paged or contiguous KV cache on the 5th-generation tensor cores (tcgen05 + TMEM +
+// TMA): items of two 128-row MMA tiles (see spf_ragged.cuh for items, units and how the line of units is cut).
+//
+// One persistent CTA per SM.  The two tiles of an item ("stream A / B": consecutive tokens x the heads of one KV
+// head) share every K/V unit of 128 keys.
+//
+//   warp 0      producer: the item's Q tiles, then K and V units through a K ring and a V ring by TMA; a unit of
+//               pages smaller than 128 tokens is one copy per page and 64 columns, issued by as many lanes, and a
+//               page that is not there is a copy from behind the pool, which fills zeros
+//   warps 1, 2  MMA issuers of the streams: S = Q K^T and O += P V (P from TMEM); the steps of the two leave in turn
+//               (a token goes back and forth), so that one stream's softmax runs under the other's products
+//   warp 3      rows of a V unit that no query of the item sees are set to zero before the unit is used: what lies
+//               behind the sequence, between the sinks and the window, or in the future may hold NaN, and 0 * NaN
+//               would reach the output (scores of such keys are replaced, so K needs no such care)
+//   warps 4-7, 8-11  softmax of stream A, B: a thread owns a row; base-2 softmax in fp32 against a reference
+//               point that is fixed by the first unit in which the row sees a key and moved only when a unit's
+//               sum overflows its limit; P rounded to the inputs' type; the epilogue writes the row
+//
+// The rings, S and P run on across items; Q is loaded as soon as the previous item's last Q K^T is done.
+// Every wait is bounded (spf_tc5.cuh).
+#include "spf_ragged.cuh"
+#include "spf_tc5.cuh"
+
+namespace spf {
+
+constexpr int RT_THREADS = 384, RT_CTAS = 148, RT_UNIT = 128, RT_ROWS = 128;
+constexpr int RT_REGS_CONTROL = 104, RT_REGS_SOFTMAX = 200;
+static_assert(4 * RT_REGS_CONTROL + 8 * RT_REGS_SOFTMAX <= 12 * 168, "setmaxnreg targets exceed the CTA's register pool");
+constexpr uint32_t RT_SLAB = 128 * 128;              // [128 rows][64 elements]
+constexpr uint32_t RT_CTRL = 2048;
+constexpr int RT_ABSENT = 16;                        // units whose absent pages are remembered
+
+template <int D>
+struct RtCfg {
+  static constexpr int SLABS = D / 64, KSTEPS = D / 16;
+  static constexpr uint32_t TILE = RT_SLAB * SLABS;
+  static constexpr int KST = D == 128 ? 3 : 6, VST = D == 128 ? 2 : 5;
+  // barriers
+  static constexpr int B_QFULL = 0, B_QEMPTY = 1, B_KFULL = 2, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
+                       B_VREADY = B_VFULL + VST, B_VEMPTY = B_VREADY + VST, B_SFULL = B_VEMPTY + VST, B_PREADY = B_SFULL + 2,
+                       B_ODONE = B_PREADY + 2, B_TOKEN = B_ODONE + 2, B_N = B_TOKEN + 2;
+  static constexpr uint32_t O_TMEM = B_N * 8, O_ABORT = O_TMEM + 8, O_ABSENT = O_ABORT + 8,
+                            O_DTAB = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u;
+  static constexpr int DT_K = 16, DT_V = DT_K + 8 * KST, DT_N = DT_V + 8 * VST;   // descriptors: 8 per tile, Q_A, Q_B, K.., V..
+  static_assert(O_DTAB + DT_N * 8 <= RT_CTRL, "control region too small");
+  static_assert(DT_N <= RT_THREADS, "a thread per descriptor");
+  static constexpr uint32_t O_Q = RT_CTRL, O_K = O_Q + 2 * TILE, O_V = O_K + KST * TILE, BYTES = O_V + VST * TILE;
+  static_assert(BYTES <= 227 * 1024, "shared memory");
+};
+
+// fp32 accumulation, M = 128; B is MN-major for the product with V
+constexpr uint32_t rt_idesc(bool fp16, int n, bool mn) {
+  return (1u << 4) | (fp16 ? 0u : (1u << 7) | (1u << 10)) | (mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+
+struct RtSteps { uint64_t d[8]; };
+// S = Q K^T: all descriptors are registers before the first MMA, so that the group leaves back to back
+template <int KSTEPS>
+__device__ __forceinline__ void rt_mma_qk(uint32_t s_tmem, const RtSteps& a, const RtSteps& b, uint32_t idesc) {
+  if (KSTEPS == 8) {
+    asm volatile(
+        "{\n\t.reg .pred pz, po;\n\tsetp.ne.b32 pz, 0, 0;\n\tsetp.eq.b32 po, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %2, %10, %1, pz;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %3, %11, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %4, %12, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %13, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %6, %14, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %7, %15, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %8, %16, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %9, %17, %1, po;\n\t}"
+        ::"r"(s_tmem), "r"(idesc),
+          "l"(a.d[0]), "l"(a.d[1]), "l"(a.d[2]), "l"(a.d[3]), "l"(a.d[4]), "l"(a.d[5]), "l"(a.d[6]), "l"(a.d[7]),
+          "l"(b.d[0]), "l"(b.d[1]), "l"(b.d[2]), "l"(b.d[3]), "l"(b.d[4]), "l"(b.d[5]), "l"(b.d[6]), "l"(b.d[7])
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred pz, po;\n\tsetp.ne.b32 pz, 0, 0;\n\tsetp.eq.b32 po, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %2, %6, %1, pz;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %3, %7, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %4, %8, %1, po;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %9, %1, po;\n\t}"
+        ::"r"(s_tmem), "r"(idesc), "l"(a.d[0]), "l"(a.d[1]), "l"(a.d[2]), "l"(a.d[3]),
+          "l"(b.d[0]), "l"(b.d[1]), "l"(b.d[2]), "l"(b.d[3])
+        : "memory");
+  }
+}
+// O (+)= P V, P at p_tmem + 8 i (16 packed columns per step)
+__device__ __forceinline__ void rt_mma_pv(uint32_t o_tmem, uint32_t p_tmem, const RtSteps& v, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred pa, po;\n\tsetp.ne.b32 pa, %2, 0;\n\tsetp.eq.b32 po, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], %11, %1, pa;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], %12, %1, po;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %13, %1, po;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %14, %1, po;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%7], %15, %1, po;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%8], %16, %1, po;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%9], %17, %1, po;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%10], %18, %1, po;\n\t}"
+      ::"r"(o_tmem), "r"(idesc), "r"(acc),
+        "r"(p_tmem), "r"(p_tmem + 8u), "r"(p_tmem + 16u), "r"(p_tmem + 24u), "r"(p_tmem + 32u), "r"(p_tmem + 40u),
+        "r"(p_tmem + 48u), "r"(p_tmem + 56u),
+        "l"(v.d[0]), "l"(v.d[1]), "l"(v.d[2]), "l"(v.d[3]), "l"(v.d[4]), "l"(v.d[5]), "l"(v.d[6]), "l"(v.d[7])
+      : "memory");
+}
+
+// columns [a, b) are masked out
+__device__ __forceinline__ void mask_between(uint32_t (&r)[32], int a, int b) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j >= a && j < b) r[j] = 0xff800000u;
+}
+
+// The parts of items that a CTA runs through, in order; every role of the CTA walks them for itself.
+struct RtWalker {
+  int req, head, tile, first, left, units;
+  RaggedReq q;
+  RaggedItem item;
+  RaggedSpan span;
+  __device__ void enter(const RaggedParams& p) {
+    item = ragged_item(p, q, head, tile);
+    span = ragged_span(p, q, tile);
+    units = min(left, span.total - first);
+  }
+  __device__ bool begin(const RaggedParams& p, const RaggedStart& s) {
+    req = s.req; head = s.head; tile = s.tile; first = s.first; left = s.units;
+    if (left <= 0) return false;
+    q = ragged_req(p, req);
+    enter(p);
+    return true;
+  }
+  __device__ bool next(const RaggedParams& p) {
+    left -= units;
+    first = 0;
+    if (left <= 0 || !ragged_next(p, req, head, tile, q)) return false;
+    enter(p);
+    return true;
+  }
+  __device__ int key0(int u) const {
+    const int s = first + u;
+    return (s < span.sink_units ? s : span.win_first + s - span.sink_units) * RT_UNIT;
+  }
+  __device__ bool both(const RaggedParams& p) const { return item.n_tok > p.stream_tokens; }
+  __device__ bool whole() const { return units == span.total; }
+};
+
+template <int D, bool FP16>
+__global__ void __launch_bounds__(RT_THREADS, 1)
+ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RaggedParams p) {
+  using C = RtCfg<D>;
+  if (*reinterpret_cast<volatile unsigned int*>(&g_tc5_timeouts) > 16u) return;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t sbase = smem_addr(smem);
+  if (sbase & 1023u) {
+    if (threadIdx.x == 0) atomicAdd(&g_tc5_timeouts, 1000u);
+    return;
+  }
+  const RaggedStart start = reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
+  if (start.units == 0) return;
+  auto bar = [&](int b) { return sbase + 8u * uint32_t(b); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::O_TMEM);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::O_ABORT);
+  volatile uint32_t* absent_of = reinterpret_cast<volatile uint32_t*>(smem + C::O_ABSENT);
+  uint64_t* dtab = reinterpret_cast<uint64_t*>(smem + C::O_DTAB);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 32) { tma_prefetch_map(&map_q); tma_prefetch_map(&map_k); tma_prefetch_map(&map_v); }
+  if (tid == 0) {
+    mbar_init(bar(C::B_QFULL), 1); mbar_init(bar(C::B_QEMPTY), 2);
+    for (int s = 0; s < C::KST; ++s) { mbar_init(bar(C::B_KFULL + s), 1); mbar_init(bar(C::B_KEMPTY + s), 2); }
+    for (int s = 0; s < C::VST; ++s) {
+      mbar_init(bar(C::B_VFULL + s), 1); mbar_init(bar(C::B_VREADY + s), 1); mbar_init(bar(C::B_VEMPTY + s), 2);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(bar(C::B_SFULL + h), 1); mbar_init(bar(C::B_PREADY + h), 128); mbar_init(bar(C::B_ODONE + h), 1);
+      mbar_init(bar(C::B_TOKEN + h), 1);
+    }
+    mbar_arrive(bar(C::B_TOKEN));     // stream A's thread goes first
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (tid >= RT_THREADS - C::DT_N) {
+    const int e = tid - (RT_THREADS - C::DT_N), ks = e & 7;
+    const uint64_t kstep = uint64_t(uint32_t(ks >> 2) * (RT_SLAB >> 4) + uint32_t(ks & 3) * (32u >> 4));
+    if (e < C::DT_K) dtab[e] = desc_kmajor(sbase + C::O_Q + uint32_t(e >> 3) * C::TILE) + kstep;
+    else if (e < C::DT_V) dtab[e] = desc_kmajor(sbase + C::O_K + uint32_t((e - C::DT_K) >> 3) * C::TILE) + kstep;
+    else dtab[e] = desc_mnmajor(sbase + C::O_V + uint32_t((e - C::DT_V) >> 3) * C::TILE) + uint64_t(uint32_t(ks) * (2048u >> 4));
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  RtWalker w = {};
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(RT_REGS_CONTROL));
+    if (warp == 0) {
+      // ---------------------------------------------------------- producer (whole warp; lane 0 waits and announces)
+      const int page = p.table ? 1 << p.page_shift : RT_UNIT;
+      const int box = min(page, RT_UNIT), per_unit = RT_UNIT / box;      // rows of a copy, copies of a unit and 64 columns
+      const int my_page = lane % per_unit, my_slab = lane / per_unit;
+      const bool copies = my_slab < C::SLABS;
+      const uint32_t my_dst = uint32_t(my_slab) * RT_SLAB + uint32_t(my_page * box) * 128u;
+      const uint32_t q_bytes = uint32_t(p.stream_tokens * p.chunk_heads) * 128u * C::SLABS;
+      auto wait0 = [&](int b, int parity) {
+        bool ok = true;
+        if (lane == 0) ok = mbar_wait(bar(b), parity, abort_flag);
+        return __shfl_sync(0xffffffffu, ok, 0);
+      };
+      // this lane's page of unit u (the id; n_pages - behind the pool, zeros - where there is none)
+      auto page_of = [&](int u) {
+        if (!p.table || u >= w.units) return 0;
+        const int key = w.key0(u) + my_page * box;
+        if (key >= w.span.keys) return p.n_pages;
+        const int id = __ldg(p.table + w.req * p.table_stride + (key >> p.page_shift));
+        return id >= 0 && id < p.n_pages ? id : p.n_pages;
+      };
+      auto load = [&](const CUtensorMap* map, int full, uint32_t tile, int key, int id, int kvh) {
+        if (lane == 0) mbar_expect_tx(bar(full), C::TILE);
+        __syncwarp();
+        if (copies) tma_load_4d(tile + my_dst, map, bar(full), my_slab * 64, p.table ? key & (page - 1) & ~(box - 1) : key, kvh, id);
+      };
+      int k_i = 0, v_i = 0, v_key = 0, v_id = 0, v_kvh = 0, pieces = 0;
+      bool ok = true;
+      auto load_v = [&]() {      // K runs one unit ahead of V
+        const int s = v_i % C::VST;
+        if (!wait0(C::B_VEMPTY + s, ((v_i / C::VST) & 1) ^ 1)) return false;
+        load(&map_v, C::B_VFULL + s, sbase + C::O_V + uint32_t(s) * C::TILE, v_key, v_id, v_kvh);
+        ++v_i;
+        return true;
+      };
+      for (bool more = w.begin(p, start); ok && more; more = w.next(p), ++pieces) {
+        if (pieces > 0) ok = wait0(C::B_QEMPTY, (pieces - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          const int streams = w.both(p) ? 2 : 1;
+          mbar_expect_tx(bar(C::B_QFULL), uint32_t(streams) * q_bytes);
+          for (int h = 0; h < streams; ++h)
+            for (int s = 0; s < C::SLABS; ++s)
+              tma_load_3d(sbase + C::O_Q + uint32_t(h) * C::TILE + uint32_t(s) * RT_SLAB, &map_q, bar(C::B_QFULL), s * 64,
+                          w.item.kvh * p.group + w.item.h0, w.q.row0 + w.item.tok0 + h * p.stream_tokens);
+        }
+        int id = page_of(0);
+        for (int u = 0; u < w.units; ++u) {
+          const int key = w.key0(u), id_next = page_of(u + 1);
+          const int s = k_i % C::KST;
+          ok = wait0(C::B_KEMPTY + s, ((k_i / C::KST) & 1) ^ 1);
+          if (!ok) break;
+          // pages that the sequence should have here and has not: a bit per 16 keys
+          const unsigned gone = p.table ? __ballot_sync(0xffffffffu, lane < per_unit && id == p.n_pages) : 0u;
+          if (lane == 0) {
+            uint32_t bits = 0;
+            for (int g = 0; gone && g < per_unit; ++g)
+              if (gone >> g & 1u) bits |= ((1u << (box >> 4)) - 1u) << (g * (box >> 4));
+            absent_of[k_i % RT_ABSENT] = bits;
+            __threadfence_block();
+          }
+          load(&map_k, C::B_KFULL + s, sbase + C::O_K + uint32_t(s) * C::TILE, key, id, w.item.kvh);
+          ++k_i;
+          if (u > 0) ok = load_v();
+          if (!ok) break;
+          v_key = key; v_id = id; v_kvh = w.item.kvh;
+          id = id_next;
+        }
+        if (ok) ok = load_v();
+      }
+      // every copy that was started must have landed before the CTA may exit
+      if (lane == 0) {
+        if (pieces > 0) mbar_wait(bar(C::B_QFULL), (pieces - 1) & 1, abort_flag, true);
+        for (int j = max(0, k_i - C::KST); j < k_i; ++j) mbar_wait(bar(C::B_KFULL + j % C::KST), (j / C::KST) & 1, abort_flag, true);
+        for (int j = max(0, v_i - C::VST); j < v_i; ++j) mbar_wait(bar(C::B_VFULL + j % C::VST), (j / C::VST) & 1, abort_flag, true);
+      }
+    } else if (warp <= 2) {
+      // ---------------------------------------------------------- MMA issuers
+      if (lane == 0) {
+        const int h = warp - 1;
+        const uint32_t ts = tmem + (h == 0 ? 0u : 128u), to = tmem + 256u + uint32_t(h) * D;
+        constexpr uint32_t ID_QK = rt_idesc(FP16, 128, false), ID_PV = rt_idesc(FP16, D, true);
+        auto fetch = [&](int first, RtSteps& o) {
+          const ulonglong2* src = reinterpret_cast<const ulonglong2*>(dtab + first);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { const ulonglong2 t = src[j]; o.d[2 * j] = t.x; o.d[2 * j + 1] = t.y; }
+        };
+        int step = 0, i = 0, np = 0, pieces = 0, u = 0;
+        bool have = w.begin(p, start);
+        bool both = w.both(p), mine = h == 0 || both;
+        bool ok = mbar_wait(bar(C::B_QFULL), 0, abort_flag) && mbar_wait(bar(C::B_KFULL), 0, abort_flag);
+        auto release = [&](int b, bool used) { if (used) tc_commit(bar(b)); else mbar_arrive(bar(b)); };
+        if (ok) {
+          RtSteps qd, kd;
+          fetch(8 * h, qd); fetch(C::DT_K, kd);
+          if (both) ok = mbar_wait(bar(C::B_TOKEN + h), step & 1, abort_flag);
+          if (ok) {
+            if (mine) { tc_fence_after(); rt_mma_qk<C::KSTEPS>(ts, qd, kd, ID_QK); tc_commit(bar(C::B_SFULL + h)); }
+            if (both) { mbar_arrive(bar(C::B_TOKEN + (h ^ 1))); ++step; }
+            release(C::B_KEMPTY, mine);
+            if (w.units == 1) release(C::B_QEMPTY, mine);
+          }
+        }
+        while (ok && have) {
+          // unit i (P V) and the one after it (Q K^T), which may open the next item
+          const bool p_both = both, p_mine = mine, p_first = u == 0, p_last = u + 1 == w.units;
+          if (p_last) {
+            have = w.next(p);
+            u = 0; ++pieces;
+            if (have) { both = w.both(p); mine = h == 0 || both; }
+          } else {
+            ++u;
+          }
+          const int vs = i % C::VST, ks = (i + 1) % C::KST;
+          const bool q_last = have && u + 1 == w.units, q_mine = have && mine;
+          ok = mbar_wait(bar(C::B_VREADY + vs), (i / C::VST) & 1, abort_flag);
+          if (ok && have) {
+            if (p_last) ok = mbar_wait(bar(C::B_QFULL), pieces & 1, abort_flag);
+            if (ok) ok = mbar_wait(bar(C::B_KFULL + ks), ((i + 1) / C::KST) & 1, abort_flag);
+          }
+          if (!ok) break;
+          RtSteps vd, qd, kd;
+          if (p_mine) fetch(C::DT_V + 8 * vs, vd);
+          if (q_mine) { fetch(8 * h, qd); fetch(C::DT_K + 8 * ks, kd); }
+          if (p_both) ok = mbar_wait(bar(C::B_TOKEN + h), step & 1, abort_flag);
+          if (ok && p_mine) ok = mbar_wait(bar(C::B_PREADY + h), np & 1, abort_flag);
+          if (!ok) break;
+          if (p_mine || q_mine) tc_fence_after();
+          if (p_mine) {
+            rt_mma_pv(to, ts, vd, ID_PV, p_first ? 0u : 1u);
+            ++np;
+            if (p_last) tc_commit(bar(C::B_ODONE + h));
+          }
+          if (q_mine) { rt_mma_qk<C::KSTEPS>(ts, qd, kd, ID_QK); tc_commit(bar(C::B_SFULL + h)); }
+          if (p_both) { mbar_arrive(bar(C::B_TOKEN + (h ^ 1))); ++step; }
+          release(C::B_VEMPTY + vs, p_mine);
+          if (have) {
+            release(C::B_KEMPTY + ks, q_mine);
+            if (q_last) release(C::B_QEMPTY, q_mine);
+          }
+          ++i;
+        }
+      }
+    } else {
+      // ---------------------------------------------------------- V rows that no query of the item sees become zeros
+      bool ok = true;
+      int i = 0;
+      for (bool more = w.begin(p, start); ok && more; more = w.next(p)) {
+        const int low = p.window > 0 ? w.item.pos0 - p.window + 1 : 0;
+        for (int u = 0; u < w.units; ++u, ++i) {
+          const int s = i % C::VST;
+          ok = mbar_wait(bar(C::B_VFULL + s), (i / C::VST) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int key = w.key0(u);
+          const int tail = min(max(w.span.keys - key, 0), RT_UNIT);                                     // rows [tail, 128)
+          const int a = min(max(p.sinks - key, 0), RT_UNIT), b = min(max(low - key, 0), tail);          // and rows [a, b)
+          if (tail < RT_UNIT || a < b) {
+            const uint32_t base = sbase + C::O_V + uint32_t(s) * C::TILE;
+            for (int r = lane >> 3; r < RT_UNIT; r += 4)
+              if (r >= tail || (r >= a && r < b))
+#pragma unroll
+                for (int sl = 0; sl < C::SLABS; ++sl)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                               ::"r"(base + uint32_t(sl) * RT_SLAB + uint32_t(r) * 128u + uint32_t(lane & 7) * 16u), "r"(0) : "memory");
+            fence_proxy_async();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(bar(C::B_VREADY + s));
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax warpgroups
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(RT_REGS_SOFTMAX));
+    // P must stay inside its type's range: a unit's sum of P above this moves the reference point to the unit's maximum
+    constexpr float SUM_LIMIT = FP16 ? 32768.f : 1180591620717411303424.f;   // 2^15, 2^70
+    constexpr float MARGIN = FP16 ? 0.f : 64.f;
+    const int h = (warp - 4) >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int t_row = row / p.chunk_heads, h_row = row - t_row * p.chunk_heads;
+    const int tok = h * p.stream_tokens + t_row;                       // token of the item
+    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+    const uint32_t tS = tmem + lane_base + uint32_t(h * 128);
+    const uint32_t tO = tmem + lane_base + 256u + uint32_t(h) * D;
+    int i = 0, k = 0, done = 0;              // units of the CTA, units and items of this stream
+    bool ok = true;
+    for (bool more = w.begin(p, start); ok && more; more = w.next(p)) {
+      if (h == 1 && !w.both(p)) { i += w.units; continue; }
+      const bool in = t_row < p.stream_tokens && tok < w.item.n_tok && h_row < w.item.heads;
+      const int hi = in ? w.item.pos0 + tok : -1, lo = p.window > 0 ? hi - p.window + 1 : 0;
+      // units inside [fast_lo, fast_hi] are seen whole by every row of the stream
+      const int fast_hi = w.item.pos0 + h * p.stream_tokens;
+      const int fast_lo = p.window > 0 ? fast_hi + p.stream_tokens - p.window : 0;
+      float m_used = -INFINITY, l_sum = 0.f;
+      for (int u = 0; u < w.units; ++u, ++i, ++k) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_SFULL + h), k & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s0[32], s1[32], s2[32], s3[32];
+        tmem_ld32_raw(tS + 0, s0);
+        tmem_ld32_raw(tS + 32, s1);
+        tmem_ld32_raw(tS + 64, s2);
+        tmem_ld32_raw(tS + 96, s3);
+        const int key = w.key0(u);
+        const uint32_t gone = absent_of[i % RT_ABSENT];
+        tc_wait_ld();
+        const bool masked = key + RT_UNIT - 1 > fast_hi || key < fast_lo || gone != 0u;
+        if (masked) {
+          const int last = hi - key;
+          mask_after(s0, last); mask_after(s1, last - 32); mask_after(s2, last - 64); mask_after(s3, last - 96);
+          if (p.window > 0) {
+            const int a = max(p.sinks - key, 0), b = lo - key;
+            mask_between(s0, a, b); mask_between(s1, a - 32, b - 32); mask_between(s2, a - 64, b - 64); mask_between(s3, a - 96, b - 96);
+          }
+          if (gone != 0u) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (gone >> g & 1u) mask_between(s0, g * 16, g * 16 + 16);
+              if (gone >> (g + 2) & 1u) mask_between(s1, g * 16, g * 16 + 16);
+              if (gone >> (g + 4) & 1u) mask_between(s2, g * 16, g * 16 + 16);
+              if (gone >> (g + 6) & 1u) mask_between(s3, g * 16, g * 16 + 16);
+            }
+          }
+        }
+        auto row_max_log2 = [&]() {
+          return fmaxf(fmaxf(row_max(s0), row_max(s1)), fmaxf(row_max(s2), row_max(s3))) * p.scale_log2;
+        };
+        auto emit_p = [&]() {
+          const float ref = m_used == -INFINITY ? 0.f : m_used;
+          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+          uint32_t pk[16];
+          if (masked) {       // exact zeros where masked: the polynomial's range ends at 2^-57
+            exp_pack_poly<0, FP16>(s0, p.scale_log2, ref, pk, l0); tmem_st16(tS + 0, pk);
+            exp_pack_poly<0, FP16>(s1, p.scale_log2, ref, pk, l1); tmem_st16(tS + 16, pk);
+            exp_pack_poly<0, FP16>(s2, p.scale_log2, ref, pk, l2); tmem_st16(tS + 32, pk);
+            exp_pack_poly<0, FP16>(s3, p.scale_log2, ref, pk, l3); tmem_st16(tS + 48, pk);
+          } else {
+            exp_pack_poly<2, FP16>(s0, p.scale_log2, ref, pk, l0); tmem_st16(tS + 0, pk);
+            exp_pack_poly<2, FP16>(s1, p.scale_log2, ref, pk, l1); tmem_st16(tS + 16, pk);
+            exp_pack_poly<2, FP16>(s2, p.scale_log2, ref, pk, l2); tmem_st16(tS + 32, pk);
+            exp_pack_poly<2, FP16>(s3, p.scale_log2, ref, pk, l3); tmem_st16(tS + 48, pk);
+          }
+          return (l0 + l1) + (l2 + l3);
+        };
+        // a row's reference is the maximum of the first unit in which it sees a key (nothing was added before)
+        if (__any_sync(0xffffffffu, m_used == -INFINITY)) {
+          const float mb = row_max_log2();
+          if (m_used == -INFINITY) m_used = mb;
+        }
+        float blk = emit_p();
+        if (u > 0 && __any_sync(0xffffffffu, in && !(blk <= SUM_LIMIT))) {
+          tc_wait_st();
+          const float mb = row_max_log2();
+          float alpha = 1.f;
+          if (mb > m_used + MARGIN) {
+            alpha = exp2f(m_used - mb);
+            m_used = mb;
+            l_sum *= alpha;
+          }
+          // S of this unit is complete, hence so is every earlier P V of the stream: O is stable
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float v[32];
+            tmem_ld32(tO + c * 32, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= alpha;
+            tmem_st32(tO + c * 32, v);
+          }
+          blk = emit_p();
+        }
+        l_sum += blk;
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(C::B_PREADY + h));
+      }
+      // ---- epilogue: the row goes to the output, or with its statistics to the scratch
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_ODONE + h), done & 1, abort_flag));
+      ++done;
+      if (!ok) break;
+      tc_fence_after();
+      const bool seen = m_used != -INFINITY;
+      if (w.whole()) {
+        const float inv = seen && l_sum > 0.f ? 1.f / l_sum : 0.f;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (in ? ragged_out(p, w.q, w.item, tok, h_row, D) : 0);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          tmem_ld32(tO + c * 32, v);
+          if (in) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint4 x;
+              x.x = pack_half2<FP16>(v[8 * j] * inv, v[8 * j + 1] * inv); x.y = pack_half2<FP16>(v[8 * j + 2] * inv, v[8 * j + 3] * inv);
+              x.z = pack_half2<FP16>(v[8 * j + 4] * inv, v[8 * j + 5] * inv); x.w = pack_half2<FP16>(v[8 * j + 6] * inv, v[8 * j + 7] * inv);
+              *reinterpret_cast<uint4*>(dst + c * 32 + j * 8) = x;
+            }
+          }
+        }
+      } else {
+        float* part = ragged_part(p, blockIdx.x, w.first == 0 ? 1 : 0, D);
+        const int at = h * RT_ROWS + row;
+        if (in) { part[at] = m_used; part[2 * RT_ROWS + at] = l_sum; }
+        float* dst = part + 4 * RT_ROWS + at * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          tmem_ld32(tO + c * 32, v);
+          if (in) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float4*>(dst + c * 32 + j * 4) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+        }
+      }
+      tc_fence_before();     // the next item's first P (after its S) lets the next product overwrite O
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// ---------------------------------------------------------------- host side
+void ragged_tc5_config(RaggedParams& p) {
+  p.head_chunks = ceil_div(p.group, RT_ROWS);
+  p.chunk_heads = ceil_div(p.group, p.head_chunks);
+  p.stream_rows = RT_ROWS;
+  p.stream_tokens = RT_ROWS / p.chunk_heads;
+  p.tile_rows = 2 * RT_ROWS;
+  p.tile_tokens = 2 * p.stream_tokens;
+  p.unit_keys = RT_UNIT;
+  p.n_ctas = RT_CTAS;
+}
+
+static bool tma_stride(int64_t s) { return s > 0 && s * 2 < (int64_t(1) << 40); }
+
+// a stride of a dimension of extent one is never used and may be anything
+bool ragged_tc5_describable(const RaggedParams& p) {
+  const bool one_head = p.n_kv_heads == 1, one_page = p.n_pages == 1;
+  return (p.n_rows == 1 || tma_stride(p.q_sn)) && (p.n_q_heads == 1 || tma_stride(p.q_sh)) && tma_stride(p.k_st) && tma_stride(p.v_st) &&
+         (one_head || (tma_stride(p.k_sh) && tma_stride(p.v_sh))) && (!p.table || one_page || (tma_stride(p.k_sp) && tma_stride(p.v_sp)));
+}
+
+// K or V as (d, token of the page, head, page); contiguous keys are one page
+static bool rt_map_kv(CUtensorMap* m, const RaggedParams& p, const void* base, int64_t sp, int64_t st, int64_t sh, int d) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const int page = p.table ? 1 << p.page_shift : p.seq_one;
+  const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(page), cuuint64_t(p.n_kv_heads), cuuint64_t(p.n_pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(st) * 2, cuuint64_t(p.n_kv_heads == 1 ? d : sh) * 2,
+                                 cuuint64_t(!p.table || p.n_pages == 1 ? d : sp) * 2};
+  const cuuint32_t box[4] = {64, cuuint32_t(p.table && page < RT_UNIT ? page : RT_UNIT), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(m, p.fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
+            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Q as (d, head, token): a copy of chunk_heads x stream_tokens rows lands as one tile, token by token
+static bool rt_map_q(CUtensorMap* m, const RaggedParams& p, int d) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(p.n_q_heads), cuuint64_t(p.n_rows)};
+  const cuuint64_t strides[2] = {cuuint64_t(p.n_q_heads == 1 ? d : p.q_sh) * 2, cuuint64_t(p.n_rows == 1 ? d : p.q_sn) * 2};
+  const cuuint32_t box[3] = {64, cuuint32_t(p.chunk_heads), cuuint32_t(p.stream_tokens)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, p.fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p.q), dims, strides, box,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool FP16>
+static int launch_tc5(const RaggedParams& p, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  if (!rt_map_q(&mq, p, D) || !rt_map_kv(&mk, p, p.k, p.k_sp, p.k_st, p.k_sh, D) || !rt_map_kv(&mv, p, p.v, p.v_sp, p.v_st, p.v_sh, D))
+    return SPF_ERR_SHAPE;
+  const cudaError_t e = cudaFuncSetAttribute(ragged_tc5_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(RtCfg<D>::BYTES));
+  if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
+  ragged_tc5_kernel<D, FP16><<<p.n_ctas, RT_THREADS, RtCfg<D>::BYTES, st>>>(mq, mk, mv, p);
+  return check_launch();
+}
+
+int ragged_tc5_attention(const RaggedParams& p, int head_dim, cudaStream_t st) {
+  if (head_dim == 128) return p.fp16 ? launch_tc5<128, true>(p, st) : launch_tc5<128, false>(p, st);
+  return p.fp16 ? launch_tc5<64, true>(p, st) : launch_tc5<64, false>(p, st);
+}
+
+unsigned int ragged_tc5_timeout_count() { return tc5_read_timeouts_here(); }
+bool ragged_tc5_reset_timeouts() { return tc5_reset_timeouts_here(); }
+bool ragged_tc5_set_wait_limit(unsigned long long ns) { return tc5_set_wait_limit_here(ns); }
+
+}  // namespace spf
