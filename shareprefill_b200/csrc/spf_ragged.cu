@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
       rem -= __shfl_sync(0xffffffffu, inc, 31);
     }
     s.units = int(min(per, all - u));
+    s.taken = s.first > 0 ? int((s.first - 1) % per) + 1 : 0;
   }
   if (lane == 0) reinterpret_cast<RaggedStart*>(p.scratch)[c] = s;
 }

@@ -40,7 +40,8 @@ struct RaggedParams {
 };
 
 // where a CTA starts (written by the schedule kernel); units: what it runs through, 0 if it has no work
-struct RaggedStart { int req, head, tile, first, units, item_units, pad0, pad1; };
+// taken: units of its first item that the CTA runs through in which the item starts
+struct RaggedStart { int req, head, tile, first, units, item_units, taken, pad; };
 
 // units of one item: [0, sink_units) and then [win_first, win_first + total - sink_units)
 struct RaggedSpan { int total, sink_units, win_first, keys; };   // keys: exclusive end of the keys in view

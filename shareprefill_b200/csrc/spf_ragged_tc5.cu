@@ -4,7 +4,8 @@
 // One persistent CTA per SM.  The two tiles of an item ("stream A / B": consecutive tokens x the heads of one KV
 // head) share every K/V unit of 128 keys.
 //
-//   warp 0      producer: the item's Q tiles, then K and V units through a K ring and a V ring by TMA; a unit of
+//   warp 0      producer: walks the CTA's parts of items and announces each to the other warps through shared memory;
+//               loads its Q tiles, then K and V units through a K ring and a V ring by TMA; a unit of
 //               pages smaller than 128 tokens is one copy per page and 64 columns, issued by as many lanes, and a
 //               page that is not there is a copy from behind the pool, which fills zeros
 //   warps 1, 2  MMA issuers of the streams: S = Q K^T and O += P V (P from TMEM); the steps of the two leave in turn
@@ -14,7 +15,8 @@
 //               would reach the output (scores of such keys are replaced, so K needs no such care)
 //   warps 4-7, 8-11  softmax of stream A, B: a thread owns a row; base-2 softmax in fp32 against a reference
 //               point that is fixed by the first unit in which the row sees a key and moved only when a unit's
-//               sum overflows its limit; P rounded to the inputs' type; the epilogue writes the row
+//               sum overflows its limit; P rounded to the inputs' type; the epilogue writes the row.  What describes
+//               the item stays in shared memory: the 128 scores of a row leave few registers
 //
 // The rings, S and P run on across items; Q is loaded as soon as the previous item's last Q K^T is done.
 // Every wait is bounded (spf_tc5.cuh).
@@ -30,17 +32,28 @@ constexpr uint32_t RT_SLAB = 128 * 128;              // [128 rows][64 elements]
 constexpr uint32_t RT_CTRL = 2048;
 constexpr int RT_ABSENT = 16;                        // units whose absent pages are remembered
 
+// A part of an item as the producer announces it.  Unit u starts at key key_a + 128 u for u < units_a, at
+// key_b + 128 (u - units_a) behind that.
+struct alignas(16) RtPart {
+  int units, units_a, key_a, key_b;           // units 0: no more parts
+  int both, whole, slot, n_tok;               // stream B has rows; the item is whole, else its partial slot
+  int heads, pos0, keys, low;                 // keys in [low, keys) or below sinks are seen by some row
+  long long out;                              // offset of the item's first token and head in the output
+  __device__ int key0(int u) const { return u < units_a ? key_a + u * 128 : key_b + (u - units_a) * 128; }
+};
+constexpr int RT_PARTS = 2;                          // announced parts
+
 template <int D>
 struct RtCfg {
   static constexpr int SLABS = D / 64, KSTEPS = D / 16;
   static constexpr uint32_t TILE = RT_SLAB * SLABS;
   static constexpr int KST = D == 128 ? 3 : 6, VST = D == 128 ? 2 : 5;
   // barriers
-  static constexpr int B_QFULL = 0, B_QEMPTY = 1, B_KFULL = 2, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
+  static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 1, B_KFULL = B_QEMPTY + 1, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
                        B_VREADY = B_VFULL + VST, B_VEMPTY = B_VREADY + VST, B_SFULL = B_VEMPTY + VST, B_PREADY = B_SFULL + 2,
                        B_ODONE = B_PREADY + 2, B_TOKEN = B_ODONE + 2, B_N = B_TOKEN + 2;
   static constexpr uint32_t O_TMEM = B_N * 8, O_ABORT = O_TMEM + 8, O_ABSENT = O_ABORT + 8,
-                            O_DTAB = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u;
+                            O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_DTAB = O_PART + RT_PARTS * sizeof(RtPart);
   static constexpr int DT_K = 16, DT_V = DT_K + 8 * KST, DT_N = DT_V + 8 * VST;   // descriptors: 8 per tile, Q_A, Q_B, K.., V..
   static_assert(O_DTAB + DT_N * 8 <= RT_CTRL, "control region too small");
   static_assert(DT_N <= RT_THREADS, "a thread per descriptor");
@@ -110,9 +123,14 @@ __device__ __forceinline__ void mask_between(uint32_t (&r)[32], int a, int b) {
     if (j >= a && j < b) r[j] = 0xff800000u;
 }
 
-// The parts of items that a CTA runs through, in order; every role of the CTA walks them for itself.
+// The parts of items that a CTA runs through, in order, and the order of each part's units.
+// A CTA that runs through the START of its last item takes the item's LAST units, and the next CTAs, which begin
+// with the rest of it, take the units from the front; a whole item without a window starts at the unit whose
+// number is that of units done, and wraps.  So CTAs that have done equally many units stand at about the same
+// key of their items, and what one of them fetched the others find in L2.  (In the order of the keys, the last
+// 2K chunk of a 34K prompt of 32 heads read its 143 MB of K and V 15 times from HBM: 2.1 GB.)
 struct RtWalker {
-  int req, head, tile, first, left, units;
+  int req, head, tile, first, left, units, done;
   RaggedReq q;
   RaggedItem item;
   RaggedSpan span;
@@ -122,25 +140,35 @@ struct RtWalker {
     units = min(left, span.total - first);
   }
   __device__ bool begin(const RaggedParams& p, const RaggedStart& s) {
-    req = s.req; head = s.head; tile = s.tile; first = s.first; left = s.units;
+    req = s.req; head = s.head; tile = s.tile; first = s.first; left = s.units; done = 0; taken = s.taken;
     if (left <= 0) return false;
     q = ragged_req(p, req);
     enter(p);
     return true;
   }
   __device__ bool next(const RaggedParams& p) {
-    left -= units;
+    left -= units; done += units;
     first = 0;
     if (left <= 0 || !ragged_next(p, req, head, tile, q)) return false;
     enter(p);
     return true;
   }
-  __device__ int key0(int u) const {
-    const int s = first + u;
-    return (s < span.sink_units ? s : span.win_first + s - span.sink_units) * RT_UNIT;
+  __device__ void order(const RaggedParams& p, RtPart& part) const {
+    const bool whole = units == span.total;
+    // an item whose start an earlier CTA runs through: that one took the last units, this part's are that many earlier
+    const int from = whole ? (p.window > 0 ? 0 : done % span.total) : first == 0 ? span.total - units : first - taken;
+    part.units = units; part.whole = whole; part.slot = first == 0 ? 1 : 0;
+    if (from < span.sink_units) {             // sinks, then the window
+      part.units_a = min(span.sink_units - from, units);
+      part.key_a = from * RT_UNIT;
+      part.key_b = span.win_first * RT_UNIT;
+    } else {                                  // up to the end, then (a whole item) from the front
+      part.units_a = min(span.total - from, units);
+      part.key_a = (span.win_first + from - span.sink_units) * RT_UNIT;
+      part.key_b = span.win_first * RT_UNIT;
+    }
   }
-  __device__ bool both(const RaggedParams& p) const { return item.n_tok > p.stream_tokens; }
-  __device__ bool whole() const { return units == span.total; }
+  int taken;    // units of the CTA's first item that the CTA where it starts runs through
 };
 
 template <int D, bool FP16>
@@ -166,6 +194,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
   if (tid == 32) { tma_prefetch_map(&map_q); tma_prefetch_map(&map_k); tma_prefetch_map(&map_v); }
   if (tid == 0) {
+    for (int s = 0; s < RT_PARTS; ++s) { mbar_init(bar(C::B_PFULL + s), 1); mbar_init(bar(C::B_PEMPTY + s), 11); }
     mbar_init(bar(C::B_QFULL), 1); mbar_init(bar(C::B_QEMPTY), 2);
     for (int s = 0; s < C::KST; ++s) { mbar_init(bar(C::B_KFULL + s), 1); mbar_init(bar(C::B_KEMPTY + s), 2); }
     for (int s = 0; s < C::VST; ++s) {
@@ -194,12 +223,16 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  RtWalker w = {};
+  RtPart* parts = reinterpret_cast<RtPart*>(smem + C::O_PART);
+  // part n has been announced
+  auto part_ready = [&](int n) { return mbar_wait(bar(C::B_PFULL + n % RT_PARTS), (n / RT_PARTS) & 1, abort_flag); };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(RT_REGS_CONTROL));
     if (warp == 0) {
       // ---------------------------------------------------------- producer (whole warp; lane 0 waits and announces)
+      RtWalker w = {};
+      RtPart part = {};
       const int page = p.table ? 1 << p.page_shift : RT_UNIT;
       const int box = min(page, RT_UNIT), per_unit = RT_UNIT / box;      // rows of a copy, copies of a unit and 64 columns
       const int my_page = lane % per_unit, my_slab = lane / per_unit;
@@ -213,8 +246,8 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       };
       // this lane's page of unit u (the id; n_pages - behind the pool, zeros - where there is none)
       auto page_of = [&](int u) {
-        if (!p.table || u >= w.units) return 0;
-        const int key = w.key0(u) + my_page * box;
+        if (!p.table || u >= part.units) return 0;
+        const int key = part.key0(u) + my_page * box;
         if (key >= w.span.keys) return p.n_pages;
         const int id = __ldg(p.table + w.req * p.table_stride + (key >> p.page_shift));
         return id >= 0 && id < p.n_pages ? id : p.n_pages;
@@ -233,11 +266,25 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ++v_i;
         return true;
       };
+      auto announce = [&](int n, const RtPart& part) {
+        const bool free = wait0(C::B_PEMPTY + n % RT_PARTS, ((n / RT_PARTS) & 1) ^ 1);
+        if (free && lane == 0) {
+          parts[n % RT_PARTS] = part;
+          mbar_arrive(bar(C::B_PFULL + n % RT_PARTS));
+        }
+        return free;
+      };
       for (bool more = w.begin(p, start); ok && more; more = w.next(p), ++pieces) {
-        if (pieces > 0) ok = wait0(C::B_QEMPTY, (pieces - 1) & 1);
+        w.order(p, part);
+        part.both = w.item.n_tok > p.stream_tokens;
+        part.n_tok = w.item.n_tok; part.heads = w.item.heads; part.pos0 = w.item.pos0; part.keys = w.span.keys;
+        part.low = p.window > 0 ? w.item.pos0 - p.window + 1 : 0;
+        part.out = ragged_out(p, w.q, w.item, 0, 0, D);
+        ok = announce(pieces, part);
+        if (ok && pieces > 0) ok = wait0(C::B_QEMPTY, (pieces - 1) & 1);
         if (!ok) break;
         if (lane == 0) {
-          const int streams = w.both(p) ? 2 : 1;
+          const int streams = part.both ? 2 : 1;
           mbar_expect_tx(bar(C::B_QFULL), uint32_t(streams) * q_bytes);
           for (int h = 0; h < streams; ++h)
             for (int s = 0; s < C::SLABS; ++s)
@@ -246,7 +293,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         int id = page_of(0);
         for (int u = 0; u < w.units; ++u) {
-          const int key = w.key0(u), id_next = page_of(u + 1);
+          const int key = part.key0(u), id_next = page_of(u + 1);
           const int s = k_i % C::KST;
           ok = wait0(C::B_KEMPTY + s, ((k_i / C::KST) & 1) ^ 1);
           if (!ok) break;
@@ -268,6 +315,10 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         if (ok) ok = load_v();
       }
+      if (ok) {
+        part.units = 0;
+        announce(pieces, part);
+      }
       // every copy that was started must have landed before the CTA may exit
       if (lane == 0) {
         if (pieces > 0) mbar_wait(bar(C::B_QFULL), (pieces - 1) & 1, abort_flag, true);
@@ -285,76 +336,68 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 4; ++j) { const ulonglong2 t = src[j]; o.d[2 * j] = t.x; o.d[2 * j + 1] = t.y; }
         };
-        int step = 0, i = 0, np = 0, pieces = 0, u = 0;
-        bool have = w.begin(p, start);
-        bool both = w.both(p), mine = h == 0 || both;
-        bool ok = mbar_wait(bar(C::B_QFULL), 0, abort_flag) && mbar_wait(bar(C::B_KFULL), 0, abort_flag);
         auto release = [&](int b, bool used) { if (used) tc_commit(bar(b)); else mbar_arrive(bar(b)); };
-        if (ok) {
-          RtSteps qd, kd;
-          fetch(8 * h, qd); fetch(C::DT_K, kd);
-          if (both) ok = mbar_wait(bar(C::B_TOKEN + h), step & 1, abort_flag);
-          if (ok) {
-            if (mine) { tc_fence_after(); rt_mma_qk<C::KSTEPS>(ts, qd, kd, ID_QK); tc_commit(bar(C::B_SFULL + h)); }
-            if (both) { mbar_arrive(bar(C::B_TOKEN + (h ^ 1))); ++step; }
-            release(C::B_KEMPTY, mine);
-            if (w.units == 1) release(C::B_QEMPTY, mine);
-          }
-        }
-        while (ok && have) {
-          // unit i (P V) and the one after it (Q K^T), which may open the next item
-          const bool p_both = both, p_mine = mine, p_first = u == 0, p_last = u + 1 == w.units;
-          if (p_last) {
-            have = w.next(p);
-            u = 0; ++pieces;
-            if (have) { both = w.both(p); mine = h == 0 || both; }
-          } else {
-            ++u;
-          }
-          const int vs = i % C::VST, ks = (i + 1) % C::KST;
-          const bool q_last = have && u + 1 == w.units, q_mine = have && mine;
-          ok = mbar_wait(bar(C::B_VREADY + vs), (i / C::VST) & 1, abort_flag);
-          if (ok && have) {
-            if (p_last) ok = mbar_wait(bar(C::B_QFULL), pieces & 1, abort_flag);
-            if (ok) ok = mbar_wait(bar(C::B_KFULL + ks), ((i + 1) / C::KST) & 1, abort_flag);
-          }
+        int step = 0, i = 0, np = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+          ok = part_ready(n);
           if (!ok) break;
-          RtSteps vd, qd, kd;
-          if (p_mine) fetch(C::DT_V + 8 * vs, vd);
-          if (q_mine) { fetch(8 * h, qd); fetch(C::DT_K + 8 * ks, kd); }
-          if (p_both) ok = mbar_wait(bar(C::B_TOKEN + h), step & 1, abort_flag);
-          if (ok && p_mine) ok = mbar_wait(bar(C::B_PREADY + h), np & 1, abort_flag);
-          if (!ok) break;
-          if (p_mine || q_mine) tc_fence_after();
-          if (p_mine) {
-            rt_mma_pv(to, ts, vd, ID_PV, p_first ? 0u : 1u);
-            ++np;
-            if (p_last) tc_commit(bar(C::B_ODONE + h));
+          const int units = parts[n % RT_PARTS].units;
+          const bool both = parts[n % RT_PARTS].both != 0, mine = h == 0 || both;
+          mbar_arrive(bar(C::B_PEMPTY + n % RT_PARTS));
+          if (units == 0) break;
+          // Step u: P V of unit u and Q K^T of unit u + 1, the two groups back to back; step -1 has only the latter
+          ok = mbar_wait(bar(C::B_QFULL), n & 1, abort_flag);
+          for (int u = -1; ok && u < units; ++u) {
+            const bool pv = u >= 0, qk = u + 1 < units;
+            const int vs = (i + C::VST - 1) % C::VST, ks = i % C::KST;     // i: units of the CTA whose Q K^T has been issued
+            if (pv) ok = mbar_wait(bar(C::B_VREADY + vs), ((i - 1) / C::VST) & 1, abort_flag);
+            if (ok && qk) ok = mbar_wait(bar(C::B_KFULL + ks), (i / C::KST) & 1, abort_flag);
+            if (!ok) break;
+            if (mine) {
+              RtSteps vd, qd, kd;
+              if (pv) fetch(C::DT_V + 8 * vs, vd);
+              if (qk) { fetch(8 * h, qd); fetch(C::DT_K + 8 * ks, kd); }
+              if (both) ok = mbar_wait(bar(C::B_TOKEN + h), step & 1, abort_flag);
+              if (ok && pv) ok = mbar_wait(bar(C::B_PREADY + h), np & 1, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              if (pv) {
+                rt_mma_pv(to, ts, vd, ID_PV, u > 0 ? 1u : 0u);
+                ++np;
+                if (!qk) tc_commit(bar(C::B_ODONE + h));
+              }
+              if (qk) { rt_mma_qk<C::KSTEPS>(ts, qd, kd, ID_QK); tc_commit(bar(C::B_SFULL + h)); }
+              if (both) { mbar_arrive(bar(C::B_TOKEN + (h ^ 1))); ++step; }
+            }
+            if (pv) release(C::B_VEMPTY + vs, mine);
+            if (qk) {
+              release(C::B_KEMPTY + ks, mine);
+              if (u + 2 == units) release(C::B_QEMPTY, mine);
+              ++i;
+            }
           }
-          if (q_mine) { rt_mma_qk<C::KSTEPS>(ts, qd, kd, ID_QK); tc_commit(bar(C::B_SFULL + h)); }
-          if (p_both) { mbar_arrive(bar(C::B_TOKEN + (h ^ 1))); ++step; }
-          release(C::B_VEMPTY + vs, p_mine);
-          if (have) {
-            release(C::B_KEMPTY + ks, q_mine);
-            if (q_last) release(C::B_QEMPTY, q_mine);
-          }
-          ++i;
         }
       }
     } else {
       // ---------------------------------------------------------- V rows that no query of the item sees become zeros
       bool ok = true;
       int i = 0;
-      for (bool more = w.begin(p, start); ok && more; more = w.next(p)) {
-        const int low = p.window > 0 ? w.item.pos0 - p.window + 1 : 0;
-        for (int u = 0; u < w.units; ++u, ++i) {
+      for (int n = 0; ok; ++n) {
+        ok = __all_sync(0xffffffffu, part_ready(n));
+        if (!ok) break;
+        const RtPart part = parts[n % RT_PARTS];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_PEMPTY + n % RT_PARTS));
+        if (part.units == 0) break;
+        for (int u = 0; u < part.units; ++u, ++i) {
           const int s = i % C::VST;
           ok = mbar_wait(bar(C::B_VFULL + s), (i / C::VST) & 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const int key = w.key0(u);
-          const int tail = min(max(w.span.keys - key, 0), RT_UNIT);                                     // rows [tail, 128)
-          const int a = min(max(p.sinks - key, 0), RT_UNIT), b = min(max(low - key, 0), tail);          // and rows [a, b)
+          const int key = part.key0(u);
+          const int tail = min(max(part.keys - key, 0), RT_UNIT);                                       // rows [tail, 128)
+          const int a = min(max(p.sinks - key, 0), RT_UNIT), b = min(max(part.low - key, 0), tail);     // and rows [a, b)
           if (tail < RT_UNIT || a < b) {
             const uint32_t base = sbase + C::O_V + uint32_t(s) * C::TILE;
             for (int r = lane >> 3; r < RT_UNIT; r += 4)
@@ -385,15 +428,25 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t tO = tmem + lane_base + 256u + uint32_t(h) * D;
     int i = 0, k = 0, done = 0;              // units of the CTA, units and items of this stream
     bool ok = true;
-    for (bool more = w.begin(p, start); ok && more; more = w.next(p)) {
-      if (h == 1 && !w.both(p)) { i += w.units; continue; }
-      const bool in = t_row < p.stream_tokens && tok < w.item.n_tok && h_row < w.item.heads;
-      const int hi = in ? w.item.pos0 + tok : -1, lo = p.window > 0 ? hi - p.window + 1 : 0;
-      // units inside [fast_lo, fast_hi] are seen whole by every row of the stream
-      const int fast_hi = w.item.pos0 + h * p.stream_tokens;
-      const int fast_lo = p.window > 0 ? fast_hi + p.stream_tokens - p.window : 0;
+    for (int n = 0; ok; ++n) {
+      ok = __all_sync(0xffffffffu, part_ready(n));
+      if (!ok) break;
+      const volatile RtPart& part = parts[n % RT_PARTS];
+      const int units = part.units;
+      auto part_done = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_PEMPTY + n % RT_PARTS));
+      };
+      if (units == 0) { part_done(); break; }
+      if (h == 1 && !part.both) { i += units; part_done(); continue; }
+      const bool in = t_row < p.stream_tokens && tok < part.n_tok && h_row < part.heads;
       float m_used = -INFINITY, l_sum = 0.f;
-      for (int u = 0; u < w.units; ++u, ++i, ++k) {
+      bool fresh = true;                     // some row of the warp has seen no key yet
+      for (int u = 0; u < units; ++u, ++i, ++k) {
+        const int key = u < part.units_a ? part.key_a + u * RT_UNIT : part.key_b + (u - part.units_a) * RT_UNIT;
+        // seen whole by every row of the stream: up to its first token's position, from its last token's window on
+        const int first_pos = part.pos0 + h * p.stream_tokens;
+        const bool past = key + RT_UNIT - 1 > first_pos, before = p.window > 0 && key < first_pos + p.stream_tokens - p.window;
         ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_SFULL + h), k & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
@@ -402,15 +455,13 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         tmem_ld32_raw(tS + 32, s1);
         tmem_ld32_raw(tS + 64, s2);
         tmem_ld32_raw(tS + 96, s3);
-        const int key = w.key0(u);
         const uint32_t gone = absent_of[i % RT_ABSENT];
         tc_wait_ld();
-        const bool masked = key + RT_UNIT - 1 > fast_hi || key < fast_lo || gone != 0u;
-        if (masked) {
-          const int last = hi - key;
-          mask_after(s0, last); mask_after(s1, last - 32); mask_after(s2, last - 64); mask_after(s3, last - 96);
-          if (p.window > 0) {
-            const int a = max(p.sinks - key, 0), b = lo - key;
+        if (past || before || gone != 0u) {
+          const int last = (in ? part.pos0 + tok : -1) - key;
+          if (past) { mask_after(s0, last); mask_after(s1, last - 32); mask_after(s2, last - 64); mask_after(s3, last - 96); }
+          if (before) {
+            const int a = max(p.sinks - key, 0), b = last - p.window + 1;
             mask_between(s0, a, b); mask_between(s1, a - 32, b - 32); mask_between(s2, a - 64, b - 64); mask_between(s3, a - 96, b - 96);
           }
           if (gone != 0u) {
@@ -430,23 +481,17 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const float ref = m_used == -INFINITY ? 0.f : m_used;
           float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
           uint32_t pk[16];
-          if (masked) {       // exact zeros where masked: the polynomial's range ends at 2^-57
-            exp_pack_poly<0, FP16>(s0, p.scale_log2, ref, pk, l0); tmem_st16(tS + 0, pk);
-            exp_pack_poly<0, FP16>(s1, p.scale_log2, ref, pk, l1); tmem_st16(tS + 16, pk);
-            exp_pack_poly<0, FP16>(s2, p.scale_log2, ref, pk, l2); tmem_st16(tS + 32, pk);
-            exp_pack_poly<0, FP16>(s3, p.scale_log2, ref, pk, l3); tmem_st16(tS + 48, pk);
-          } else {
-            exp_pack_poly<2, FP16>(s0, p.scale_log2, ref, pk, l0); tmem_st16(tS + 0, pk);
-            exp_pack_poly<2, FP16>(s1, p.scale_log2, ref, pk, l1); tmem_st16(tS + 16, pk);
-            exp_pack_poly<2, FP16>(s2, p.scale_log2, ref, pk, l2); tmem_st16(tS + 32, pk);
-            exp_pack_poly<2, FP16>(s3, p.scale_log2, ref, pk, l3); tmem_st16(tS + 48, pk);
-          }
+          exp_pack_poly<2, FP16>(s0, p.scale_log2, ref, pk, l0); tmem_st16(tS + 0, pk);
+          exp_pack_poly<2, FP16>(s1, p.scale_log2, ref, pk, l1); tmem_st16(tS + 16, pk);
+          exp_pack_poly<2, FP16>(s2, p.scale_log2, ref, pk, l2); tmem_st16(tS + 32, pk);
+          exp_pack_poly<2, FP16>(s3, p.scale_log2, ref, pk, l3); tmem_st16(tS + 48, pk);
           return (l0 + l1) + (l2 + l3);
         };
         // a row's reference is the maximum of the first unit in which it sees a key (nothing was added before)
-        if (__any_sync(0xffffffffu, m_used == -INFINITY)) {
+        if (fresh) {
           const float mb = row_max_log2();
           if (m_used == -INFINITY) m_used = mb;
+          fresh = __any_sync(0xffffffffu, m_used == -INFINITY);
         }
         float blk = emit_p();
         if (u > 0 && __any_sync(0xffffffffu, in && !(blk <= SUM_LIMIT))) {
@@ -480,9 +525,9 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!ok) break;
       tc_fence_after();
       const bool seen = m_used != -INFINITY;
-      if (w.whole()) {
+      if (part.whole) {
         const float inv = seen && l_sum > 0.f ? 1.f / l_sum : 0.f;
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + (in ? ragged_out(p, w.q, w.item, tok, h_row, D) : 0);
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (in ? part.out + (int64_t(tok) * p.n_q_heads + h_row) * D : 0);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
@@ -498,10 +543,10 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
         }
       } else {
-        float* part = ragged_part(p, blockIdx.x, w.first == 0 ? 1 : 0, D);
+        float* dst_part = ragged_part(p, blockIdx.x, part.slot, D);
         const int at = h * RT_ROWS + row;
-        if (in) { part[at] = m_used; part[2 * RT_ROWS + at] = l_sum; }
-        float* dst = part + 4 * RT_ROWS + at * D;
+        if (in) { dst_part[at] = m_used; dst_part[2 * RT_ROWS + at] = l_sum; }
+        float* dst = dst_part + 4 * RT_ROWS + at * D;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
@@ -514,6 +559,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       tc_fence_before();     // the next item's first P (after its S) lets the next product overwrite O
+      part_done();
     }
   }
   __syncwarp();
