@@ -116,12 +116,8 @@ __device__ __forceinline__ void rt_mma_pv(uint32_t o_tmem, uint32_t p_tmem, cons
       : "memory");
 }
 
-// columns [a, b) are masked out
-__device__ __forceinline__ void mask_between(uint32_t (&r)[32], int a, int b) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (j >= a && j < b) r[j] = 0xff800000u;
-}
+// the n lowest bits (n below 0: none, above 32: all)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
 // The parts of items that a CTA runs through, in order, and the order of each part's units.
 // A CTA that runs through the START of its last item takes the item's LAST units, and the next CTAs, which begin
@@ -450,30 +446,33 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_SFULL + h), k & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
+        // Masking rewrites S in TMEM, 32 columns at a time, before the row is read: kept apart like this it costs the
+        // units that need none nothing but the branch (masks on the row's registers cost them 6%).
+        const uint32_t gone = absent_of[i % RT_ABSENT];
+        if (past || before || gone != 0u) {
+          const int last = (in ? part.pos0 + tok : -1) - key;            // last column the row sees
+          const int a = max(p.sinks - key, 0), b = before ? last - p.window + 1 : 0;    // and not [a, b)
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t bad = (gone >> (2 * c) & 1u ? 0xffffu : 0u) | (gone >> (2 * c + 1) & 1u ? 0xffff0000u : 0u);
+            const uint32_t keep = low_bits(last + 1 - c * 32) & ~(low_bits(b - c * 32) & ~low_bits(a - c * 32)) & ~bad;
+            if (__any_sync(0xffffffffu, keep != 0xffffffffu)) {
+              float v[32];
+              tmem_ld32(tS + c * 32, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!(keep >> j & 1u)) v[j] = -INFINITY;
+              tmem_st32(tS + c * 32, v);
+            }
+          }
+          tc_wait_st();
+        }
         uint32_t s0[32], s1[32], s2[32], s3[32];
         tmem_ld32_raw(tS + 0, s0);
         tmem_ld32_raw(tS + 32, s1);
         tmem_ld32_raw(tS + 64, s2);
         tmem_ld32_raw(tS + 96, s3);
-        const uint32_t gone = absent_of[i % RT_ABSENT];
         tc_wait_ld();
-        if (past || before || gone != 0u) {
-          const int last = (in ? part.pos0 + tok : -1) - key;
-          if (past) { mask_after(s0, last); mask_after(s1, last - 32); mask_after(s2, last - 64); mask_after(s3, last - 96); }
-          if (before) {
-            const int a = max(p.sinks - key, 0), b = last - p.window + 1;
-            mask_between(s0, a, b); mask_between(s1, a - 32, b - 32); mask_between(s2, a - 64, b - 64); mask_between(s3, a - 96, b - 96);
-          }
-          if (gone != 0u) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              if (gone >> g & 1u) mask_between(s0, g * 16, g * 16 + 16);
-              if (gone >> (g + 2) & 1u) mask_between(s1, g * 16, g * 16 + 16);
-              if (gone >> (g + 4) & 1u) mask_between(s2, g * 16, g * 16 + 16);
-              if (gone >> (g + 6) & 1u) mask_between(s3, g * 16, g * 16 + 16);
-            }
-          }
-        }
         auto row_max_log2 = [&]() {
           return fmaxf(fmaxf(row_max(s0), row_max(s1)), fmaxf(row_max(s2), row_max(s3))) * p.scale_log2;
         };
