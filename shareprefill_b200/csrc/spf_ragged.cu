@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.n_kv_heads * p.head_chunks;
   for (int r = warp; r < p.n_requests; r += SCH_WARPS) {
-    const RaggedReq q = ragged_req(p, r);
+    const RaggedReq q = ragged_req(p, r, false);
     const int tiles = ragged_tiles(p, q.n);
     long long s = 0;
     for (int t = lane; t < tiles; t += 32) s += ragged_span(p, q, t).total;
@@ -52,9 +52,18 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
     carry += wsum[SCH_WARPS - 1];
     __syncthreads();
   }
+  const long long all = carry, per = max((all + p.n_ctas - 1) / p.n_ctas, 1ll);
+  // tiles of request r that a CTA runs through, rounded
+  auto stride_of = [&](int r, int tiles) {
+    const long long sum = (upto[r] - (r > 0 ? upto[r - 1] : 0)) / heads;
+    return sum > 0 ? int(min(max((2 * per * tiles + sum) / (2 * sum), 1ll), (long long)tiles)) : 1;
+  };
+  if (blockIdx.x == 0 && p.window > 0)
+    for (int r = threadIdx.x; r < p.n_requests; r += SCH_NT)
+      reinterpret_cast<int32_t*>(p.scratch + ragged_starts_bytes(p.n_ctas))[r] = stride_of(r, ragged_tiles(p, ragged_req(p, r, false).n));
   const int c = blockIdx.x * SCH_WARPS + warp;
   if (c >= p.n_ctas) return;
-  const long long all = carry, per = max((all + p.n_ctas - 1) / p.n_ctas, 1ll), u = per * c;
+  const long long u = per * c;
   RaggedStart s = {};
   if (u < all) {
     int lo = 0, hi = p.n_requests - 1;   // first request whose inclusive sum is above u
@@ -64,8 +73,9 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
     }
     const long long before = lo > 0 ? upto[lo - 1] : 0;
     const long long a_head = (upto[lo] - before) / heads;
-    const RaggedReq q = ragged_req(p, lo);
+    RaggedReq q = ragged_req(p, lo, false);
     const int tiles = ragged_tiles(p, q.n);
+    if (p.window > 0) q.stride = stride_of(lo, tiles);
     s.req = lo;
     s.head = int((u - before) / a_head);
     long long rem = (u - before) - a_head * s.head;
