@@ -19,6 +19,7 @@ bool force_generic_profile() { return g_force_generic_profile.load(std::memory_o
 void note_cuda_error(cudaError_t e) { g_last_error = e; }
 
 static inline bool strides_ok(int64_t sn, int64_t sh) { return (sn % 8 == 0) && (sh % 8 == 0); }
+static inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 static inline int log2_ceil(int x) { int b = 0; while ((1 << b) < x) ++b; return b; }
 }  // namespace spf
 
@@ -444,7 +445,7 @@ int spf_paged_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, i
     return SPF_ERR_RANGE;
   if (n_requests > SPF_MAX_REQUESTS || (int64_t(table_width) << shift) > SPF_MAX_KEYS || n_rows > SPF_MAX_KEYS)
     return SPF_ERR_TOO_LARGE;
-  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(scratch) ||
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned32(out) || !aligned32(scratch) ||
       !strides_ok(q_stride_n, q_stride_h) || !strides_ok(k_stride_page, k_stride_token) || k_stride_head % 8 ||
       !strides_ok(v_stride_page, v_stride_token) || v_stride_head % 8)
     return SPF_ERR_ALIGN;
@@ -473,7 +474,7 @@ int spf_window_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, 
   if (rc) return rc;
   if (n_new < 0 || n_keys < n_new) return SPF_ERR_RANGE;
   if (n_keys > SPF_MAX_KEYS) return SPF_ERR_TOO_LARGE;
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(scratch) ||
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned32(out) || !aligned32(scratch) ||
       !strides_ok(q_stride_n, q_stride_h) || !strides_ok(k_stride_n, k_stride_h) || !strides_ok(v_stride_n, v_stride_h))
     return SPF_ERR_ALIGN;
   RaggedParams p;

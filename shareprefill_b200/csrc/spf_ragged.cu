@@ -10,20 +10,7 @@ namespace spf {
 // sums, and each of its warps finds the start of one CTA: request by binary search, head by division, tile
 // by a scan over the tiles.
 constexpr int SCH_NT = 1024, SCH_WARPS = SCH_NT / 32;
-
-__device__ __forceinline__ long long warp_sum_ll(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {   // inclusive
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
+constexpr int FEW_REQUESTS = 32, FEW_TILES = 512;
 
 __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedParams p) {
   __shared__ long long upto[SPF_MAX_REQUESTS];   // inclusive sums over the requests
@@ -31,7 +18,7 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.n_kv_heads * p.head_chunks;
   for (int r = warp; r < p.n_requests; r += SCH_WARPS) {
-    const RaggedReq q = ragged_req(p, r, false);
+    const RaggedReq q = ragged_req_plain(p, r);
     const int tiles = ragged_tiles(p, q.n);
     long long s = 0;
     for (int t = lane; t < tiles; t += 32) s += ragged_span(p, q, t).total;
@@ -53,14 +40,10 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
     __syncthreads();
   }
   const long long all = carry, per = max((all + p.n_ctas - 1) / p.n_ctas, 1ll);
-  // tiles of request r that a CTA runs through, rounded
-  auto stride_of = [&](int r, int tiles) {
-    const long long sum = (upto[r] - (r > 0 ? upto[r - 1] : 0)) / heads;
-    return sum > 0 ? int(min(max((2 * per * tiles + sum) / (2 * sum), 1ll), (long long)tiles)) : 1;
-  };
+  auto head_units = [&](int r) { return (upto[r] - (r > 0 ? upto[r - 1] : 0)) / heads; };
   if (blockIdx.x == 0 && p.window > 0)
     for (int r = threadIdx.x; r < p.n_requests; r += SCH_NT)
-      reinterpret_cast<int32_t*>(p.scratch + ragged_starts_bytes(p.n_ctas))[r] = stride_of(r, ragged_tiles(p, ragged_req(p, r, false).n));
+      ragged_strides(p)[r] = ragged_stride(per, ragged_tiles(p, ragged_req_plain(p, r).n), head_units(r));
   const int c = blockIdx.x * SCH_WARPS + warp;
   if (c >= p.n_ctas) return;
   const long long u = per * c;
@@ -71,34 +54,16 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
       const int mid = (lo + hi) >> 1;
       if (upto[mid] > u) hi = mid; else lo = mid + 1;
     }
-    const long long before = lo > 0 ? upto[lo - 1] : 0;
-    const long long a_head = (upto[lo] - before) / heads;
-    RaggedReq q = ragged_req(p, lo, false);
-    const int tiles = ragged_tiles(p, q.n);
-    if (p.window > 0) q.stride = stride_of(lo, tiles);
-    s.req = lo;
-    s.head = int((u - before) / a_head);
-    long long rem = (u - before) - a_head * s.head;
-    for (int t0 = 0; t0 < tiles; t0 += 32) {
-      const int cost = t0 + lane < tiles ? ragged_span(p, q, t0 + lane).total : 0;
-      const long long inc = warp_scan_ll(cost, lane);
-      const unsigned above = __ballot_sync(0xffffffffu, inc > rem);
-      if (above) {
-        const int at = __ffs(above) - 1;
-        s.tile = t0 + at;
-        s.item_units = __shfl_sync(0xffffffffu, cost, at);
-        s.first = int(rem - __shfl_sync(0xffffffffu, inc - cost, at));
-        break;
-      }
-      rem -= __shfl_sync(0xffffffffu, inc, 31);
-    }
-    s.units = int(min(per, all - u));
-    s.taken = s.first > 0 ? int((s.first - 1) % per) + 1 : 0;
+    RaggedReq q = ragged_req_plain(p, lo);
+    if (p.window > 0) q.stride = ragged_stride(per, ragged_tiles(p, q.n), head_units(lo));
+    s = ragged_cut(p, lo, q, lo > 0 ? upto[lo - 1] : 0, head_units(lo), u, per, all, lane);
   }
   if (lane == 0) reinterpret_cast<RaggedStart*>(p.scratch)[c] = s;
 }
 
-int ragged_schedule(const RaggedParams& p, cudaStream_t st) {
+int ragged_schedule(RaggedParams& p, cudaStream_t st) {
+  p.few = p.n_requests <= FEW_REQUESTS && p.n_rows / p.tile_tokens + p.n_requests <= FEW_TILES;
+  if (p.few) return SPF_OK;
   ragged_schedule_kernel<<<ceil_div(p.n_ctas, SCH_WARPS), SCH_NT, 0, st>>>(p);
   return check_launch();
 }
@@ -118,7 +83,8 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
   const int per = starts[0].units;             // every CTA but the last runs through equally many
   if (s.first > per) return;                   // an earlier CTA starts inside this item too
   const int last = c + (s.item_units - s.first + per - 1) / per - 1;
-  const RaggedReq q = ragged_req(p, s.req);
+  RaggedReq q = ragged_req_plain(p, s.req);
+  if (p.window > 0) q.stride = ragged_strides(p)[s.req];
   const RaggedItem item = ragged_item(p, q, s.head, s.tile);
   auto part = [&](int i) { return ragged_part(p, i < 0 ? c - 1 : c + i, i < 0 ? 1 : 0, D); };
   const int n = last - c + 1;
@@ -195,10 +161,19 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(rsm) + warp * (RR_STAGES * 2 * TILE_B);
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
-  const RaggedStart start = reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
+  __shared__ RaggedStart sh_start;
+  __shared__ int32_t sh_strides[FEW_REQUESTS];
+  if (p.few) {
+    if (warp == 0) {
+      const RaggedStart s = ragged_start_few(p, blockIdx.x, lane, sh_strides);
+      if (lane == 0) sh_start = s;
+    }
+    __syncthreads();
+  }
+  const RaggedStart start = p.few ? sh_start : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
   int left = start.units, req = start.req, head = start.head, tile = start.tile, first = start.first;
   if (left == 0) return;
-  RaggedReq q = ragged_req(p, req);
+  RaggedReq q = ragged_req(p, req, sh_strides);
 
   while (true) {
     const RaggedSpan span = ragged_span(p, q, tile);
@@ -388,7 +363,7 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     left -= units;
     if (left == 0) return;
     first = 0;
-    if (!ragged_next(p, req, head, tile, q)) return;
+    if (!ragged_next(p, req, head, tile, q, sh_strides)) return;
     __syncthreads();   // the buffers become rings again
   }
 }
@@ -400,7 +375,8 @@ void ragged_rows_config(RaggedParams& p) {
   p.chunk_heads = ceil_div(p.group, p.head_chunks);
   p.stream_rows = RR_ROWS;
   p.tile_tokens = p.stream_tokens = RR_ROWS / p.chunk_heads;
-  p.unit_keys = RR_TT * RR_NW;
+  p.unit_shift = 6;
+  static_assert(RR_TT * RR_NW == 64, "keys of a unit");
   p.n_ctas = 2 * 148;
 }
 

@@ -6,7 +6,7 @@
 //
 // Work is cut twice.  An ITEM is a tile of packed query rows (tile_tokens consecutive tokens x the query
 // heads that share a KV head, row = token * chunk_heads + head) of one request and one KV head; its cost is the
-// number of UNITS (unit_keys consecutive keys) that any of its rows sees.  All units of all items form
+// number of UNITS (runs of 64 or 128 keys) that any of its rows sees.  All units of all items form
 // one line, which is cut into equal pieces, one per CTA: a CTA runs through the end of one item, whole
 // items, and the start of another.  Whole items are written to the output, the two broken ones leave
 // their partial (max, sum, unnormalised output) behind and a second kernel joins them.  The load is even
@@ -35,7 +35,8 @@ struct RaggedParams {
   // how the work is cut
   int head_chunks, chunk_heads;              // a KV head's group as head_chunks pieces of at most chunk_heads heads
   int stream_rows, stream_tokens;            // an item's rows come in streams (one MMA tile each) of stream_tokens tokens
-  int tile_rows, tile_tokens, unit_keys, n_ctas;   // tile_rows / stream_rows streams an item
+  int tile_rows, tile_tokens, unit_shift, n_ctas;  // tile_rows / stream_rows streams an item; log2 of the keys of a unit
+  int few;                                   // every CTA finds its start itself (no schedule kernel)
   char* scratch;
 };
 
@@ -58,15 +59,28 @@ inline int64_t ragged_scratch_bytes(int n_ctas, int tile_rows, int head_dim) {
 // first packed row, new tokens, sequence length (whatever the arrays hold, rows stay in the batch); stride of its tiles
 struct RaggedReq { int row0, n, seq, stride; };
 
-// `strides`: the schedule has been made
-__device__ __forceinline__ RaggedReq ragged_req(const RaggedParams& p, int r, bool strides = true) {
+__device__ __forceinline__ int32_t* ragged_strides(const RaggedParams& p) {
+  return reinterpret_cast<int32_t*>(p.scratch + ragged_starts_bytes(p.n_ctas));
+}
+
+// request r as if its tiles were in order
+__device__ __forceinline__ RaggedReq ragged_req_plain(const RaggedParams& p, int r) {
   RaggedReq q;
-  q.stride = strides && p.window > 0 ? reinterpret_cast<const int32_t*>(p.scratch + ragged_starts_bytes(p.n_ctas))[r] : 1;
+  q.stride = 1;
   if (p.cu == nullptr) {
     q.row0 = 0; q.n = p.n_rows; q.seq = p.seq_one;
   } else {
     const int a = min(max(__ldg(p.cu + r), 0), p.n_rows), b = min(max(__ldg(p.cu + r + 1), a), p.n_rows);
     q.row0 = a; q.n = b - a; q.seq = min(max(__ldg(p.seq + r), 0), SPF_MAX_KEYS);
+  }
+  return q;
+}
+// `own`: the strides that this CTA found itself (shared memory), where p.few.  (A pointer to either memory instead of
+// the branch made a mixed batch of 16 requests 40% slower.)
+__device__ __forceinline__ RaggedReq ragged_req(const RaggedParams& p, int r, const int32_t* own) {
+  RaggedReq q = ragged_req_plain(p, r);
+  if (p.window > 0) {
+    if (p.few) q.stride = own[r]; else q.stride = __ldg(ragged_strides(p) + r);
   }
   return q;
 }
@@ -93,21 +107,21 @@ __device__ __forceinline__ RaggedSpan ragged_span(const RaggedParams& p, const R
   RaggedSpan s;
   s.keys = int(max(end, int64_t(0)));
   const int low = p.window > 0 ? max(first_pos - p.window + 1, 0) : 0;
-  const int end_unit = (s.keys + p.unit_keys - 1) / p.unit_keys;
-  s.win_first = min(low / p.unit_keys, end_unit);
-  s.sink_units = min(p.sinks / p.unit_keys + (p.sinks % p.unit_keys != 0), s.win_first);
+  const int rest = (1 << p.unit_shift) - 1, end_unit = (s.keys + rest) >> p.unit_shift;
+  s.win_first = min(low >> p.unit_shift, end_unit);
+  s.sink_units = min((p.sinks >> p.unit_shift) + ((p.sinks & rest) != 0), s.win_first);
   s.total = max(s.sink_units + end_unit - s.win_first, 1);   // an item that sees nothing still has zeros to write
   return s;
 }
 
 // the item after (req, head, tile); false behind the last one
-__device__ __forceinline__ bool ragged_next(const RaggedParams& p, int& req, int& head, int& tile, RaggedReq& q) {
+__device__ __forceinline__ bool ragged_next(const RaggedParams& p, int& req, int& head, int& tile, RaggedReq& q, const int32_t* own) {
   if (++tile < ragged_tiles(p, q.n)) return true;
   tile = 0;
   if (++head < p.n_kv_heads * p.head_chunks) return true;
   head = 0;
   while (++req < p.n_requests) {
-    q = ragged_req(p, req);
+    q = ragged_req(p, req, own);
     if (q.n > 0) return true;
   }
   return false;
@@ -134,6 +148,95 @@ __device__ __forceinline__ float* ragged_part(const RaggedParams& p, int cta, in
          (2 * int64_t(cta) + which) * ragged_partial_floats(p.tile_rows, d);
 }
 
+__device__ __forceinline__ long long warp_sum_ll(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Tiles of a request that a CTA runs through, rounded: `units` of one head's `tiles` tiles, `per` units per CTA.
+__device__ __forceinline__ int ragged_stride(long long per, int tiles, long long units) {
+  return units > 0 ? int(min(max((2 * per * tiles + units) / (2 * units), 1ll), (long long)tiles)) : 1;
+}
+
+// Where the line is cut for CTA c: `u` units into it, which lies in request `req` (q) whose units begin at `before` and
+// are `a_head` per head.  One warp; the result is in every lane.
+__device__ __forceinline__ RaggedStart ragged_cut(const RaggedParams& p, int req, const RaggedReq& q, long long before, long long a_head,
+                                                  long long u, long long per, long long all, int lane) {
+  RaggedStart s = {};
+  const int tiles = ragged_tiles(p, q.n);
+  s.req = req;
+  s.head = int((u - before) / a_head);
+  long long rem = (u - before) - a_head * s.head;
+  for (int t0 = 0; t0 < tiles; t0 += 32) {
+    const int cost = t0 + lane < tiles ? ragged_span(p, q, t0 + lane).total : 0;
+    const long long inc = warp_scan_ll(cost, lane);
+    const unsigned above = __ballot_sync(0xffffffffu, inc > rem);
+    if (above) {
+      const int at = __ffs(above) - 1;
+      s.tile = t0 + at;
+      s.item_units = __shfl_sync(0xffffffffu, cost, at);
+      s.first = int(rem - __shfl_sync(0xffffffffu, inc - cost, at));
+      break;
+    }
+    rem -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+  s.units = int(min(per, all - u));
+  s.taken = s.first > 0 ? int((s.first - 1) % per) + 1 : 0;
+  return s;
+}
+
+// The schedule of a short line (up to 32 requests, few tiles), found by one warp of every CTA for itself: a kernel less.
+// Leaves the strides in `strides` [32] and, for the join, the start and (CTA 0) the strides in the scratch.
+__device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, int c, int lane, int32_t* strides) {
+  const int heads = p.n_kv_heads * p.head_chunks;
+  RaggedReq q = {};
+  q.stride = 1;
+  if (lane < p.n_requests) q = ragged_req_plain(p, lane);
+  const int tiles = ragged_tiles(p, q.n);
+  long long sum = 0;
+  if (__any_sync(0xffffffffu, tiles > 1)) {
+    for (int r = 0; r < p.n_requests; ++r) {
+      RaggedReq o;
+      o.row0 = 0; o.stride = 1;
+      o.n = __shfl_sync(0xffffffffu, q.n, r); o.seq = __shfl_sync(0xffffffffu, q.seq, r);
+      const int n_tiles = ragged_tiles(p, o.n);
+      int part = 0;
+      for (int t = lane; t < n_tiles; t += 32) part += ragged_span(p, o, t).total;
+      const long long all = warp_sum_ll(part);
+      if (lane == r) sum = all;
+    }
+  } else if (tiles == 1) {
+    sum = ragged_span(p, q, 0).total;
+  }
+  const long long upto = warp_scan_ll(sum * heads, lane), all = __shfl_sync(0xffffffffu, upto, 31);
+  const long long per = max((all + p.n_ctas - 1) / p.n_ctas, 1ll), u = per * c;
+  if (p.window > 0) {
+    q.stride = ragged_stride(per, tiles, sum);
+    strides[lane] = q.stride;
+    if (c == 0 && lane < p.n_requests) ragged_strides(p)[lane] = q.stride;
+  }
+  RaggedStart s = {};
+  if (u < all) {
+    const int at = __ffs(__ballot_sync(0xffffffffu, upto > u)) - 1;
+    RaggedReq o;
+    o.row0 = 0;
+    o.n = __shfl_sync(0xffffffffu, q.n, at); o.seq = __shfl_sync(0xffffffffu, q.seq, at); o.stride = __shfl_sync(0xffffffffu, q.stride, at);
+    const long long a_head = __shfl_sync(0xffffffffu, sum, at), end = __shfl_sync(0xffffffffu, upto, at);
+    s = ragged_cut(p, at, o, end - a_head * heads, a_head, u, per, all, lane);
+  }
+  if (lane == 0) reinterpret_cast<RaggedStart*>(p.scratch)[c] = s;
+  return s;
+}
+
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   if (FP16) {
@@ -145,7 +248,8 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 #endif  // __CUDACC__
 
-int ragged_schedule(const RaggedParams& p, cudaStream_t st);
+// decides whether the CTAs find their starts themselves, launches the schedule kernel if not
+int ragged_schedule(RaggedParams& p, cudaStream_t st);
 int ragged_merge(const RaggedParams& p, int head_dim, cudaStream_t st);
 // up to 16 packed rows an item: bandwidth bound (single tokens); also what TMA cannot describe
 void ragged_rows_config(RaggedParams& p);

@@ -48,12 +48,16 @@ struct RtCfg {
   static constexpr int SLABS = D / 64, KSTEPS = D / 16;
   static constexpr uint32_t TILE = RT_SLAB * SLABS;
   static constexpr int KST = D == 128 ? 3 : 6, VST = D == 128 ? 2 : 5;
+  // pairs of exponentials out of eight that go to the FMA pipe.  Measured with 1 / 2 / 3: at D = 128 the last 2K chunk of
+  // a 34K prompt takes 1030 / 1055 / 1287 us (3 spills), at D = 64, where the products take half the time, a mixed batch
+  // 147 / 140 / 207 us
+  static constexpr int POLY = D == 128 ? 1 : 2;
   // barriers
-  static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 1, B_KFULL = B_QEMPTY + 1, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
+  static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
                        B_VREADY = B_VFULL + VST, B_VEMPTY = B_VREADY + VST, B_SFULL = B_VEMPTY + VST, B_PREADY = B_SFULL + 2,
                        B_ODONE = B_PREADY + 2, B_TOKEN = B_ODONE + 2, B_N = B_TOKEN + 2;
   static constexpr uint32_t O_TMEM = B_N * 8, O_ABORT = O_TMEM + 8, O_ABSENT = O_ABORT + 8,
-                            O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_DTAB = O_PART + RT_PARTS * sizeof(RtPart);
+                            O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_START = O_PART + RT_PARTS * sizeof(RtPart), O_DTAB = O_START + sizeof(RaggedStart) + 32 * 4;
   static constexpr int DT_K = 16, DT_V = DT_K + 8 * KST, DT_N = DT_V + 8 * VST;   // descriptors: 8 per tile, Q_A, Q_B, K.., V..
   static_assert(O_DTAB + DT_N * 8 <= RT_CTRL, "control region too small");
   static_assert(DT_N <= RT_THREADS, "a thread per descriptor");
@@ -116,6 +120,13 @@ __device__ __forceinline__ void rt_mma_pv(uint32_t o_tmem, uint32_t p_tmem, cons
       : "memory");
 }
 
+// 32 bytes to a 32-byte boundary.  A thread writes its own row, so an instruction touches 32 lines whatever its width:
+// half as many instructions are half the time (of 16-byte stores: 5% of a windowed prompt).
+__device__ __forceinline__ void store_32(void* dst, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 // the n lowest bits (n below 0: none, above 32: all)
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
@@ -127,6 +138,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 // 2K chunk of a 34K prompt of 32 heads read its 143 MB of K and V 15 times from HBM: 2.1 GB.)
 struct RtWalker {
   int req, head, tile, first, left, units, done;
+  const int32_t* own;
   RaggedReq q;
   RaggedItem item;
   RaggedSpan span;
@@ -135,17 +147,18 @@ struct RtWalker {
     span = ragged_span(p, q, tile);
     units = min(left, span.total - first);
   }
-  __device__ bool begin(const RaggedParams& p, const RaggedStart& s) {
+  __device__ bool begin(const RaggedParams& p, const RaggedStart& s, const int32_t* own_strides) {
+    own = own_strides;
     req = s.req; head = s.head; tile = s.tile; first = s.first; left = s.units; done = 0; taken = s.taken;
     if (left <= 0) return false;
-    q = ragged_req(p, req);
+    q = ragged_req(p, req, own);
     enter(p);
     return true;
   }
   __device__ bool next(const RaggedParams& p) {
     left -= units; done += units;
     first = 0;
-    if (left <= 0 || !ragged_next(p, req, head, tile, q)) return false;
+    if (left <= 0 || !ragged_next(p, req, head, tile, q, own)) return false;
     enter(p);
     return true;
   }
@@ -172,15 +185,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1)
 ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RaggedParams p) {
   using C = RtCfg<D>;
-  if (*reinterpret_cast<volatile unsigned int*>(&g_tc5_timeouts) > 16u) return;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t sbase = smem_addr(smem);
-  if (sbase & 1023u) {
-    if (threadIdx.x == 0) atomicAdd(&g_tc5_timeouts, 1000u);
+  const bool skewed = (sbase & 1023u) != 0;     // the swizzled tiles need a 1024-byte aligned base
+  if (skewed || *reinterpret_cast<volatile unsigned int*>(&g_tc5_timeouts) > 16u) {
+    if (threadIdx.x == 0) {
+      if (skewed) atomicAdd(&g_tc5_timeouts, 1000u);
+      reinterpret_cast<RaggedStart*>(p.scratch)[blockIdx.x] = RaggedStart{};      // nothing for the join to read
+    }
     return;
   }
-  const RaggedStart start = reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
-  if (start.units == 0) return;
   auto bar = [&](int b) { return sbase + 8u * uint32_t(b); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::O_TMEM);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::O_ABORT);
@@ -191,12 +205,12 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (tid == 32) { tma_prefetch_map(&map_q); tma_prefetch_map(&map_k); tma_prefetch_map(&map_v); }
   if (tid == 0) {
     for (int s = 0; s < RT_PARTS; ++s) { mbar_init(bar(C::B_PFULL + s), 1); mbar_init(bar(C::B_PEMPTY + s), 11); }
-    mbar_init(bar(C::B_QFULL), 1); mbar_init(bar(C::B_QEMPTY), 2);
     for (int s = 0; s < C::KST; ++s) { mbar_init(bar(C::B_KFULL + s), 1); mbar_init(bar(C::B_KEMPTY + s), 2); }
     for (int s = 0; s < C::VST; ++s) {
       mbar_init(bar(C::B_VFULL + s), 1); mbar_init(bar(C::B_VREADY + s), 1); mbar_init(bar(C::B_VEMPTY + s), 2);
     }
     for (int h = 0; h < 2; ++h) {
+      mbar_init(bar(C::B_QFULL + h), 1); mbar_init(bar(C::B_QEMPTY + h), 1);
       mbar_init(bar(C::B_SFULL + h), 1); mbar_init(bar(C::B_PREADY + h), 128); mbar_init(bar(C::B_ODONE + h), 1);
       mbar_init(bar(C::B_TOKEN + h), 1);
     }
@@ -210,6 +224,21 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (e < C::DT_K) dtab[e] = desc_kmajor(sbase + C::O_Q + uint32_t(e >> 3) * C::TILE) + kstep;
     else if (e < C::DT_V) dtab[e] = desc_kmajor(sbase + C::O_K + uint32_t((e - C::DT_K) >> 3) * C::TILE) + kstep;
     else dtab[e] = desc_mnmajor(sbase + C::O_V + uint32_t((e - C::DT_V) >> 3) * C::TILE) + uint64_t(uint32_t(ks) * (2048u >> 4));
+  }
+  // Rows of the Q tiles that no copy fills (a group that does not divide 128) would be garbage, NaN perhaps, and a row whose
+  // sum is not finite asks for a new reference point in every unit
+  for (int e = p.stream_tokens * p.chunk_heads * 8 + tid; e < RT_ROWS * 8; e += RT_THREADS) {
+#pragma unroll
+    for (int s = 0; s < 2 * C::SLABS; ++s)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + C::O_Q + uint32_t(s) * RT_SLAB + uint32_t(e) * 16u), "r"(0) : "memory");
+    fence_proxy_async();
+  }
+  RaggedStart* sh_start = reinterpret_cast<RaggedStart*>(smem + C::O_START);
+  int32_t* sh_strides = reinterpret_cast<int32_t*>(smem + C::O_START + sizeof(RaggedStart));
+  if (warp == 2) {
+    const RaggedStart s = p.few ? ragged_start_few(p, blockIdx.x, lane, sh_strides)
+                                : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
+    if (lane == 0) *sh_start = s;
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512u));
@@ -229,6 +258,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // ---------------------------------------------------------- producer (whole warp; lane 0 waits and announces)
       RtWalker w = {};
       RtPart part = {};
+      const RaggedStart start = *sh_start;
       const int page = p.table ? 1 << p.page_shift : RT_UNIT;
       const int box = min(page, RT_UNIT), per_unit = RT_UNIT / box;      // rows of a copy, copies of a unit and 64 columns
       const int my_page = lane % per_unit, my_slab = lane / per_unit;
@@ -270,23 +300,29 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         return free;
       };
-      for (bool more = w.begin(p, start); ok && more; more = w.next(p), ++pieces) {
+      // a stream's Q tile is free when its last Q K^T of the previous part is done
+      int q_n[2] = {0, 0};
+      auto load_q = [&](int h) {
+        if (q_n[h] > 0 && !wait0(C::B_QEMPTY + h, (q_n[h] - 1) & 1)) return false;
+        if (lane == 0) {
+          mbar_expect_tx(bar(C::B_QFULL + h), q_bytes);
+          for (int s = 0; s < C::SLABS; ++s)
+            tma_load_3d(sbase + C::O_Q + uint32_t(h) * C::TILE + uint32_t(s) * RT_SLAB, &map_q, bar(C::B_QFULL + h), s * 64,
+                        w.item.kvh * p.group + w.item.h0, w.q.row0 + w.item.tok0 + h * p.stream_tokens);
+        }
+        ++q_n[h];
+        return true;
+      };
+      for (bool more = w.begin(p, start, sh_strides); ok && more; more = w.next(p), ++pieces) {
         w.order(p, part);
         part.both = w.item.n_tok > p.stream_tokens;
         part.n_tok = w.item.n_tok; part.heads = w.item.heads; part.pos0 = w.item.pos0; part.keys = w.span.keys;
         part.low = p.window > 0 ? w.item.pos0 - p.window + 1 : 0;
         part.out = ragged_out(p, w.q, w.item, 0, 0, D);
         ok = announce(pieces, part);
-        if (ok && pieces > 0) ok = wait0(C::B_QEMPTY, (pieces - 1) & 1);
+        if (ok) ok = load_q(0);
+        if (ok && part.both) ok = load_q(1);
         if (!ok) break;
-        if (lane == 0) {
-          const int streams = part.both ? 2 : 1;
-          mbar_expect_tx(bar(C::B_QFULL), uint32_t(streams) * q_bytes);
-          for (int h = 0; h < streams; ++h)
-            for (int s = 0; s < C::SLABS; ++s)
-              tma_load_3d(sbase + C::O_Q + uint32_t(h) * C::TILE + uint32_t(s) * RT_SLAB, &map_q, bar(C::B_QFULL), s * 64,
-                          w.item.kvh * p.group + w.item.h0, w.q.row0 + w.item.tok0 + h * p.stream_tokens);
-        }
         int id = page_of(0);
         for (int u = 0; u < w.units; ++u) {
           const int key = part.key0(u), id_next = page_of(u + 1);
@@ -317,7 +353,8 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       // every copy that was started must have landed before the CTA may exit
       if (lane == 0) {
-        if (pieces > 0) mbar_wait(bar(C::B_QFULL), (pieces - 1) & 1, abort_flag, true);
+        for (int h = 0; h < 2; ++h)
+          if (q_n[h] > 0) mbar_wait(bar(C::B_QFULL + h), (q_n[h] - 1) & 1, abort_flag, true);
         for (int j = max(0, k_i - C::KST); j < k_i; ++j) mbar_wait(bar(C::B_KFULL + j % C::KST), (j / C::KST) & 1, abort_flag, true);
         for (int j = max(0, v_i - C::VST); j < v_i; ++j) mbar_wait(bar(C::B_VFULL + j % C::VST), (j / C::VST) & 1, abort_flag, true);
       }
@@ -333,7 +370,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           for (int j = 0; j < 4; ++j) { const ulonglong2 t = src[j]; o.d[2 * j] = t.x; o.d[2 * j + 1] = t.y; }
         };
         auto release = [&](int b, bool used) { if (used) tc_commit(bar(b)); else mbar_arrive(bar(b)); };
-        int step = 0, i = 0, np = 0;
+        int step = 0, i = 0, np = 0, nq = 0;
         bool ok = true;
         for (int n = 0; ok; ++n) {
           ok = part_ready(n);
@@ -343,7 +380,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           mbar_arrive(bar(C::B_PEMPTY + n % RT_PARTS));
           if (units == 0) break;
           // Step u: P V of unit u and Q K^T of unit u + 1, the two groups back to back; step -1 has only the latter
-          ok = mbar_wait(bar(C::B_QFULL), n & 1, abort_flag);
+          if (mine) ok = mbar_wait(bar(C::B_QFULL + h), nq++ & 1, abort_flag);
           for (int u = -1; ok && u < units; ++u) {
             const bool pv = u >= 0, qk = u + 1 < units;
             const int vs = (i + C::VST - 1) % C::VST, ks = i % C::KST;     // i: units of the CTA whose Q K^T has been issued
@@ -369,7 +406,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (pv) release(C::B_VEMPTY + vs, mine);
             if (qk) {
               release(C::B_KEMPTY + ks, mine);
-              if (u + 2 == units) release(C::B_QEMPTY, mine);
+              if (mine && u + 2 == units) tc_commit(bar(C::B_QEMPTY + h));
               ++i;
             }
           }
@@ -415,42 +452,52 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // P must stay inside its type's range: a unit's sum of P above this moves the reference point to the unit's maximum
     constexpr float SUM_LIMIT = FP16 ? 32768.f : 1180591620717411303424.f;   // 2^15, 2^70
     constexpr float MARGIN = FP16 ? 0.f : 64.f;
-    const int h = (warp - 4) >> 2, quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const int t_row = row / p.chunk_heads, h_row = row - t_row * p.chunk_heads;
-    const int tok = h * p.stream_tokens + t_row;                       // token of the item
-    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
-    const uint32_t tS = tmem + lane_base + uint32_t(h * 128);
-    const uint32_t tO = tmem + lane_base + 256u + uint32_t(h) * D;
-    int i = 0, k = 0, done = 0;              // units of the CTA, units and items of this stream
+    // The 128 scores of a row and the constants of the exponentials leave about twenty registers: what the loop over
+    // units does not need is looked up (in shared memory) or computed again where it is used.
+    const int h = (warp - 4) >> 2;
+    const uint32_t tS = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(h * 128);
+    auto o_tmem = [&]() { return tmem + (uint32_t((warp & 3) * 32) << 16) + 256u + uint32_t(h) * D; };
+    // this thread's row: token of the item, head of the chunk, and whether the item has it
+    struct Place { int tok, head; bool in; };
+    auto place = [&](const volatile RtPart& part) {
+      const int row = (warp & 3) * 32 + lane, t = row / p.chunk_heads;
+      Place x;
+      x.head = row - t * p.chunk_heads;
+      x.tok = h * p.stream_tokens + t;
+      x.in = t < p.stream_tokens && x.tok < part.n_tok && x.head < part.heads;
+      return x;
+    };
+    // bit 0: units of this stream, bit 1: its items, bits 2, 3: parts, from bit 4: units of the CTA (the first three
+    // wrap, which is all that the barriers' phases need)
+    uint32_t seen_so_far = 0;
     bool ok = true;
-    for (int n = 0; ok; ++n) {
-      ok = __all_sync(0xffffffffu, part_ready(n));
+    while (true) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_PFULL + int(seen_so_far >> 2 & 1u)), seen_so_far >> 3 & 1u, abort_flag));
       if (!ok) break;
-      const volatile RtPart& part = parts[n % RT_PARTS];
-      const int units = part.units;
+      const volatile RtPart& part = parts[seen_so_far >> 2 & 1u];
       auto part_done = [&]() {
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_PEMPTY + n % RT_PARTS));
+        if (lane == 0) mbar_arrive(bar(C::B_PEMPTY + int(seen_so_far >> 2 & 1u)));
+        seen_so_far = (seen_so_far & ~12u) | ((seen_so_far + 4u) & 12u);
       };
-      if (units == 0) { part_done(); break; }
-      if (h == 1 && !part.both) { i += units; part_done(); continue; }
-      const bool in = t_row < p.stream_tokens && tok < part.n_tok && h_row < part.heads;
+      if (part.units == 0) { part_done(); break; }
+      if (h == 1 && !part.both) { seen_so_far += uint32_t(part.units) << 4; part_done(); continue; }
       float m_used = -INFINITY, l_sum = 0.f;
       bool fresh = true;                     // some row of the warp has seen no key yet
-      for (int u = 0; u < units; ++u, ++i, ++k) {
+      for (int u = 0; u < part.units; ++u) {
         const int key = u < part.units_a ? part.key_a + u * RT_UNIT : part.key_b + (u - part.units_a) * RT_UNIT;
         // seen whole by every row of the stream: up to its first token's position, from its last token's window on
         const int first_pos = part.pos0 + h * p.stream_tokens;
         const bool past = key + RT_UNIT - 1 > first_pos, before = p.window > 0 && key < first_pos + p.stream_tokens - p.window;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_SFULL + h), k & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_SFULL + h), seen_so_far & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after();
         // Masking rewrites S in TMEM, 32 columns at a time, before the row is read: kept apart like this it costs the
         // units that need none nothing but the branch (masks on the row's registers cost them 6%).
-        const uint32_t gone = absent_of[i % RT_ABSENT];
+        const uint32_t gone = absent_of[(seen_so_far >> 4) % RT_ABSENT];
         if (past || before || gone != 0u) {
-          const int last = (in ? part.pos0 + tok : -1) - key;            // last column the row sees
+          const Place x = place(part);
+          const int last = (x.in ? part.pos0 + x.tok : -1) - key;        // last column the row sees
           const int a = max(p.sinks - key, 0), b = before ? last - p.window + 1 : 0;    // and not [a, b)
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
@@ -467,24 +514,16 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
           tc_wait_st();
         }
-        uint32_t s0[32], s1[32], s2[32], s3[32];
-        tmem_ld32_raw(tS + 0, s0);
-        tmem_ld32_raw(tS + 32, s1);
-        tmem_ld32_raw(tS + 64, s2);
-        tmem_ld32_raw(tS + 96, s3);
-        tc_wait_ld();
         auto row_max_log2 = [&]() {
-          return fmaxf(fmaxf(row_max(s0), row_max(s1)), fmaxf(row_max(s2), row_max(s3))) * p.scale_log2;
-        };
-        auto emit_p = [&]() {
-          const float ref = m_used == -INFINITY ? 0.f : m_used;
-          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
-          uint32_t pk[16];
-          exp_pack_poly<2, FP16>(s0, p.scale_log2, ref, pk, l0); tmem_st16(tS + 0, pk);
-          exp_pack_poly<2, FP16>(s1, p.scale_log2, ref, pk, l1); tmem_st16(tS + 16, pk);
-          exp_pack_poly<2, FP16>(s2, p.scale_log2, ref, pk, l2); tmem_st16(tS + 32, pk);
-          exp_pack_poly<2, FP16>(s3, p.scale_log2, ref, pk, l3); tmem_st16(tS + 48, pk);
-          return (l0 + l1) + (l2 + l3);
+          float m = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t r[32];
+            tmem_ld32_raw(tS + c * 32, r);
+            tc_wait_ld();
+            m = fmaxf(m, row_max(r));
+          }
+          return m * p.scale_log2;
         };
         // a row's reference is the maximum of the first unit in which it sees a key (nothing was added before)
         if (fresh) {
@@ -492,9 +531,28 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (m_used == -INFINITY) m_used = mb;
           fresh = __any_sync(0xffffffffu, m_used == -INFINITY);
         }
-        float blk = emit_p();
-        if (u > 0 && __any_sync(0xffffffffu, in && !(blk <= SUM_LIMIT))) {
-          tc_wait_st();
+        // P of the row, held in registers until its sum has been looked at: S stays in TMEM for the case that the reference
+        // has to move, and no more than three quarters of it are in registers
+        uint32_t pk0[16], pk1[16], pk2[16], pk3[16];
+        float blk;
+        bool moved = u == 0;
+        while (true) {
+          const float ref = m_used == -INFINITY ? 0.f : m_used;
+          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+          uint32_t s0[32], s1[32], s2[32], s3[32];
+          tmem_ld32_raw(tS + 0, s0);
+          tmem_ld32_raw(tS + 32, s1);
+          tc_wait_ld();
+          tmem_ld32_raw(tS + 64, s2);
+          exp_pack_poly<C::POLY, FP16>(s0, p.scale_log2, ref, pk0, l0);
+          tmem_ld32_raw(tS + 96, s3);
+          exp_pack_poly<C::POLY, FP16>(s1, p.scale_log2, ref, pk1, l1);
+          tc_wait_ld();
+          exp_pack_poly<C::POLY, FP16>(s2, p.scale_log2, ref, pk2, l2);
+          exp_pack_poly<C::POLY, FP16>(s3, p.scale_log2, ref, pk3, l3);
+          blk = (l0 + l1) + (l2 + l3);
+          if (moved || !__any_sync(0xffffffffu, !(blk <= SUM_LIMIT))) break;
+          moved = true;
           const float mb = row_max_log2();
           float alpha = 1.f;
           if (mb > m_used + MARGIN) {
@@ -506,54 +564,59 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             float v[32];
-            tmem_ld32(tO + c * 32, v);
+            tmem_ld32(o_tmem() + c * 32, v);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= alpha;
-            tmem_st32(tO + c * 32, v);
+            tmem_st32(o_tmem() + c * 32, v);
           }
-          blk = emit_p();
         }
+        tmem_st16(tS + 0, pk0); tmem_st16(tS + 16, pk1); tmem_st16(tS + 32, pk2); tmem_st16(tS + 48, pk3);
         l_sum += blk;
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(bar(C::B_PREADY + h));
+        seen_so_far = (seen_so_far ^ 1u) + 16u;
       }
       // ---- epilogue: the row goes to the output, or with its statistics to the scratch
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_ODONE + h), done & 1, abort_flag));
-      ++done;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_ODONE + h), seen_so_far >> 1 & 1u, abort_flag));
       if (!ok) break;
+      seen_so_far ^= 2u;
       tc_fence_after();
-      const bool seen = m_used != -INFINITY;
+      const Place x = place(part);
       if (part.whole) {
-        const float inv = seen && l_sum > 0.f ? 1.f / l_sum : 0.f;
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + (in ? part.out + (int64_t(tok) * p.n_q_heads + h_row) * D : 0);
+        const float inv = m_used != -INFINITY && l_sum > 0.f ? 1.f / l_sum : 0.f;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (x.in ? part.out + (int64_t(x.tok) * p.n_q_heads + x.head) * D : 0);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
-          tmem_ld32(tO + c * 32, v);
-          if (in) {
+          tmem_ld32(o_tmem() + c * 32, v);
+          if (x.in) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint4 x;
-              x.x = pack_half2<FP16>(v[8 * j] * inv, v[8 * j + 1] * inv); x.y = pack_half2<FP16>(v[8 * j + 2] * inv, v[8 * j + 3] * inv);
-              x.z = pack_half2<FP16>(v[8 * j + 4] * inv, v[8 * j + 5] * inv); x.w = pack_half2<FP16>(v[8 * j + 6] * inv, v[8 * j + 7] * inv);
-              *reinterpret_cast<uint4*>(dst + c * 32 + j * 8) = x;
+            for (int j = 0; j < 2; ++j) {
+              uint32_t o[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e] = pack_half2<FP16>(v[16 * j + 2 * e] * inv, v[16 * j + 2 * e + 1] * inv);
+              store_32(dst + c * 32 + j * 16, o);
             }
           }
         }
       } else {
         float* dst_part = ragged_part(p, blockIdx.x, part.slot, D);
-        const int at = h * RT_ROWS + row;
-        if (in) { dst_part[at] = m_used; dst_part[2 * RT_ROWS + at] = l_sum; }
+        const int at = h * RT_ROWS + (warp & 3) * 32 + lane;
+        if (x.in) { dst_part[at] = m_used; dst_part[2 * RT_ROWS + at] = l_sum; }
         float* dst = dst_part + 4 * RT_ROWS + at * D;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
-          tmem_ld32(tO + c * 32, v);
-          if (in) {
+          tmem_ld32(o_tmem() + c * 32, v);
+          if (x.in) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<float4*>(dst + c * 32 + j * 4) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            for (int j = 0; j < 4; ++j) {
+              uint32_t o[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(v[8 * j + e]);
+              store_32(dst + c * 32 + j * 8, o);
+            }
           }
         }
       }
@@ -578,7 +641,8 @@ void ragged_tc5_config(RaggedParams& p) {
   p.stream_tokens = RT_ROWS / p.chunk_heads;
   p.tile_rows = 2 * RT_ROWS;
   p.tile_tokens = 2 * p.stream_tokens;
-  p.unit_keys = RT_UNIT;
+  p.unit_shift = 7;
+  static_assert(RT_UNIT == 128, "keys of a unit");
   p.n_ctas = RT_CTAS;
 }
 
