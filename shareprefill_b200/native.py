@@ -7,7 +7,6 @@ library is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import os
 from typing import NamedTuple, Optional
 
@@ -404,29 +403,33 @@ class PagedPlan(NamedTuple):
     ring_state: torch.Tensor    # int32 [2]: head, count
 
 
-def _i32(t: torch.Tensor, name: str, dev) -> torch.Tensor:
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev:
+def _i32(t: torch.Tensor, name: str, dev):
+    if t.dtype is not torch.int32 or t.device != dev or not t.is_contiguous():
         raise SpfError(f"{name} must be a contiguous int32 tensor on {dev} (got {t.dtype} on {t.device})")
-    return t
 
 
-def _need_cuda(t: torch.Tensor, what: str):
-    if not t.is_cuda:
+def _block_table(t: torch.Tensor, rows: int, dev):
+    """(row stride, width) of a block table of ``rows`` requests"""
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.device != dev:
+        raise SpfError(f"block_table must be an int32 [R, width] tensor on {dev}")
+    (r, width), (step, one) = t.shape, t.stride()
+    if r != rows or one != 1:
+        raise SpfError(f"block_table must have {rows} contiguous rows (got shape {tuple(t.shape)}, strides {t.stride()})")
+    return (step if r > 1 else width), width
+
+
+def _elsewhere(dev, what: str):
+    """The context to re-enter a call in whose tensors are not on the current device; None where they are."""
+    if dev.type != "cuda":
         raise SpfError(f"{what} needs CUDA tensors: there is no CPU fallback")
+    return None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _on_device(fn):
-    """Run ``fn`` with its first tensor's device as the current one."""
-    @functools.wraps(fn)
-    def wrapped(first, *args, **kwargs):
-        if first.is_cuda and first.device.index != torch.cuda.current_device():
-            with torch.cuda.device(first.device):
-                return fn(first, *args, **kwargs)
-        return fn(first, *args, **kwargs)
-    return wrapped
+def _raw_stream(dev) -> int:
+    """The device's current stream as an integer (torch.cuda.current_stream() takes 3 us to make an object of it)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-@_on_device
 def paged_plan(cached_len, new_len, block_table, free_ring, ring_state, n_rows: int, page_size: int,
                ring_state_out=None) -> PagedPlan:
     """Pages, offsets, slots and positions of a step's new tokens, computed on the GPU.
@@ -435,78 +438,89 @@ def paged_plan(cached_len, new_len, block_table, free_ring, ring_state, n_rows: 
     int32 ring of free page ids with ring_state = ``{head, count}``; n_rows: rows of the packed batch (at
     least the sum of new_len; further rows get slot -1).  Requests that cannot be served are refused, see
     ``spf_paged_plan``.  The new ring state goes to ring_state_out (ring_state itself may be given)."""
-    _need_cuda(cached_len, "paged_plan")
-    lib, dev, r = load(), cached_len.device, cached_len.numel()
-    for t, name in ((cached_len, "cached_len"), (new_len, "new_len"), (free_ring, "free_ring"), (ring_state, "ring_state")):
-        _i32(t, name, dev)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.device != dev:
-        raise SpfError(f"block_table must be an int32 [R, width] tensor with contiguous rows on {dev}")
-    if new_len.numel() != r or block_table.shape[0] != r or ring_state.numel() != 2:
-        raise SpfError(f"paged_plan: {r} cached lengths, {new_len.numel()} new lengths, {block_table.shape[0]} table rows, "
-                       f"{ring_state.numel()} ring state words")
-    if ring_state_out is None:
-        ring_state_out = torch.empty(2, dtype=torch.int32, device=dev)
-    elif _i32(ring_state_out, "ring_state_out", dev).numel() != 2:
-        raise SpfError("ring_state_out must hold two words")
-    n_rows = int(n_rows)
+    dev = cached_len.device
+    ctx = _elsewhere(dev, "paged_plan")
+    if ctx is not None:
+        with ctx:
+            return paged_plan(cached_len, new_len, block_table, free_ring, ring_state, n_rows, page_size, ring_state_out)
+    r = cached_len.numel()
+    _i32(cached_len, "cached_len", dev), _i32(new_len, "new_len", dev)
+    _i32(free_ring, "free_ring", dev), _i32(ring_state, "ring_state", dev)
+    step, width = _block_table(block_table, r, dev)
+    if new_len.numel() != r or ring_state.numel() != 2:
+        raise SpfError(f"paged_plan: {r} cached lengths, {new_len.numel()} new lengths, {ring_state.numel()} ring state words")
+    if ring_state_out is not None:
+        _i32(ring_state_out, "ring_state_out", dev)
+        if ring_state_out.numel() != 2:
+            raise SpfError("ring_state_out must hold two words")
     if n_rows < 0:
         raise SpfError("n_rows must not be negative")
-    ints = torch.empty(3 * r + 1 + n_rows, dtype=torch.int32, device=dev)
-    cu_new, seq_len, refused, positions = ints.split([r + 1, r, r, n_rows])
-    slot_map = torch.empty(n_rows, dtype=torch.int64, device=dev)
-    _check(lib.spf_paged_plan(cached_len.data_ptr(), new_len.data_ptr(), r, int(page_size), block_table.data_ptr(),
-                              block_table.stride(0) if r > 1 else block_table.shape[1], block_table.shape[1],
-                              free_ring.data_ptr(), free_ring.numel(), ring_state.data_ptr(), ring_state_out.data_ptr(),
-                              cu_new.data_ptr(), seq_len.data_ptr(), slot_map.data_ptr(), positions.data_ptr(),
-                              refused.data_ptr(), n_rows, _stream()), "spf_paged_plan")
+    # one allocation: slots first (8 bytes each), then the 4-byte outputs
+    words = cached_len.new_empty(3 * n_rows + 3 * r + 3)
+    slots, cu_new, seq_len, refused, positions, state = torch.split_with_sizes(words, [2 * n_rows, r + 1, r, r, n_rows, 2])
+    if ring_state_out is None:
+        ring_state_out = state
+    slot_map = slots.view(torch.int64)
+    at = words.data_ptr()
+    ints = at + 8 * n_rows
+    _check(load().spf_paged_plan(cached_len.data_ptr(), new_len.data_ptr(), r, page_size, block_table.data_ptr(), step, width,
+                                 free_ring.data_ptr(), free_ring.numel(), ring_state.data_ptr(), ring_state_out.data_ptr(),
+                                 ints, ints + 4 * (r + 1), at, ints + 4 * (3 * r + 1), ints + 4 * (2 * r + 1), n_rows,
+                                 _raw_stream(dev)), "spf_paged_plan")
     _launched(1)
     return PagedPlan(cu_new, seq_len, slot_map, positions, refused, ring_state_out)
 
 
 def _paged_views(k_cache, v_cache, dtype, dev, what):
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+    """Shapes and strides of a paged cache, checked against the rows it is used with."""
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape or ks[3] != 1 or vs[3] != 1:
         raise SpfError(f"{what}: caches must be [n_pages, page_size, Hkv, D] views of one shape with contiguous D "
-                       f"(got {tuple(k_cache.shape)} and {tuple(v_cache.shape)})")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype or dtype not in _DTYPE_CODE:
+                       f"(got {tuple(shape)} and {tuple(v_cache.shape)})")
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype or dtype not in _DTYPE_CODE:
         raise SpfError(f"{what}: q/k/v and caches must all be bfloat16 or all float16 (got {dtype}, {k_cache.dtype}, "
                        f"{v_cache.dtype})")
     if k_cache.device != dev or v_cache.device != dev:
         raise SpfError(f"{what}: caches are on {k_cache.device} and {v_cache.device}, the rows on {dev}")
+    return shape, ks, vs
 
 
 def _rows(t: torch.Tensor, name: str):
-    if t.dim() != 3 or t.stride(2) != 1:
+    step = t.stride()
+    if len(step) != 3 or step[2] != 1:
         raise SpfError(f"{name} must be a [rows, heads, D] view with a contiguous head dimension")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    return t.data_ptr(), step[0], step[1]
 
 
-@_on_device
 def paged_write(k, v, slot_map, k_cache, v_cache) -> None:
     """``k_cache[slot] = k[row]``, ``v_cache[slot] = v[row]`` for the rows of ``slot_map`` (int64 ``[rows]``, as
     ``paged_plan`` returns it); slots outside the cache are skipped, slots of one call must differ."""
-    _need_cuda(k, "paged_write")
-    _paged_views(k_cache, v_cache, k.dtype, k.device, "paged_write")
+    dev = k.device
+    ctx = _elsewhere(dev, "paged_write")
+    if ctx is not None:
+        with ctx:
+            return paged_write(k, v, slot_map, k_cache, v_cache)
+    (pages, page_size, hkv, hd), ks, vs = _paged_views(k_cache, v_cache, k.dtype, dev, "paged_write")
+    (kp, kn, kh), (vp, vn, vh) = _rows(k, "k"), _rows(v, "v")
     n, h, d = k.shape
-    if k.shape != v.shape or v.dtype != k.dtype or v.device != k.device or (h, d) != tuple(k_cache.shape[2:]):
+    if k.shape != v.shape or v.dtype is not k.dtype or v.device != dev or h != hkv or d != hd:
         raise SpfError(f"paged_write: rows {tuple(k.shape)} and {tuple(v.shape)} do not match caches {tuple(k_cache.shape)}")
-    if slot_map.dtype != torch.int64 or not slot_map.is_contiguous() or slot_map.numel() != n or slot_map.device != k.device:
-        raise SpfError(f"slot_map must be a contiguous int64 tensor of {n} slots on {k.device}")
-    kp, vp = _rows(k, "k"), _rows(v, "v")
-    _check(load().spf_paged_write(*kp, *vp, slot_map.data_ptr(), n, h, d, k_cache.data_ptr(), *k_cache.stride()[:3],
-                                  v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[0], k_cache.shape[1], _stream()),
+    if slot_map.dtype is not torch.int64 or not slot_map.is_contiguous() or slot_map.numel() != n or slot_map.device != dev:
+        raise SpfError(f"slot_map must be a contiguous int64 tensor of {n} slots on {dev}")
+    _check(load().spf_paged_write(kp, kn, kh, vp, vn, vh, slot_map.data_ptr(), n, h, d, k_cache.data_ptr(), ks[0], ks[1], ks[2],
+                                  v_cache.data_ptr(), vs[0], vs[1], vs[2], pages, page_size, _raw_stream(dev)),
            "spf_paged_write")
     _launched(1)
 
 
 def _attention_out(q, out):
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or out.device != q.device:
         raise SpfError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}")
     return out
 
 
-@_on_device
 def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: int, softmax_scale: float, window: int = 0,
                     sinks: int = 0, out=None):
     """Attention of every request's new tokens (packed rows ``[rows, H, D]``, a chunk or a single token each) over its
@@ -515,52 +529,54 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
     block_table, cu_new, seq_len: as ``paged_plan`` leaves them; max_new: at least the largest number of new tokens of
     a request; window: keys a token sees including its own (0: all), sinks: first tokens that stay visible.  Rows
     that see nothing are zero, rows behind the last request stay as they were in ``out``."""
-    _need_cuda(q, "paged_attention")
-    lib, dev = load(), q.device
-    qp = _rows(q, "q")
-    _paged_views(k_cache, v_cache, q.dtype, dev, "paged_attention")
+    dev, dtype = q.device, q.dtype
+    ctx = _elsewhere(dev, "paged_attention")
+    if ctx is not None:
+        with ctx:
+            return paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new, softmax_scale, window, sinks, out)
+    lib = load()
+    qp, qn, qh = _rows(q, "q")
+    (pages, page_size, hkv, hd), ks, vs = _paged_views(k_cache, v_cache, dtype, dev, "paged_attention")
     n, h, d = q.shape
     r = seq_len.numel()
     _i32(cu_new, "cu_new", dev), _i32(seq_len, "seq_len", dev)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.device != dev:
-        raise SpfError(f"block_table must be an int32 [R, width] tensor with contiguous rows on {dev}")
-    if cu_new.numel() != r + 1 or block_table.shape[0] != r or k_cache.shape[3] != d:
-        raise SpfError(f"paged_attention: {r} lengths, {cu_new.numel()} offsets, {block_table.shape[0]} table rows; "
-                       f"head size {d} of q, {k_cache.shape[3]} of the cache")
+    step, width = _block_table(block_table, r, dev)
+    if cu_new.numel() != r + 1 or hd != d:
+        raise SpfError(f"paged_attention: {r} lengths, {cu_new.numel()} offsets; head size {d} of q, {hd} of the cache")
     out = _attention_out(q, out)
-    hkv, max_new = k_cache.shape[2], int(max_new)
     need = lib.spf_paged_scratch_bytes(max_new, h, hkv, d)
-    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    _check(lib.spf_paged_attention(*qp, n, h, k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(),
-                                   *v_cache.stride()[:3], k_cache.shape[0], k_cache.shape[1], hkv, d, _DTYPE_CODE[q.dtype],
-                                   block_table.data_ptr(), block_table.stride(0) if r > 1 else block_table.shape[1],
-                                   block_table.shape[1], cu_new.data_ptr(), seq_len.data_ptr(), r, max_new,
-                                   float(softmax_scale), int(window), int(sinks), out.data_ptr(), scratch.data_ptr(), need,
-                                   _stream()), "spf_paged_attention")
-    _launched(3)
+    scratch = torch.empty(need or 32, dtype=torch.uint8, device=dev)
+    _check(lib.spf_paged_attention(qp, qn, qh, n, h, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1],
+                                   vs[2], pages, page_size, hkv, d, _DTYPE_CODE[dtype], block_table.data_ptr(), step, width,
+                                   cu_new.data_ptr(), seq_len.data_ptr(), r, max_new, softmax_scale, window, sinks,
+                                   out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)), "spf_paged_attention")
+    _launched(2)
     return out
 
 
-@_on_device
 def window_attention(q, k, v, softmax_scale: float, window: int, sinks: int = 0, out=None):
     """q ``[n, H, D]``: the last n of the N tokens of k/v ``[N, Hkv, D]`` -> ``[n, H, D]``; a token sees the last
     ``window`` keys up to its own (0: all) and the first ``sinks``."""
-    _need_cuda(q, "window_attention")
-    lib, dev = load(), q.device
-    qp, kp, vp = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
-    n, h, d = q.shape
-    if k.shape != v.shape or k.shape[2] != d:
+    dev, dtype = q.device, q.dtype
+    ctx = _elsewhere(dev, "window_attention")
+    if ctx is not None:
+        with ctx:
+            return window_attention(q, k, v, softmax_scale, window, sinks, out)
+    lib = load()
+    (qp, qn, qh), (kp, kn, kh), (vp, vn, vh) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    (n, h, d), (keys, hkv, hd) = q.shape, k.shape
+    if k.shape != v.shape or hd != d:
         raise SpfError(f"window_attention: keys {tuple(k.shape)} and values {tuple(v.shape)} do not match queries {tuple(q.shape)}")
-    if q.dtype not in _DTYPE_CODE or k.dtype != q.dtype or v.dtype != q.dtype or k.device != dev or v.device != dev:
-        raise SpfError(f"window_attention: q/k/v must all be bfloat16 or all float16 on one device (got {q.dtype}, {k.dtype}, "
+    if dtype not in _DTYPE_CODE or k.dtype is not dtype or v.dtype is not dtype or k.device != dev or v.device != dev:
+        raise SpfError(f"window_attention: q/k/v must all be bfloat16 or all float16 on one device (got {dtype}, {k.dtype}, "
                        f"{v.dtype} on {dev}, {k.device}, {v.device})")
     out = _attention_out(q, out)
-    need = lib.spf_paged_scratch_bytes(max(n, 1), h, k.shape[1], d)
-    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    _check(lib.spf_window_attention(*qp, *kp, *vp, n, k.shape[0], h, k.shape[1], d, _DTYPE_CODE[q.dtype],
-                                    float(softmax_scale), int(window), int(sinks), out.data_ptr(), scratch.data_ptr(), need,
-                                    _stream()), "spf_window_attention")
-    _launched(3)
+    need = lib.spf_paged_scratch_bytes(n or 1, h, hkv, d)
+    scratch = torch.empty(need or 32, dtype=torch.uint8, device=dev)
+    _check(lib.spf_window_attention(qp, qn, qh, kp, kn, kh, vp, vn, vh, n, keys, h, hkv, d, _DTYPE_CODE[dtype], softmax_scale,
+                                    window, sinks, out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)),
+           "spf_window_attention")
+    _launched(2)
     return out
 
 
