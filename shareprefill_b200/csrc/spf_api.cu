@@ -412,7 +412,7 @@ static int run_ragged(RaggedParams& p, int max_new, int head_dim, int64_t scratc
   if (scratch_bytes < ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim)) return SPF_ERR_RANGE;
   int rc = ragged_schedule(p, st);
   if (rc == SPF_OK) rc = tc5 ? ragged_tc5_attention(p, head_dim, st) : ragged_rows_attention(p, head_dim, st);
-  if (rc == SPF_OK) rc = ragged_merge(p, head_dim, st);
+  if (rc == SPF_OK) rc = ragged_merge(p, max_new, head_dim, st);
   return rc;
 }
 

@@ -69,39 +69,98 @@ int ragged_schedule(RaggedParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- join of broken items
-// Block (c, y): CTA c's start lies inside an item; if c is the first such CTA of that item, the pieces of
-// CTAs c - 1 (its second slot) and c, c + 1, ... (their first slots) are that item's.  A warp owns rows.
-constexpr int MRG_NT = 256;
+// Block (c, y): CTA c's start lies inside an item; if c is the first such CTA of that item, the item's parts are
+// CTA c - 1's second slot and the first slots of c, c + 1, ...  The block joins MRG_ROWS rows.  Its time is the
+// latency of a few dependent loads, so what is known to be needed is requested at once: in a large tile (a chunk,
+// cut once or twice) a warp takes a row, MRG_FEW parts at a time, and of single tokens (28 heads over 128K keys: cut
+// into 74) a block takes a row, whose parts the warps share and add up through shared memory.  (With a warp per
+// row and one part at a time in both cases the join took 43 us after such a token, 25 us after a 2K chunk.)
+constexpr int MRG_NT = 256, MRG_WARPS = MRG_NT / 32, MRG_FEW = 4;
 
 template <int D, bool FP16>
-__global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams p) {
+__global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams p, int rows_per_block) {
   constexpr int PER = D / 32;
+  __shared__ float acc_of[MRG_WARPS][D], sum_of[MRG_WARPS];
   const RaggedStart* starts = reinterpret_cast<const RaggedStart*>(p.scratch);
   const int c = blockIdx.x + 1;
   const RaggedStart s = starts[c];
-  if (s.units == 0 || s.first == 0) return;
   const int per = starts[0].units;             // every CTA but the last runs through equally many
-  if (s.first > per) return;                   // an earlier CTA starts inside this item too
-  const int last = c + (s.item_units - s.first + per - 1) / per - 1;
+  if (s.units == 0 || s.first == 0 || s.first > per) return;   // the last: an earlier CTA starts inside this item too
+  const int n = (s.item_units - s.first + per - 1) / per + 1;   // parts
   RaggedReq q = ragged_req_plain(p, s.req);
   if (p.window > 0) q.stride = ragged_strides(p)[s.req];
-  const RaggedItem item = ragged_item(p, q, s.head, s.tile);
-  auto part = [&](int i) { return ragged_part(p, i < 0 ? c - 1 : c + i, i < 0 ? 1 : 0, D); };
-  const int n = last - c + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int row = blockIdx.y * (MRG_NT / 32) + warp; row < p.tile_rows; row += gridDim.y * (MRG_NT / 32)) {
-    const int in_stream = row % p.stream_rows, t = in_stream / p.chunk_heads, h = in_stream - t * p.chunk_heads;
-    const int tok = row / p.stream_rows * p.stream_tokens + t;
-    if (t >= p.stream_tokens || tok >= item.n_tok || h >= item.heads) continue;
+  const int64_t tile = ragged_partial_floats(p.tile_rows, D);
+  const float* base = ragged_part(p, c - 1, 1, D);
+  auto part = [&](int i) { return i == 0 ? base : base + (2 * i - 1) * tile; };   // (c - 1, 1), (c, 0), (c + 1, 0), ...
+  // the row's place; false: not a row of the item
+  auto place = [&](int row, int& tok, int& h, const RaggedItem& item) {
+    const int in_stream = row % p.stream_rows, t = in_stream / p.chunk_heads;
+    h = in_stream - t * p.chunk_heads;
+    tok = row / p.stream_rows * p.stream_tokens + t;
+    return t < p.stream_tokens && tok < item.n_tok && h < item.heads;
+  };
+  const int row_end = min(int(blockIdx.y + 1) * rows_per_block, p.tile_rows);
+  if (rows_per_block > 1) {
+#pragma unroll 2
+    for (int row = blockIdx.y * rows_per_block + warp; row < row_end; row += MRG_WARPS) {
+      float top = -INFINITY, sum = 0.f, acc[PER];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+      for (int i0 = 0; i0 < n; i0 += MRG_FEW) {
+        float m[MRG_FEW], l[MRG_FEW], o[MRG_FEW][PER];
+#pragma unroll
+        for (int i = 0; i < MRG_FEW; ++i) {
+          m[i] = -INFINITY;
+          if (i0 + i < n) {
+            const float* x = part(i0 + i);
+            m[i] = x[row];
+            l[i] = x[p.tile_rows + row];
+#pragma unroll
+            for (int e = 0; e < PER; e += 2)
+              *reinterpret_cast<float2*>(&o[i][e]) = *reinterpret_cast<const float2*>(x + 2 * p.tile_rows + row * D + lane * PER + e);
+          }
+        }
+        const float t = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), ref = t == -INFINITY ? 0.f : t;
+        const float a = exp2f(top - ref);
+        top = t;
+        sum *= a;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= a;
+#pragma unroll
+        for (int i = 0; i < MRG_FEW; ++i)
+          if (i0 + i < n) {
+            const float w = exp2f(m[i] - ref);
+            sum += l[i] * w;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] += o[i][e] * w;
+          }
+      }
+      const RaggedItem item = ragged_item(p, q, s.head, s.tile);
+      int tok, h;
+      if (place(row, tok, h, item)) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D) + lane * PER);
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) dst[e >> 1] = pack_half2<FP16>(acc[e] * inv, acc[e + 1] * inv);
+      }
+    }
+    return;
+  }
+  const RaggedItem item = ragged_item(p, q, s.head, s.tile);
+  for (int row = blockIdx.y * rows_per_block; row < row_end; ++row) {
+    int tok, h;
+    if (!place(row, tok, h, item)) continue;          // the same for the whole block
     float top = -INFINITY;
-    for (int i = lane - 1; i < n; i += 32) top = fmaxf(top, part(i)[row]);
+#pragma unroll 4
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[row]);
     top = warp_max(top);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
 #pragma unroll 4
-    for (int i = -1; i < n; ++i) {
+    for (int i = warp; i < n; i += MRG_WARPS) {
       const float* x = part(i);
       const float w = exp2f(x[row] - ref);
       sum += x[p.tile_rows + row] * w;
@@ -112,24 +171,37 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
         acc[e] += t.x * w; acc[e + 1] += t.y * w;
       }
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D) + lane * PER);
+    __syncthreads();                                  // the previous row has been read
 #pragma unroll
-    for (int e = 0; e < PER; e += 2) dst[e >> 1] = pack_half2<FP16>(acc[e] * inv, acc[e + 1] * inv);
+    for (int e = 0; e < PER; ++e) acc_of[warp][lane * PER + e] = acc[e];
+    if (lane == 0) sum_of[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+      float total = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < MRG_WARPS; ++w) {
+        total += sum_of[w];
+        x += acc_of[w][2 * threadIdx.x]; y += acc_of[w][2 * threadIdx.x + 1];
+      }
+      const float inv = total > 0.f ? 1.f / total : 0.f;
+      reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D))[threadIdx.x] =
+          pack_half2<FP16>(x * inv, y * inv);
+    }
   }
 }
 
-int ragged_merge(const RaggedParams& p, int head_dim, cudaStream_t st) {
-  if (p.n_ctas < 2) return SPF_OK;
-  const dim3 grid(p.n_ctas - 1, ceil_div(p.tile_rows, MRG_NT / 32));
-  if (head_dim == 128) {
-    if (p.fp16) ragged_merge_kernel<128, true><<<grid, MRG_NT, 0, st>>>(p);
-    else ragged_merge_kernel<128, false><<<grid, MRG_NT, 0, st>>>(p);
-  } else {
-    if (p.fp16) ragged_merge_kernel<64, true><<<grid, MRG_NT, 0, st>>>(p);
-    else ragged_merge_kernel<64, false><<<grid, MRG_NT, 0, st>>>(p);
-  }
+// Rows that an item can have follow from max_new; a block takes one of few rows (single tokens), 16 of a large tile.
+template <int D, bool FP16>
+static int launch_merge(const RaggedParams& p, int max_new, cudaStream_t st) {
+  const int rows = max_new <= p.stream_tokens ? max_new * p.chunk_heads : p.tile_rows;
+  const int per_block = rows <= 16 ? 1 : 16;
+  ragged_merge_kernel<D, FP16><<<dim3(p.n_ctas - 1, ceil_div(rows, per_block)), MRG_NT, 0, st>>>(p, per_block);
   return check_launch();
+}
+
+int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t st) {
+  if (head_dim == 128) return p.fp16 ? launch_merge<128, true>(p, max_new, st) : launch_merge<128, false>(p, max_new, st);
+  return p.fp16 ? launch_merge<64, true>(p, max_new, st) : launch_merge<64, false>(p, max_new, st);
 }
 
 // ---------------------------------------------------------------- items of up to 16 rows

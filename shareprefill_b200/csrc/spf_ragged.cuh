@@ -250,7 +250,7 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 
 // decides whether the CTAs find their starts themselves, launches the schedule kernel if not
 int ragged_schedule(RaggedParams& p, cudaStream_t st);
-int ragged_merge(const RaggedParams& p, int head_dim, cudaStream_t st);
+int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t st);
 // up to 16 packed rows an item: bandwidth bound (single tokens); also what TMA cannot describe
 void ragged_rows_config(RaggedParams& p);
 int ragged_rows_attention(const RaggedParams& p, int head_dim, cudaStream_t st);
