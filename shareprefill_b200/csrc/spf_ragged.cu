@@ -81,6 +81,7 @@ template <int D, bool FP16>
 __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams p, int rows_per_block) {
   constexpr int PER = D / 32;
   __shared__ float acc_of[MRG_WARPS][D], sum_of[MRG_WARPS];
+  ragged_wait_before();
   const RaggedStart* starts = reinterpret_cast<const RaggedStart*>(p.scratch);
   const int c = blockIdx.x + 1;
   const RaggedStart s = starts[c];
@@ -195,8 +196,7 @@ template <int D, bool FP16>
 static int launch_merge(const RaggedParams& p, int max_new, cudaStream_t st) {
   const int rows = max_new <= p.stream_tokens ? max_new * p.chunk_heads : p.tile_rows;
   const int per_block = rows <= 16 ? 1 : 16;
-  ragged_merge_kernel<D, FP16><<<dim3(p.n_ctas - 1, ceil_div(rows, per_block)), MRG_NT, 0, st>>>(p, per_block);
-  return check_launch();
+  return ragged_launch_after(ragged_merge_kernel<D, FP16>, dim3(p.n_ctas - 1, ceil_div(rows, per_block)), MRG_NT, 0, st, p, per_block);
 }
 
 int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t st) {
@@ -241,6 +241,8 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
       if (lane == 0) sh_start = s;
     }
     __syncthreads();
+  } else {
+    ragged_wait_before();
   }
   const RaggedStart start = p.few ? sh_start : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
   int left = start.units, req = start.req, head = start.head, tile = start.tile, first = start.first;
@@ -458,6 +460,7 @@ static int launch_rows(const RaggedParams& p, cudaStream_t st) {
   static_assert(SMEM >= RR_NW * (16 * D + 32) * 4, "the join of the warps must fit in the rings");
   const cudaError_t e = cudaFuncSetAttribute(ragged_rows_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
+  if (!p.few) return ragged_launch_after(ragged_rows_kernel<D, FP16>, dim3(p.n_ctas), RR_NT, SMEM, st, p);
   ragged_rows_kernel<D, FP16><<<p.n_ctas, RR_NT, SMEM, st>>>(p);
   return check_launch();
 }

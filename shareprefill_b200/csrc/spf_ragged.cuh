@@ -56,6 +56,22 @@ inline int64_t ragged_scratch_bytes(int n_ctas, int tile_rows, int head_dim) {
 }
 
 #ifdef __CUDACC__
+// Launch behind `st`'s last kernel so that the blocks may start while that one ends; they call ragged_wait_before()
+// before they read what it wrote (or return).
+template <typename... A, typename... B>
+inline int ragged_launch_after(void (*kernel)(A...), dim3 grid, int threads, int smem, cudaStream_t st, B... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = size_t(smem); cfg.stream = st;
+  cfg.attrs = &attr; cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
+  return check_launch();
+}
+__device__ __forceinline__ void ragged_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // first packed row, new tokens, sequence length (whatever the arrays hold, rows stay in the batch); stride of its tiles
 struct RaggedReq { int row0, n, seq, stride; };
 

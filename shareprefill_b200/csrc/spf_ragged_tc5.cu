@@ -236,6 +236,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   RaggedStart* sh_start = reinterpret_cast<RaggedStart*>(smem + C::O_START);
   int32_t* sh_strides = reinterpret_cast<int32_t*>(smem + C::O_START + sizeof(RaggedStart));
   if (warp == 2) {
+    if (!p.few) ragged_wait_before();
     const RaggedStart s = p.few ? ragged_start_few(p, blockIdx.x, lane, sh_strides)
                                 : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
     if (lane == 0) *sh_start = s;
@@ -690,6 +691,7 @@ static int launch_tc5(const RaggedParams& p, cudaStream_t st) {
     return SPF_ERR_SHAPE;
   const cudaError_t e = cudaFuncSetAttribute(ragged_tc5_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(RtCfg<D>::BYTES));
   if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
+  if (!p.few) return ragged_launch_after(ragged_tc5_kernel<D, FP16>, dim3(p.n_ctas), RT_THREADS, int(RtCfg<D>::BYTES), st, mq, mk, mv, p);
   ragged_tc5_kernel<D, FP16><<<p.n_ctas, RT_THREADS, RtCfg<D>::BYTES, st>>>(mq, mk, mv, p);
   return check_launch();
 }
