@@ -84,6 +84,26 @@ def shareprefill_attention_core(module, query_states, key_states, value_states, 
         f"dropout (got {query_states.dtype} on {query_states.device}, head_dim {head_dim}, dropout {dropout})")
 
 
+def sliding_window_attention(module, query_states, key_states, value_states, window: int) -> torch.Tensor:
+    """A layer with a sliding window: ``[1,H,N,D]`` -> ``[1,N,H,D]``, every token sees the last ``window`` keys up to its
+    own.  The reference refuses such layers (attn/shareprefill_attn.py:160-184); they need no block selection.  A prompt brings
+    all its keys, a decode step one query and the keys that its cache kept (all, or at least the last ``window``).
+    Batch 1: padding is not visible at this interface."""
+    bsz, _, q_len, head_dim = query_states.shape
+    if bsz != 1:
+        raise NotImplementedError("sliding-window layers are served with batch size 1")
+    if q_len != 1 and q_len != key_states.shape[2]:
+        raise native.SpfError(f"sliding window: {q_len} queries with {key_states.shape[2]} keys is neither a prompt nor a decode step")
+    dropout = float(getattr(module, "attention_dropout", 0.0) or 0.0) if module.training else 0.0
+    if dropout != 0.0:
+        raise native.SpfError(f"sliding window: the B200 kernels have no attention dropout (got {dropout})")
+    if window < 1:
+        raise native.SpfError(f"sliding window must be at least 1 (got {window})")
+    out = native.window_attention(_token_major(query_states[0]), _token_major(key_states[0]), _token_major(value_states[0]),
+                                  getattr(module, "scaling", 1.0 / math.sqrt(head_dim)), window)
+    return out[None]
+
+
 def dense_avg_attn(sharing, pat, num_heads: int) -> torch.Tensor:
     """The reference's ``avg_attn [1,H,nb,nb]`` (zeros except for this layer's pivots)."""
     nb = pat.num_blocks
@@ -104,10 +124,15 @@ def shareprefill_attention_forward(module, query_states, key_states, value_state
     """Hugging Face attention interface: q ``[B,H,N,D]``, k/v ``[B,Hkv,N,D]`` ->
     ``(attn_output [B,N,H,D] contiguous, attn_weights or None)``.  ``attention_mask``,
     ``scaling`` and ``dropout`` are ignored as in the reference (the scale is read from
-    ``module.scaling``)."""
+    ``module.scaling``).  Layers that pass ``sliding_window`` go to ``sliding_window_attention``."""
     sliding_window = kwargs.pop("sliding_window", None)
-    if sliding_window is not None:
-        raise NotImplementedError("SharePrefill attention does not support sliding-window mode yet.")
     gqa_interleave = kwargs.pop("gqa_interleave", False)
+    if sliding_window is not None:
+        if gqa_interleave:
+            raise NotImplementedError("gqa_interleave=True is not supported by the B200 kernels")
+        for name in ("s_aux", "softcap"):      # what some models with windowed layers change the softmax by
+            if kwargs.get(name) is not None:
+                raise NotImplementedError(f"{name} is not supported by the B200 kernels")
+        return sliding_window_attention(module, query_states, key_states, value_states, int(sliding_window)), None
     return shareprefill_attention_core(module, query_states, key_states, value_states,
                                        gqa_interleave=gqa_interleave)

@@ -401,19 +401,30 @@ static int check_ragged(int n_q_heads, int n_kv_heads, int head_dim, int dtype, 
   return SPF_OK;
 }
 
-// Items of up to 16 rows go to the bandwidth-bound kernel, more to the tcgen05 one, unless TMA cannot describe the
-// tensors (strides of 0 in expanded views).
-static bool few_rows(int group, int max_new) { return int64_t(group) * max_new <= 16; }
+// Requests of up to 16 rows per KV head (single tokens) go to the bandwidth-bound kernel, others to the tcgen05 one, each
+// in its own pass over the batch where it may hold both.  (All through the tcgen05 kernel, whose 128-row tiles such
+// requests leave empty, a batch of 14 tokens and two chunks took 131 us instead of 62.)  Tensors that TMA cannot
+// describe (strides of 0 in expanded views) go to the first kernel whole.
+static bool few_rows(int group, int max_new) { return int64_t(group) * max_new <= RAGGED_FEW_ROWS; }
 
-static int run_ragged(RaggedParams& p, int max_new, int head_dim, int64_t scratch_bytes, cudaStream_t st) {
-  const bool tc5 = !few_rows(p.group, max_new) && ragged_tc5_describable(p);
+static int run_pass(RaggedParams p, bool tc5, int only, int max_new, int head_dim, cudaStream_t st) {
+  p.only = only;
   if (tc5) ragged_tc5_config(p); else ragged_rows_config(p);
-  if (tc5 && timeouts_tripped()) return SPF_ERR_TIMEOUT;
-  if (scratch_bytes < ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim)) return SPF_ERR_RANGE;
   int rc = ragged_schedule(p, st);
   if (rc == SPF_OK) rc = tc5 ? ragged_tc5_attention(p, head_dim, st) : ragged_rows_attention(p, head_dim, st);
   if (rc == SPF_OK) rc = ragged_merge(p, max_new, head_dim, st);
   return rc;
+}
+
+static int run_ragged(RaggedParams& p, int max_new, int head_dim, int64_t scratch_bytes, cudaStream_t st) {
+  if (scratch_bytes < spf_paged_scratch_bytes(max_new, p.n_q_heads, p.n_kv_heads, head_dim)) return SPF_ERR_RANGE;
+  if (few_rows(p.group, max_new) || !ragged_tc5_describable(p)) return run_pass(p, false, 0, max_new, head_dim, st);
+  if (timeouts_tripped()) return SPF_ERR_TIMEOUT;
+  // some request brings less than max_new tokens, perhaps few enough
+  const bool mixed = p.n_requests > 1 && p.group <= RAGGED_FEW_ROWS && p.n_rows < int64_t(p.n_requests) * max_new;
+  if (!mixed) return run_pass(p, true, 0, max_new, head_dim, st);
+  const int rc = run_pass(p, false, 1, RAGGED_FEW_ROWS / p.group, head_dim, st);
+  return rc == SPF_OK ? run_pass(p, true, 2, max_new, head_dim, st) : rc;
 }
 
 int64_t spf_paged_scratch_bytes(int max_new, int n_q_heads, int n_kv_heads, int head_dim) {

@@ -19,6 +19,8 @@
 
 namespace spf {
 
+constexpr int RAGGED_FEW_ROWS = 16;          // tokens x heads of a KV head that the bandwidth-bound kernel takes
+
 struct RaggedParams {
   const void* q; int64_t q_sn, q_sh;
   const void* k; int64_t k_sp, k_st, k_sh;   // strides of a page, a token of a page, a KV head
@@ -36,6 +38,7 @@ struct RaggedParams {
   int head_chunks, chunk_heads;              // a KV head's group as head_chunks pieces of at most chunk_heads heads
   int stream_rows, stream_tokens;            // an item's rows come in streams (one MMA tile each) of stream_tokens tokens
   int tile_rows, tile_tokens, unit_shift, n_ctas;  // tile_rows / stream_rows streams an item; log2 of the keys of a unit
+  int only;                                  // requests of this launch: 0 all, 1 those of up to 16 rows per KV head, 2 the others
   int few;                                   // every CTA finds its start itself (no schedule kernel)
   char* scratch;
 };
@@ -88,6 +91,7 @@ __device__ __forceinline__ RaggedReq ragged_req_plain(const RaggedParams& p, int
   } else {
     const int a = min(max(__ldg(p.cu + r), 0), p.n_rows), b = min(max(__ldg(p.cu + r + 1), a), p.n_rows);
     q.row0 = a; q.n = b - a; q.seq = min(max(__ldg(p.seq + r), 0), SPF_MAX_KEYS);
+    if (p.only != 0 && (q.n <= RAGGED_FEW_ROWS / p.group) != (p.only == 1)) q.n = 0;
   }
   return q;
 }

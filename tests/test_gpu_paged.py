@@ -123,6 +123,9 @@ CASES = [
     ([(50, 3), (0, 20)], 16, 200, 1, 64, BF16, 0, 0, "token"),
     ([(0, 1000)], 256, 6, 2, 128, BF16, 8, 1, "token"),
     ([(3000, 64)] + [(i * 37, 1) for i in range(40)], 16, 8, 2, 128, BF16, 0, 0, "token"),
+    ([(i * 29, 1 + 41 * (i % 3)) for i in range(45)], 32, 8, 2, 64, BF16, 90, 2, "head"),
+    ([(700, 5), (0, 5), (33, 5)], 64, 16, 2, 128, FP16, 0, 0, "token"),                # all bring as many
+    ([(5, 2), (900, 1)], 16, 12, 1, 128, BF16, 0, 0, "token"),                         # 12 rows and 24
 ]
 
 
@@ -215,6 +218,7 @@ def test_cache_of_more_than_32_bits_of_elements(new):
     (700, 1500, 14, 2, 128, BF16, 300, 140, "token"), (257, 900, 4, 4, 128, BF16, 5000, 3, "head"),
     (640, 640, 8, 1, 128, BF16, 1, 0, "token"), (300, 1000, 40, 1, 64, FP16, 129, 1, "token"),
     (513, 513, 8, 2, 128, BF16, 0, 9, "token"), (1500, 1500, 32, 8, 64, BF16, 128, 128, "token"),
+    (2100, 2100, 64, 1, 64, BF16, 100, 3, "token"), (1200, 2000, 64, 1, 64, BF16, 0, 0, "token"),    # more than 512 tiles, and less
 ])
 def test_window_attention_matches_the_statement(new, keys, heads, kv_heads, dim, dtype, window, sinks, layout):
     g = torch.Generator().manual_seed(new + keys)

@@ -85,3 +85,23 @@ def test_statement_of_the_attention():
     assert torch.allclose(out, v[2:].double().expand(-1, 2, -1))       # a window of one: the token's own value
     out, _ = R.attention(q, k, v, 2, 0.3, present=torch.zeros(5, dtype=torch.bool))
     assert bool((out == 0).all())
+
+
+def test_sliding_window_layers_refuse_what_they_cannot_do():
+    from types import SimpleNamespace
+
+    from shareprefill_b200.attention import shareprefill_attention_forward as forward
+    module = SimpleNamespace(training=False, attention_dropout=0.1, scaling=0.1)
+    x = torch.zeros(1, 4, 9, 64, dtype=torch.bfloat16)
+    with pytest.raises(native.SpfError, match="CUDA"):
+        forward(module, x, x[:, :2], x[:, :2], None, sliding_window=4)
+    for kw, q in ((dict(s_aux=torch.zeros(4)), x), (dict(softcap=30.0), x), (dict(gqa_interleave=True), x), ({}, x.expand(2, -1, -1, -1))):
+        with pytest.raises(NotImplementedError):
+            forward(module, q, x[:, :2], x[:, :2], None, sliding_window=4, **kw)
+    with pytest.raises(native.SpfError, match="neither"):
+        forward(module, x[:, :, :5], x[:, :2], x[:, :2], None, sliding_window=4)
+    with pytest.raises(native.SpfError, match="at least 1"):
+        forward(module, x, x[:, :2], x[:, :2], None, sliding_window=0)
+    module.training = True
+    with pytest.raises(native.SpfError, match="dropout"):
+        forward(module, x, x[:, :2], x[:, :2], None, sliding_window=4)
