@@ -80,7 +80,7 @@ constexpr int MRG_NT = 256, MRG_WARPS = MRG_NT / 32, MRG_FEW = 4;
 template <int D, bool FP16>
 __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams p, int rows_per_block) {
   constexpr int PER = D / 32;
-  __shared__ float acc_of[MRG_WARPS][D], sum_of[MRG_WARPS];
+  __shared__ float acc_of[MRG_WARPS][D], sum_of[MRG_WARPS], top_of[MRG_WARPS];
   ragged_wait_before();
   const RaggedStart* starts = reinterpret_cast<const RaggedStart*>(p.scratch);
   const int c = blockIdx.x + 1;
@@ -101,44 +101,49 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
     tok = row / p.stream_rows * p.stream_tokens + t;
     return t < p.stream_tokens && tok < item.n_tok && h < item.heads;
   };
-  const int row_end = min(int(blockIdx.y + 1) * rows_per_block, p.tile_rows);
+  const RaggedItem item = ragged_item(p, q, s.head, s.tile);
+  // parts i, i + step, ... of a row, MRG_FEW requested at a time
+  float top, sum, acc[PER];
+  auto add_up = [&](int row, int first, int step) {
+    top = -INFINITY; sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    for (int i0 = first; i0 < n; i0 += MRG_FEW * step) {
+      float m[MRG_FEW], l[MRG_FEW], o[MRG_FEW][PER];
+#pragma unroll
+      for (int i = 0; i < MRG_FEW; ++i) {
+        m[i] = -INFINITY;
+        if (i0 + i * step < n) {
+          const float* x = part(i0 + i * step);
+          m[i] = x[row];
+          l[i] = x[p.tile_rows + row];
+#pragma unroll
+          for (int e = 0; e < PER; e += 2)
+            *reinterpret_cast<float2*>(&o[i][e]) = *reinterpret_cast<const float2*>(x + 2 * p.tile_rows + row * D + lane * PER + e);
+        }
+      }
+      const float t = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), ref = t == -INFINITY ? 0.f : t;
+      const float a = exp2f(top - ref);
+      top = t;
+      sum *= a;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] *= a;
+#pragma unroll
+      for (int i = 0; i < MRG_FEW; ++i)
+        if (i0 + i * step < n) {
+          const float w = exp2f(m[i] - ref);
+          sum += l[i] * w;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] += o[i][e] * w;
+        }
+    }
+  };
+  int tok, h;
   if (rows_per_block > 1) {
+    const int row_end = min(int(blockIdx.y + 1) * rows_per_block, p.tile_rows);
 #pragma unroll 2
     for (int row = blockIdx.y * rows_per_block + warp; row < row_end; row += MRG_WARPS) {
-      float top = -INFINITY, sum = 0.f, acc[PER];
-#pragma unroll
-      for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-      for (int i0 = 0; i0 < n; i0 += MRG_FEW) {
-        float m[MRG_FEW], l[MRG_FEW], o[MRG_FEW][PER];
-#pragma unroll
-        for (int i = 0; i < MRG_FEW; ++i) {
-          m[i] = -INFINITY;
-          if (i0 + i < n) {
-            const float* x = part(i0 + i);
-            m[i] = x[row];
-            l[i] = x[p.tile_rows + row];
-#pragma unroll
-            for (int e = 0; e < PER; e += 2)
-              *reinterpret_cast<float2*>(&o[i][e]) = *reinterpret_cast<const float2*>(x + 2 * p.tile_rows + row * D + lane * PER + e);
-          }
-        }
-        const float t = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), ref = t == -INFINITY ? 0.f : t;
-        const float a = exp2f(top - ref);
-        top = t;
-        sum *= a;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] *= a;
-#pragma unroll
-        for (int i = 0; i < MRG_FEW; ++i)
-          if (i0 + i < n) {
-            const float w = exp2f(m[i] - ref);
-            sum += l[i] * w;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) acc[e] += o[i][e] * w;
-          }
-      }
-      const RaggedItem item = ragged_item(p, q, s.head, s.tile);
-      int tok, h;
+      add_up(row, 0, 1);
       if (place(row, tok, h, item)) {
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
         uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D) + lane * PER);
@@ -148,46 +153,27 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
     }
     return;
   }
-  const RaggedItem item = ragged_item(p, q, s.head, s.tile);
-  for (int row = blockIdx.y * rows_per_block; row < row_end; ++row) {
-    int tok, h;
-    if (!place(row, tok, h, item)) continue;          // the same for the whole block
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[row]);
-    top = warp_max(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[PER];
+  if (!place(blockIdx.y, tok, h, item)) return;
+  add_up(blockIdx.y, warp, MRG_WARPS);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < n; i += MRG_WARPS) {
-      const float* x = part(i);
-      const float w = exp2f(x[row] - ref);
-      sum += x[p.tile_rows + row] * w;
-      const float* o = x + 2 * p.tile_rows + row * D + lane * PER;
+  for (int e = 0; e < PER; ++e) acc_of[warp][lane * PER + e] = acc[e];
+  if (lane == 0) { sum_of[warp] = sum; top_of[warp] = top; }
+  __syncthreads();
+  if (threadIdx.x < D / 2) {
+    float all_top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < PER; e += 2) {
-        const float2 t = *reinterpret_cast<const float2*>(o + e);
-        acc[e] += t.x * w; acc[e + 1] += t.y * w;
-      }
+    for (int w = 0; w < MRG_WARPS; ++w) all_top = fmaxf(all_top, top_of[w]);
+    const float ref = all_top == -INFINITY ? 0.f : all_top;
+    float total = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < MRG_WARPS; ++w) {
+      const float a = exp2f(top_of[w] - ref);
+      total += sum_of[w] * a;
+      x += acc_of[w][2 * threadIdx.x] * a; y += acc_of[w][2 * threadIdx.x + 1] * a;
     }
-    __syncthreads();                                  // the previous row has been read
-#pragma unroll
-    for (int e = 0; e < PER; ++e) acc_of[warp][lane * PER + e] = acc[e];
-    if (lane == 0) sum_of[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x < D / 2) {
-      float total = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-      for (int w = 0; w < MRG_WARPS; ++w) {
-        total += sum_of[w];
-        x += acc_of[w][2 * threadIdx.x]; y += acc_of[w][2 * threadIdx.x + 1];
-      }
-      const float inv = total > 0.f ? 1.f / total : 0.f;
-      reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D))[threadIdx.x] =
-          pack_half2<FP16>(x * inv, y * inv);
-    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D))[threadIdx.x] =
+        pack_half2<FP16>(x * inv, y * inv);
   }
 }
 
@@ -395,16 +381,19 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     __syncthreads();
 
     // join the warps through shared memory (the rings are drained)
-    constexpr int WSTRIDE = 16 * D + 32;
+    constexpr int DS = D + 8, WSTRIDE = 16 * DS + 32;   // rows 8 banks apart; only rows that there are
     float* wbuf = reinterpret_cast<float*>(rsm) + warp * WSTRIDE;
+    if (in0) {
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      *reinterpret_cast<float2*>(wbuf + r0 * D + j * 8 + cq) = make_float2(o[j][0], o[j][1]);
-      *reinterpret_cast<float2*>(wbuf + r1 * D + j * 8 + cq) = make_float2(o[j][2], o[j][3]);
+      for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(wbuf + r0 * DS + j * 8 + cq) = make_float2(o[j][0], o[j][1]);
+    }
+    if (in1) {
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(wbuf + r1 * DS + j * 8 + cq) = make_float2(o[j][2], o[j][3]);
     }
     if ((lane & 3) == 0) {
-      wbuf[16 * D + r0] = m0; wbuf[16 * D + r1] = m1;
-      wbuf[16 * D + 16 + r0] = l0; wbuf[16 * D + 16 + r1] = l1;
+      wbuf[16 * DS + r0] = m0; wbuf[16 * DS + r1] = m1;
+      wbuf[16 * DS + 16 + r0] = l0; wbuf[16 * DS + 16 + r1] = l1;
     }
     __syncthreads();
     const float* all = reinterpret_cast<const float*>(rsm);
@@ -415,14 +404,14 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
       if (h >= item.heads) continue;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < RR_NW; ++w) top = fmaxf(top, all[w * WSTRIDE + 16 * D + r]);
+      for (int w = 0; w < RR_NW; ++w) top = fmaxf(top, all[w * WSTRIDE + 16 * DS + r]);
       const float ref = top == -INFINITY ? 0.f : top;
       float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
       for (int w = 0; w < RR_NW; ++w) {
-        const float sc = exp2f(all[w * WSTRIDE + 16 * D + r] - ref);
-        sum += all[w * WSTRIDE + 16 * D + 16 + r] * sc;
-        const float2 t = *reinterpret_cast<const float2*>(all + w * WSTRIDE + r * D + d);
+        const float sc = exp2f(all[w * WSTRIDE + 16 * DS + r] - ref);
+        sum += all[w * WSTRIDE + 16 * DS + 16 + r] * sc;
+        const float2 t = *reinterpret_cast<const float2*>(all + w * WSTRIDE + r * DS + d);
         x += t.x * sc; y += t.y * sc;
       }
       if (whole) {
@@ -457,7 +446,7 @@ void ragged_rows_config(RaggedParams& p) {
 template <int D, bool FP16>
 static int launch_rows(const RaggedParams& p, cudaStream_t st) {
   constexpr int SMEM = rr_smem_bytes<D>();
-  static_assert(SMEM >= RR_NW * (16 * D + 32) * 4, "the join of the warps must fit in the rings");
+  static_assert(SMEM >= RR_NW * (16 * (D + 8) + 32) * 4, "the join of the warps must fit in the rings");
   const cudaError_t e = cudaFuncSetAttribute(ragged_rows_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
   if (!p.few) return ragged_launch_after(ragged_rows_kernel<D, FP16>, dim3(p.n_ctas), RR_NT, SMEM, st, p);

@@ -182,9 +182,15 @@ __device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {   // 
   return v;
 }
 
+// 64-bit division takes some hundred instructions, and few lines need it
+__device__ __forceinline__ long long div_ll(long long a, long long b) {
+  if (((a | b) >> 31) == 0) return (long long)(unsigned(a) / unsigned(b));
+  return a / b;
+}
+
 // Tiles of a request that a CTA runs through, rounded: `units` of one head's `tiles` tiles, `per` units per CTA.
 __device__ __forceinline__ int ragged_stride(long long per, int tiles, long long units) {
-  return units > 0 ? int(min(max((2 * per * tiles + units) / (2 * units), 1ll), (long long)tiles)) : 1;
+  return units > 0 ? int(min(max(div_ll(2 * per * tiles + units, 2 * units), 1ll), (long long)tiles)) : 1;
 }
 
 // Where the line is cut for CTA c: `u` units into it, which lies in request `req` (q) whose units begin at `before` and
@@ -194,7 +200,7 @@ __device__ __forceinline__ RaggedStart ragged_cut(const RaggedParams& p, int req
   RaggedStart s = {};
   const int tiles = ragged_tiles(p, q.n);
   s.req = req;
-  s.head = int((u - before) / a_head);
+  s.head = int(div_ll(u - before, a_head));
   long long rem = (u - before) - a_head * s.head;
   for (int t0 = 0; t0 < tiles; t0 += 32) {
     const int cost = t0 + lane < tiles ? ragged_span(p, q, t0 + lane).total : 0;
@@ -210,7 +216,7 @@ __device__ __forceinline__ RaggedStart ragged_cut(const RaggedParams& p, int req
     rem -= __shfl_sync(0xffffffffu, inc, 31);
   }
   s.units = int(min(per, all - u));
-  s.taken = s.first > 0 ? int((s.first - 1) % per) + 1 : 0;
+  s.taken = s.first > 0 ? s.first - int(div_ll(s.first - 1, per) * per) : 0;
   return s;
 }
 
@@ -238,7 +244,7 @@ __device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, i
     sum = ragged_span(p, q, 0).total;
   }
   const long long upto = warp_scan_ll(sum * heads, lane), all = __shfl_sync(0xffffffffu, upto, 31);
-  const long long per = max((all + p.n_ctas - 1) / p.n_ctas, 1ll), u = per * c;
+  const long long per = max(div_ll(all + p.n_ctas - 1, p.n_ctas), 1ll), u = per * c;
   if (p.window > 0) {
     q.stride = ragged_stride(per, tiles, sum);
     strides[lane] = q.stride;
