@@ -408,7 +408,7 @@ static int check_ragged(int n_q_heads, int n_kv_heads, int head_dim, int dtype, 
 static bool few_rows(int group, int max_new) { return int64_t(group) * max_new <= RAGGED_FEW_ROWS; }
 
 static int run_pass(RaggedParams p, bool tc5, int only, int max_new, int head_dim, cudaStream_t st) {
-  p.only = only;
+  p.only = only; p.head_dim = head_dim;
   if (tc5) ragged_tc5_config(p); else ragged_rows_config(p);
   int rc = ragged_schedule(p, st);
   if (rc == SPF_OK) rc = tc5 ? ragged_tc5_attention(p, head_dim, st) : ragged_rows_attention(p, head_dim, st);

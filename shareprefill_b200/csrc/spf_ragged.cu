@@ -70,16 +70,36 @@ int ragged_schedule(RaggedParams& p, cudaStream_t st) {
 
 // ---------------------------------------------------------------- join of broken items
 // Block (c, y): CTA c's start lies inside an item; if c is the first such CTA of that item, the item's parts are
-// CTA c - 1's second slot and the first slots of c, c + 1, ...  The block joins MRG_ROWS rows.  Its time is the
-// latency of a few dependent loads, so what is known to be needed is requested at once: in a large tile (a chunk,
-// cut once or twice) a warp takes a row, MRG_FEW parts at a time, and of single tokens (28 heads over 128K keys: cut
-// into 74) a block takes a row, whose parts the warps share and add up through shared memory.  (With a warp per
-// row and one part at a time in both cases the join took 43 us after such a token, 25 us after a 2K chunk.)
+// CTA c - 1's second slot and the first slots of c, c + 1, ...  The time is the latency of a few dependent loads, so
+// what is known to be needed is requested at once and the place of the output comes with the start record.
+//   large tiles (a chunk, cut once or twice): D / 16 lanes take a row, 16 columns each, two parts at a time
+//   single tokens (28 heads over 128K keys: cut into 74): a block takes a row, whose parts the warps share, four at a
+//   time, and add up through shared memory
+// (With a warp per row and one part at a time in both cases the join took 43 us after such a token, 25 us after a 2K chunk.)
 constexpr int MRG_NT = 256, MRG_WARPS = MRG_NT / 32, MRG_FEW = 4;
 
+// running maximum, sum and output of parts whose m, l and (16-byte pieces of) o are given; m = -inf: no part
+template <int N, int V>
+__device__ __forceinline__ void merge_in(const float (&m)[N], const float (&l)[N], const float (&o)[N][V], float& top, float& sum, float (&acc)[V]) {
+  float t = top;
+#pragma unroll
+  for (int i = 0; i < N; ++i) t = fmaxf(t, m[i]);
+  const float ref = t == -INFINITY ? 0.f : t, a = exp2f(top - ref);
+  top = t;
+  sum *= a;
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] *= a;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float w = exp2f(m[i] - ref);
+    sum += l[i] * w;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] += o[i][e] * w;
+  }
+}
+
 template <int D, bool FP16>
-__global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams p, int rows_per_block) {
-  constexpr int PER = D / 32;
+__global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams p, bool large) {
   __shared__ float acc_of[MRG_WARPS][D], sum_of[MRG_WARPS], top_of[MRG_WARPS];
   ragged_wait_before();
   const RaggedStart* starts = reinterpret_cast<const RaggedStart*>(p.scratch);
@@ -88,73 +108,65 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
   const int per = starts[0].units;             // every CTA but the last runs through equally many
   if (s.units == 0 || s.first == 0 || s.first > per) return;   // the last: an earlier CTA starts inside this item too
   const int n = (s.item_units - s.first + per - 1) / per + 1;   // parts
-  RaggedReq q = ragged_req_plain(p, s.req);
-  if (p.window > 0) q.stride = ragged_strides(p)[s.req];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t tile = ragged_partial_floats(p.tile_rows, D);
   const float* base = ragged_part(p, c - 1, 1, D);
   auto part = [&](int i) { return i == 0 ? base : base + (2 * i - 1) * tile; };   // (c - 1, 1), (c, 0), (c + 1, 0), ...
-  // the row's place; false: not a row of the item
-  auto place = [&](int row, int& tok, int& h, const RaggedItem& item) {
-    const int in_stream = row % p.stream_rows, t = in_stream / p.chunk_heads;
-    h = in_stream - t * p.chunk_heads;
-    tok = row / p.stream_rows * p.stream_tokens + t;
-    return t < p.stream_tokens && tok < item.n_tok && h < item.heads;
+  // offset of the row in the output, in elements; -1: not a row of the item
+  auto place = [&](int row) -> int64_t {
+    const int in_stream = row % p.stream_rows, t = in_stream / p.chunk_heads, h = in_stream - t * p.chunk_heads;
+    const int tok = row / p.stream_rows * p.stream_tokens + t;
+    if (t >= p.stream_tokens || tok >= s.n_tok || h >= s.heads) return -1;
+    return s.out + (int64_t(tok) * p.n_q_heads + h) * D;
   };
-  const RaggedItem item = ragged_item(p, q, s.head, s.tile);
-  // parts i, i + step, ... of a row, MRG_FEW requested at a time
-  float top, sum, acc[PER];
-  auto add_up = [&](int row, int first, int step) {
-    top = -INFINITY; sum = 0.f;
+  if (large) {
+    constexpr int LANES = D / 16, N = 2;       // lane x has columns 4 x + 4 LANES j .. + 3, j < 4
+    const int row = blockIdx.y * (MRG_NT / LANES) + threadIdx.x / LANES, x4 = (threadIdx.x % LANES) * 4;
+    float top = -INFINITY, sum = 0.f, acc[16];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    for (int i0 = first; i0 < n; i0 += MRG_FEW * step) {
-      float m[MRG_FEW], l[MRG_FEW], o[MRG_FEW][PER];
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += N) {
+      float m[N], l[N], o[N][16];
 #pragma unroll
-      for (int i = 0; i < MRG_FEW; ++i) {
-        m[i] = -INFINITY;
-        if (i0 + i * step < n) {
-          const float* x = part(i0 + i * step);
-          m[i] = x[row];
-          l[i] = x[p.tile_rows + row];
+      for (int i = 0; i < N; ++i) {
+        const float* x = part(min(i0 + i, n - 1));
+        m[i] = i0 + i < n ? x[row] : -INFINITY;
+        l[i] = x[p.tile_rows + row];
 #pragma unroll
-          for (int e = 0; e < PER; e += 2)
-            *reinterpret_cast<float2*>(&o[i][e]) = *reinterpret_cast<const float2*>(x + 2 * p.tile_rows + row * D + lane * PER + e);
-        }
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4*>(&o[i][4 * j]) = *reinterpret_cast<const float4*>(x + 2 * p.tile_rows + row * D + x4 + j * 4 * LANES);
       }
-      const float t = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), ref = t == -INFINITY ? 0.f : t;
-      const float a = exp2f(top - ref);
-      top = t;
-      sum *= a;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) acc[e] *= a;
-#pragma unroll
-      for (int i = 0; i < MRG_FEW; ++i)
-        if (i0 + i * step < n) {
-          const float w = exp2f(m[i] - ref);
-          sum += l[i] * w;
-#pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] += o[i][e] * w;
-        }
+      merge_in(m, l, o, top, sum, acc);
     }
-  };
-  int tok, h;
-  if (rows_per_block > 1) {
-    const int row_end = min(int(blockIdx.y + 1) * rows_per_block, p.tile_rows);
-#pragma unroll 2
-    for (int row = blockIdx.y * rows_per_block + warp; row < row_end; row += MRG_WARPS) {
-      add_up(row, 0, 1);
-      if (place(row, tok, h, item)) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D) + lane * PER);
+    const int64_t at = place(row);
+    if (at < 0) return;                        // what was read of such a row was never written, and is not used
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) dst[e >> 1] = pack_half2<FP16>(acc[e] * inv, acc[e + 1] * inv);
-      }
-    }
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at + x4 + j * 4 * LANES) =
+          make_uint2(pack_half2<FP16>(acc[4 * j] * inv, acc[4 * j + 1] * inv), pack_half2<FP16>(acc[4 * j + 2] * inv, acc[4 * j + 3] * inv));
     return;
   }
-  if (!place(blockIdx.y, tok, h, item)) return;
-  add_up(blockIdx.y, warp, MRG_WARPS);
+  constexpr int PER = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y;
+  const int64_t at = place(row);
+  if (at < 0) return;
+  float top = -INFINITY, sum = 0.f, acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  for (int i0 = warp; i0 < n; i0 += MRG_FEW * MRG_WARPS) {
+    float m[MRG_FEW], l[MRG_FEW], o[MRG_FEW][PER];
+#pragma unroll
+    for (int i = 0; i < MRG_FEW; ++i) {
+      const bool there = i0 + i * MRG_WARPS < n;
+      const float* x = part(there ? i0 + i * MRG_WARPS : i0);
+      m[i] = there ? x[row] : -INFINITY;
+      l[i] = x[p.tile_rows + row];
+#pragma unroll
+      for (int e = 0; e < PER; e += 2)
+        *reinterpret_cast<float2*>(&o[i][e]) = *reinterpret_cast<const float2*>(x + 2 * p.tile_rows + row * D + lane * PER + e);
+    }
+    merge_in(m, l, o, top, sum, acc);
+  }
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc_of[warp][lane * PER + e] = acc[e];
   if (lane == 0) { sum_of[warp] = sum; top_of[warp] = top; }
@@ -172,17 +184,17 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
       x += acc_of[w][2 * threadIdx.x] * a; y += acc_of[w][2 * threadIdx.x + 1] * a;
     }
     const float inv = total > 0.f ? 1.f / total : 0.f;
-    reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, tok, h, D))[threadIdx.x] =
-        pack_half2<FP16>(x * inv, y * inv);
+    reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at)[threadIdx.x] = pack_half2<FP16>(x * inv, y * inv);
   }
 }
 
-// Rows that an item can have follow from max_new; a block takes one of few rows (single tokens), 16 of a large tile.
+// Rows that an item can have follow from max_new.
 template <int D, bool FP16>
 static int launch_merge(const RaggedParams& p, int max_new, cudaStream_t st) {
   const int rows = max_new <= p.stream_tokens ? max_new * p.chunk_heads : p.tile_rows;
-  const int per_block = rows <= 16 ? 1 : 16;
-  return ragged_launch_after(ragged_merge_kernel<D, FP16>, dim3(p.n_ctas - 1, ceil_div(rows, per_block)), MRG_NT, 0, st, p, per_block);
+  const bool large = rows > RAGGED_FEW_ROWS;
+  const int blocks = large ? ceil_div(rows, MRG_NT / (D / 16)) : rows;
+  return ragged_launch_after(ragged_merge_kernel<D, FP16>, dim3(p.n_ctas - 1, blocks), MRG_NT, 0, st, p, large);
 }
 
 int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t st) {

@@ -30,7 +30,7 @@ struct RaggedParams {
   int table_width, n_pages, page_shift;
   const int32_t* cu; const int32_t* seq;     // [R + 1], [R]; nullptr: one request of n_rows tokens, seq_one keys
   int n_requests, n_rows, seq_one;
-  int n_q_heads, n_kv_heads, group;
+  int n_q_heads, n_kv_heads, group, head_dim;
   int window, sinks;                         // window 0: none
   float scale_log2;
   int fp16;
@@ -43,9 +43,10 @@ struct RaggedParams {
   char* scratch;
 };
 
-// where a CTA starts (written by the schedule kernel; tile: in the line's order); units: what it runs through, 0 if it has no work
-// taken: units of its first item that the CTA runs through in which the item starts
-struct RaggedStart { int req, head, tile, first, units, item_units, taken, pad; };
+// Where a CTA starts (tile: in the line's order).  units: what it runs through, 0 if it has no work; taken: units of its
+// first item that the CTA runs through in which the item starts; n_tok, heads, out: that item's tokens, heads and
+// offset in the output, for the join.
+struct alignas(16) RaggedStart { int req, head, tile, first, units, item_units, taken, n_tok, heads, pad; long long out; };
 
 // units of one item: [0, sink_units) and then [win_first, win_first + total - sink_units)
 struct RaggedSpan { int total, sink_units, win_first, keys; };   // keys: exclusive end of the keys in view
@@ -151,7 +152,7 @@ __device__ __forceinline__ bool ragged_next(const RaggedParams& p, int& req, int
 struct RaggedItem { int kvh, h0, heads, tok0, n_tok, pos0; };   // first head of the chunk (in its group), heads and tokens there are
 __device__ __forceinline__ RaggedItem ragged_item(const RaggedParams& p, const RaggedReq& q, int head, int at) {
   RaggedItem t;
-  t.kvh = head / p.head_chunks;
+  t.kvh = p.head_chunks == 1 ? head : head / p.head_chunks;
   t.h0 = (head - t.kvh * p.head_chunks) * p.chunk_heads;
   t.heads = min(p.chunk_heads, p.group - t.h0);
   t.tok0 = ragged_place(p, q, at) * p.tile_tokens;
@@ -217,6 +218,9 @@ __device__ __forceinline__ RaggedStart ragged_cut(const RaggedParams& p, int req
   }
   s.units = int(min(per, all - u));
   s.taken = s.first > 0 ? s.first - int(div_ll(s.first - 1, per) * per) : 0;
+  const RaggedItem item = ragged_item(p, q, s.head, s.tile);
+  s.n_tok = item.n_tok; s.heads = item.heads;
+  s.out = ragged_out(p, q, item, 0, 0, p.head_dim);
   return s;
 }
 
@@ -254,7 +258,7 @@ __device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, i
   if (u < all) {
     const int at = __ffs(__ballot_sync(0xffffffffu, upto > u)) - 1;
     RaggedReq o;
-    o.row0 = 0;
+    o.row0 = __shfl_sync(0xffffffffu, q.row0, at);
     o.n = __shfl_sync(0xffffffffu, q.n, at); o.seq = __shfl_sync(0xffffffffu, q.seq, at); o.stride = __shfl_sync(0xffffffffu, q.stride, at);
     const long long a_head = __shfl_sync(0xffffffffu, sum, at), end = __shfl_sync(0xffffffffu, upto, at);
     s = ragged_cut(p, at, o, end - a_head * heads, a_head, u, per, all, lane);

@@ -57,7 +57,7 @@ struct RtCfg {
                        B_VREADY = B_VFULL + VST, B_VEMPTY = B_VREADY + VST, B_SFULL = B_VEMPTY + VST, B_PREADY = B_SFULL + 2,
                        B_ODONE = B_PREADY + 2, B_TOKEN = B_ODONE + 2, B_N = B_TOKEN + 2;
   static constexpr uint32_t O_TMEM = B_N * 8, O_ABORT = O_TMEM + 8, O_ABSENT = O_ABORT + 8,
-                            O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_START = O_PART + RT_PARTS * sizeof(RtPart), O_DTAB = O_START + sizeof(RaggedStart) + 32 * 4;
+                            O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_STRIDES = O_PART + RT_PARTS * sizeof(RtPart), O_DTAB = O_STRIDES + 32 * 4;
   static constexpr int DT_K = 16, DT_V = DT_K + 8 * KST, DT_N = DT_V + 8 * VST;   // descriptors: 8 per tile, Q_A, Q_B, K.., V..
   static_assert(O_DTAB + DT_N * 8 <= RT_CTRL, "control region too small");
   static_assert(DT_N <= RT_THREADS, "a thread per descriptor");
@@ -202,8 +202,8 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* dtab = reinterpret_cast<uint64_t*>(smem + C::O_DTAB);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  if (tid == 32) { tma_prefetch_map(&map_q); tma_prefetch_map(&map_k); tma_prefetch_map(&map_v); }
-  if (tid == 0) {
+  if (tid == 64) { tma_prefetch_map(&map_q); tma_prefetch_map(&map_k); tma_prefetch_map(&map_v); }
+  if (tid == 96) {
     for (int s = 0; s < RT_PARTS; ++s) { mbar_init(bar(C::B_PFULL + s), 1); mbar_init(bar(C::B_PEMPTY + s), 11); }
     for (int s = 0; s < C::KST; ++s) { mbar_init(bar(C::B_KFULL + s), 1); mbar_init(bar(C::B_KEMPTY + s), 2); }
     for (int s = 0; s < C::VST; ++s) {
@@ -233,17 +233,37 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + C::O_Q + uint32_t(s) * RT_SLAB + uint32_t(e) * 16u), "r"(0) : "memory");
     fence_proxy_async();
   }
-  RaggedStart* sh_start = reinterpret_cast<RaggedStart*>(smem + C::O_START);
-  int32_t* sh_strides = reinterpret_cast<int32_t*>(smem + C::O_START + sizeof(RaggedStart));
-  if (warp == 2) {
-    if (!p.few) ragged_wait_before();
-    const RaggedStart s = p.few ? ragged_start_few(p, blockIdx.x, lane, sh_strides)
-                                : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
-    if (lane == 0) *sh_start = s;
-  }
-  if (warp == 0) {
+  if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  // The producer finds the CTA's first part while the others set up: from here to the first scores is a chain of loads
+  int32_t* sh_strides = reinterpret_cast<int32_t*>(smem + C::O_STRIDES);
+  RtWalker w = {};
+  RtPart part = {};
+  bool more = false;
+  int id = 0;
+  const int page = p.table ? 1 << p.page_shift : RT_UNIT;
+  const int box = min(page, RT_UNIT), per_unit = RT_UNIT / box;      // rows of a copy, copies of a unit and 64 columns
+  const int my_page = lane % per_unit;
+  // this lane's page of unit u (the id; n_pages - behind the pool, zeros - where there is none)
+  auto page_of = [&](int u) {
+    if (!p.table || u >= part.units) return 0;
+    const int key = part.key0(u) + my_page * box;
+    if (key >= w.span.keys) return p.n_pages;
+    const int got = __ldg(p.table + w.req * p.table_stride + (key >> p.page_shift));
+    return got >= 0 && got < p.n_pages ? got : p.n_pages;
+  };
+  if (warp == 0) {
+    if (!p.few) ragged_wait_before();
+    const RaggedStart start = p.few ? ragged_start_few(p, blockIdx.x, lane, sh_strides)
+                                    : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
+    __syncwarp();
+    more = w.begin(p, start, sh_strides);
+    if (more) {
+      w.order(p, part);
+      id = page_of(0);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -257,12 +277,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(RT_REGS_CONTROL));
     if (warp == 0) {
       // ---------------------------------------------------------- producer (whole warp; lane 0 waits and announces)
-      RtWalker w = {};
-      RtPart part = {};
-      const RaggedStart start = *sh_start;
-      const int page = p.table ? 1 << p.page_shift : RT_UNIT;
-      const int box = min(page, RT_UNIT), per_unit = RT_UNIT / box;      // rows of a copy, copies of a unit and 64 columns
-      const int my_page = lane % per_unit, my_slab = lane / per_unit;
+      const int my_slab = lane / per_unit;
       const bool copies = my_slab < C::SLABS;
       const uint32_t my_dst = uint32_t(my_slab) * RT_SLAB + uint32_t(my_page * box) * 128u;
       const uint32_t q_bytes = uint32_t(p.stream_tokens * p.chunk_heads) * 128u * C::SLABS;
@@ -270,14 +285,6 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         bool ok = true;
         if (lane == 0) ok = mbar_wait(bar(b), parity, abort_flag);
         return __shfl_sync(0xffffffffu, ok, 0);
-      };
-      // this lane's page of unit u (the id; n_pages - behind the pool, zeros - where there is none)
-      auto page_of = [&](int u) {
-        if (!p.table || u >= part.units) return 0;
-        const int key = part.key0(u) + my_page * box;
-        if (key >= w.span.keys) return p.n_pages;
-        const int id = __ldg(p.table + w.req * p.table_stride + (key >> p.page_shift));
-        return id >= 0 && id < p.n_pages ? id : p.n_pages;
       };
       auto load = [&](const CUtensorMap* map, int full, uint32_t tile, int key, int id, int kvh) {
         if (lane == 0) mbar_expect_tx(bar(full), C::TILE);
@@ -314,18 +321,16 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ++q_n[h];
         return true;
       };
-      for (bool more = w.begin(p, start, sh_strides); ok && more; more = w.next(p), ++pieces) {
-        w.order(p, part);
+      while (ok && more) {
         part.both = w.item.n_tok > p.stream_tokens;
         part.n_tok = w.item.n_tok; part.heads = w.item.heads; part.pos0 = w.item.pos0; part.keys = w.span.keys;
         part.low = p.window > 0 ? w.item.pos0 - p.window + 1 : 0;
         part.out = ragged_out(p, w.q, w.item, 0, 0, D);
         ok = announce(pieces, part);
-        if (ok) ok = load_q(0);
-        if (ok && part.both) ok = load_q(1);
+        // Q before the first K unit: the other way round a windowed prompt takes 4% longer
+        if (ok) ok = load_q(0) && (!part.both || load_q(1));
         if (!ok) break;
-        int id = page_of(0);
-        for (int u = 0; u < w.units; ++u) {
+        for (int u = 0; u < part.units; ++u) {
           const int key = part.key0(u), id_next = page_of(u + 1);
           const int s = k_i % C::KST;
           ok = wait0(C::B_KEMPTY + s, ((k_i / C::KST) & 1) ^ 1);
@@ -347,6 +352,12 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           id = id_next;
         }
         if (ok) ok = load_v();
+        ++pieces;
+        more = w.next(p);
+        if (more) {
+          w.order(p, part);
+          id = page_of(0);
+        }
       }
       if (ok) {
         part.units = 0;
@@ -380,7 +391,8 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const bool both = parts[n % RT_PARTS].both != 0, mine = h == 0 || both;
           mbar_arrive(bar(C::B_PEMPTY + n % RT_PARTS));
           if (units == 0) break;
-          // Step u: P V of unit u and Q K^T of unit u + 1, the two groups back to back; step -1 has only the latter
+          // Step u: P V of unit u and Q K^T of unit u + 1, the two groups back to back.  Step -1 has only the latter and
+          // takes no turn: stream A's next item must not wait for stream B's last softmax
           if (mine) ok = mbar_wait(bar(C::B_QFULL + h), nq++ & 1, abort_flag);
           for (int u = -1; ok && u < units; ++u) {
             const bool pv = u >= 0, qk = u + 1 < units;
@@ -392,7 +404,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               RtSteps vd, qd, kd;
               if (pv) fetch(C::DT_V + 8 * vs, vd);
               if (qk) { fetch(8 * h, qd); fetch(C::DT_K + 8 * ks, kd); }
-              if (both) ok = mbar_wait(bar(C::B_TOKEN + h), step & 1, abort_flag);
+              if (both && pv) ok = mbar_wait(bar(C::B_TOKEN + h), step & 1, abort_flag);
               if (ok && pv) ok = mbar_wait(bar(C::B_PREADY + h), np & 1, abort_flag);
               if (!ok) break;
               tc_fence_after();
@@ -402,7 +414,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 if (!qk) tc_commit(bar(C::B_ODONE + h));
               }
               if (qk) { rt_mma_qk<C::KSTEPS>(ts, qd, kd, ID_QK); tc_commit(bar(C::B_SFULL + h)); }
-              if (both) { mbar_arrive(bar(C::B_TOKEN + (h ^ 1))); ++step; }
+              if (both && pv) { mbar_arrive(bar(C::B_TOKEN + (h ^ 1))); ++step; }
             }
             if (pv) release(C::B_VEMPTY + vs, mine);
             if (qk) {
@@ -628,7 +640,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
