@@ -316,7 +316,7 @@ int spf_paged_write(const void* k, int64_t k_stride_n, int64_t k_stride_h,
  *   request past it need not be computed.  cu_new and seq_len are clipped to the batch on the device.
  *   Keys that a request does not see are not read, or not used, whatever they hold (NaN included), except that
  *   a NaN or infinity in a VALUE row that some token of a chunk sees can reach the chunk's other tokens.
- *   out and scratch start on 32-byte boundaries.
+ *   out and scratch start on 32-byte boundaries and overlap no input.  There is no backward pass.
  *   scratch: spf_paged_scratch_bytes() bytes, overwritten; calls that may run at the same
  *   time need their own.
  */

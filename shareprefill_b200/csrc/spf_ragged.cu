@@ -6,10 +6,11 @@
 namespace spf {
 
 // ---------------------------------------------------------------- schedule
-// Every block sums the units of every request (a warp per request, its lanes over the tiles), scans the
-// sums, and each of its warps finds the start of one CTA: request by binary search, head by division, tile
+// Every block sums the units of every request (a thread per request of one tile, a warp, its lanes over the tiles, per
+// larger one), scans the sums, and each of its warps finds the start of one CTA: request by binary search, head by division, tile
 // by a scan over the tiles.
-constexpr int SCH_NT = 1024, SCH_WARPS = SCH_NT / 32;
+// (blocks of 1024 threads, so of 32 starts, put the whole work on a few SMs: 15 us for 512 windowed tiles)
+constexpr int SCH_NT = 256, SCH_WARPS = SCH_NT / 32;
 constexpr int FEW_REQUESTS = 32, FEW_TILES = 512;
 
 __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedParams p) {
@@ -17,30 +18,44 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
   __shared__ long long wsum[SCH_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.n_kv_heads * p.head_chunks;
-  for (int r = warp; r < p.n_requests; r += SCH_WARPS) {
+  int more = 0;
+  for (int r = threadIdx.x; r < p.n_requests; r += SCH_NT) {
     const RaggedReq q = ragged_req_plain(p, r);
     const int tiles = ragged_tiles(p, q.n);
-    long long s = 0;
-    for (int t = lane; t < tiles; t += 32) s += ragged_span(p, q, t).total;
-    s = warp_sum_ll(s);
-    if (lane == 0) upto[r] = s * heads;
+    upto[r] = tiles > 1 ? -1 : tiles == 1 ? (long long)ragged_span(p, q, 0).total * heads : 0;
+    more |= tiles > 1;
   }
-  __syncthreads();
+  if (__syncthreads_or(more)) {
+    for (int r = warp; r < p.n_requests; r += SCH_WARPS) {
+      if (upto[r] >= 0) continue;
+      const RaggedReq q = ragged_req_plain(p, r);
+      const int tiles = ragged_tiles(p, q.n);
+      long long s = 0;
+#pragma unroll 4
+      for (int t = lane; t < tiles; t += 32) s += ragged_span(p, q, t).total;
+      s = warp_sum_ll(s);
+      if (lane == 0) upto[r] = s * heads;
+    }
+    __syncthreads();
+  }
   long long carry = 0;
   for (int r0 = 0; r0 < p.n_requests; r0 += SCH_NT) {
     const int r = r0 + threadIdx.x;
     long long v = warp_scan_ll(r < p.n_requests ? upto[r] : 0, lane);
     if (lane == 31) wsum[warp] = v;
     __syncthreads();
-    if (warp == 0) wsum[lane] = warp_scan_ll(wsum[lane], lane);
+    if (warp == 0) {
+      const long long t = warp_scan_ll(lane < SCH_WARPS ? wsum[lane] : 0, lane);
+      if (lane < SCH_WARPS) wsum[lane] = t;
+    }
     __syncthreads();
     if (warp > 0) v += wsum[warp - 1];
     if (r < p.n_requests) upto[r] = v + carry;
     carry += wsum[SCH_WARPS - 1];
     __syncthreads();
   }
-  const long long all = carry, per = max((all + p.n_ctas - 1) / p.n_ctas, 1ll);
-  auto head_units = [&](int r) { return (upto[r] - (r > 0 ? upto[r - 1] : 0)) / heads; };
+  const long long all = carry, per = max(div_ll(all + p.n_ctas - 1, p.n_ctas), 1ll);
+  auto head_units = [&](int r) { return div_ll(upto[r] - (r > 0 ? upto[r - 1] : 0), heads); };
   if (blockIdx.x == 0 && p.window > 0)
     for (int r = threadIdx.x; r < p.n_requests; r += SCH_NT)
       ragged_strides(p)[r] = ragged_stride(per, ragged_tiles(p, ragged_req_plain(p, r).n), head_units(r));

@@ -203,18 +203,36 @@ __device__ __forceinline__ RaggedStart ragged_cut(const RaggedParams& p, int req
   s.req = req;
   s.head = int(div_ll(u - before, a_head));
   long long rem = (u - before) - a_head * s.head;
-  for (int t0 = 0; t0 < tiles; t0 += 32) {
-    const int cost = t0 + lane < tiles ? ragged_span(p, q, t0 + lane).total : 0;
-    const long long inc = warp_scan_ll(cost, lane);
-    const unsigned above = __ballot_sync(0xffffffffu, inc > rem);
+  for (int t0 = 0; t0 < tiles; t0 += 128) {          // four tiles a lane: their spans are independent, the scan is not
+    const int mine = t0 + 4 * lane;
+    int cost[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cost[i] = mine + i < tiles ? ragged_span(p, q, mine + i).total : 0;
+      sum += cost[i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned above = __ballot_sync(0xffffffffu, upto > rem);
     if (above) {
       const int at = __ffs(above) - 1;
-      s.tile = t0 + at;
-      s.item_units = __shfl_sync(0xffffffffu, cost, at);
-      s.first = int(rem - __shfl_sync(0xffffffffu, inc - cost, at));
+      rem -= __shfl_sync(0xffffffffu, upto - sum, at);
+      s.tile = t0 + 4 * at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = __shfl_sync(0xffffffffu, cost[i], at);
+        if (s.item_units == 0) {
+          if (rem < c) { s.item_units = c; s.first = int(rem); }
+          else { rem -= c; ++s.tile; }
+        }
+      }
       break;
     }
-    rem -= __shfl_sync(0xffffffffu, inc, 31);
+    rem -= __shfl_sync(0xffffffffu, upto, 31);
   }
   s.units = int(min(per, all - u));
   s.taken = s.first > 0 ? s.first - int(div_ll(s.first - 1, per) * per) : 0;
@@ -240,6 +258,7 @@ __device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, i
       o.n = __shfl_sync(0xffffffffu, q.n, r); o.seq = __shfl_sync(0xffffffffu, q.seq, r);
       const int n_tiles = ragged_tiles(p, o.n);
       int part = 0;
+#pragma unroll 4
       for (int t = lane; t < n_tiles; t += 32) part += ragged_span(p, o, t).total;
       const long long all = warp_sum_ll(part);
       if (lane == r) sum = all;

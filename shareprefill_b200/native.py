@@ -453,8 +453,9 @@ def paged_plan(cached_len, new_len, block_table, free_ring, ring_state, n_rows: 
         _i32(ring_state_out, "ring_state_out", dev)
         if ring_state_out.numel() != 2:
             raise SpfError("ring_state_out must hold two words")
-    if n_rows < 0:
-        raise SpfError("n_rows must not be negative")
+    n_rows = int(n_rows)
+    if not 0 <= n_rows < 1 << 31:
+        raise SpfError(f"n_rows must be a row count (got {n_rows})")
     # one allocation: slots first (8 bytes each), then the 4-byte outputs
     words = cached_len.new_empty(3 * n_rows + 3 * r + 3)
     slots, cu_new, seq_len, refused, positions, state = torch.split_with_sizes(words, [2 * n_rows, r + 1, r, r, n_rows, 2])
@@ -463,7 +464,7 @@ def paged_plan(cached_len, new_len, block_table, free_ring, ring_state, n_rows: 
     slot_map = slots.view(torch.int64)
     at = words.data_ptr()
     ints = at + 8 * n_rows
-    _check(load().spf_paged_plan(cached_len.data_ptr(), new_len.data_ptr(), r, page_size, block_table.data_ptr(), step, width,
+    _check(load().spf_paged_plan(cached_len.data_ptr(), new_len.data_ptr(), r, _c_int(page_size), block_table.data_ptr(), step, width,
                                  free_ring.data_ptr(), free_ring.numel(), ring_state.data_ptr(), ring_state_out.data_ptr(),
                                  ints, ints + 4 * (r + 1), at, ints + 4 * (3 * r + 1), ints + 4 * (2 * r + 1), n_rows,
                                  _raw_stream(dev)), "spf_paged_plan")
@@ -513,9 +514,16 @@ def paged_write(k, v, slot_map, k_cache, v_cache) -> None:
     _launched(1)
 
 
+def _c_int(x) -> int:
+    """x as a C int; what is larger than any length is the largest one (ctypes would drop its upper bits)."""
+    return min(int(x), 0x7fffffff)
+
+
 def _attention_out(q, out):
     if out is None:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.data_ptr() == q.data_ptr() and q.numel():
+        raise SpfError("out must not be q: rows are written while others are still read")
     if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or out.device != q.device:
         raise SpfError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}")
     return out
@@ -544,11 +552,12 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
     if cu_new.numel() != r + 1 or hd != d:
         raise SpfError(f"paged_attention: {r} lengths, {cu_new.numel()} offsets; head size {d} of q, {hd} of the cache")
     out = _attention_out(q, out)
+    max_new = _c_int(max_new)
     need = lib.spf_paged_scratch_bytes(max_new, h, hkv, d)
     scratch = torch.empty(need or 32, dtype=torch.uint8, device=dev)
     _check(lib.spf_paged_attention(qp, qn, qh, n, h, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1],
                                    vs[2], pages, page_size, hkv, d, _DTYPE_CODE[dtype], block_table.data_ptr(), step, width,
-                                   cu_new.data_ptr(), seq_len.data_ptr(), r, max_new, softmax_scale, window, sinks,
+                                   cu_new.data_ptr(), seq_len.data_ptr(), r, max_new, softmax_scale, _c_int(window), _c_int(sinks),
                                    out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)), "spf_paged_attention")
     _launched(2)
     return out
@@ -574,7 +583,7 @@ def window_attention(q, k, v, softmax_scale: float, window: int, sinks: int = 0,
     need = lib.spf_paged_scratch_bytes(n or 1, h, hkv, d)
     scratch = torch.empty(need or 32, dtype=torch.uint8, device=dev)
     _check(lib.spf_window_attention(qp, qn, qh, kp, kn, kh, vp, vn, vh, n, keys, h, hkv, d, _DTYPE_CODE[dtype], softmax_scale,
-                                    window, sinks, out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)),
+                                    _c_int(window), _c_int(sinks), out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)),
            "spf_window_attention")
     _launched(2)
     return out

@@ -263,6 +263,33 @@ def test_peaked_scores_and_expanded_caches(new, gain):
     assert bool(((got.double().cpu() - out).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("new,heads", [(1, 2), (90, 2), (33, 80)])
+def test_caches_that_no_tensor_map_describes(new, heads):
+    # keys expanded over heads and tokens (strides of 0) take the other kernel, at any number of rows
+    dim = 64
+    g = torch.Generator().manual_seed(19)
+    q = torch.randn(new, heads, dim, generator=g).to(FP16)
+    k, v = (torch.randn(300, 1, dim, generator=g).to(FP16) for _ in range(2))
+    out, mass = R.attention(q, k.expand(-1, 2, -1), v.expand(-1, 2, -1), 300 - new, 0.2, 50, 3)
+    got = native.window_attention(q.cuda(), k.cuda().expand(-1, 2, -1), v.cuda().expand(-1, 2, -1), 0.2, 50, 3)
+    R.check(got, out, mass, FP16, 300, 5.0)
+    one = k[:1].cuda().expand(300, 2, -1)                 # every token the same key and value
+    got = native.window_attention(q.cuda(), one, one, 0.2, 50, 3)
+    assert float((got.cpu().double() - k[0].double()).abs().max()) <= 2 ** -10 * float(k[0].abs().max())
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_numbers_of_other_types_and_beyond_an_int(new):
+    import numpy as np
+    g = torch.Generator().manual_seed(29)
+    q = torch.randn(new, 4, 64, generator=g).to(BF16)
+    k, v = (torch.randn(200, 2, 64, generator=g).to(BF16) for _ in range(2))
+    out, mass = R.attention(q, k, v, 200 - new, 0.125, 0, 0)
+    for window, sinks in ((2 ** 31, 0), (2 ** 32 + 1, 2 ** 40), (np.int64(2 ** 30), np.int32(3)), (np.int64(0), 5), (1, 2 ** 33)):
+        got = native.window_attention(q.cuda(), k.cuda(), v.cuda(), np.float64(0.125), window, sinks)
+        R.check(got, out, mass, BF16, 200, 5.0, f"{window} {sinks}")
+
+
 # ---------------------------------------------------------------------------------- run together
 def test_a_serving_loop_plan_write_attend_over_pages():
     page, heads, kv_heads, dim, dtype, window, sinks = 16, 8, 2, 128, BF16, 60, 3
@@ -331,6 +358,67 @@ def test_captured_graphs_replay_with_new_lengths_side_by_side(new):
                 R.check(s["out"][cu[r]:cu[r + 1]], *want[i][r], BF16, 400, 5.0, f"graph {i} request {r} cut {cut}")
 
 
+def test_a_whole_step_captured_and_replayed():
+    # plan, write and attention in one graph: lengths, rows and the ring's state live in its buffers
+    page, heads, kv_heads, dim, dtype, rows = 16, 8, 2, 64, BF16, 24
+    g = torch.Generator().manual_seed(37)
+    k_cache, v_cache = (torch.full((40, page, kv_heads, dim), float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    table = torch.full((3, 12), -1, dtype=torch.int32, device="cuda")
+    ring, state, seq, fresh = torch.randperm(40, generator=g).to(torch.int32).cuda(), _ints([38, 40]), _ints([0, 0, 0]), _ints([0, 0, 0])
+    q = torch.zeros(rows, heads, dim, dtype=dtype, device="cuda")
+    k, v = (torch.zeros(rows, kv_heads, dim, dtype=dtype, device="cuda") for _ in range(2))
+
+    def step():
+        plan = native.paged_plan(seq, fresh, table, ring, state, rows, page, ring_state_out=state)
+        native.paged_write(k, v, plan.slot_map, k_cache, v_cache)
+        out = native.paged_attention(q, k_cache, v_cache, table, plan.cu_new, plan.seq_len, 10, 0.125, 40, 2)
+        seq.copy_(plan.seq_len)
+        return out
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()                                            # no tokens: warms up, changes nothing
+    torch.cuda.synchronize()
+    assert state.tolist() == [38, 40]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    history = [(torch.empty(0, kv_heads, dim, dtype=dtype),) * 2 for _ in range(3)]
+    for new in ([10, 3, 0], [1, 1, 9], [10, 1, 10], [1, 0, 1], [7, 10, 1]):
+        rows_q = torch.randn(rows, heads, dim, generator=g).to(dtype)
+        rows_k, rows_v = (torch.randn(rows, kv_heads, dim, generator=g).to(dtype) for _ in range(2))
+        q.copy_(rows_q), k.copy_(rows_k), v.copy_(rows_v), fresh.copy_(_ints(new))
+        graph.replay()
+        at = 0
+        for r, n in enumerate(new):
+            hk, hv = history[r]
+            history[r] = (torch.cat([hk, rows_k[at:at + n]]), torch.cat([hv, rows_v[at:at + n]]))
+            if n:
+                want, mass = R.attention(rows_q[at:at + n], *history[r], len(hk), 0.125, 40, 2)
+                R.check(out[at:at + n], want, mass, dtype, 100, 5.0, f"{new} request {r}")
+            at += n
+    assert seq.tolist() == [len(h[0]) for h in history]
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_calls_on_two_streams_at_once(new):
+    batches = []
+    for i in range(2):
+        pool, cu, q = _batch([(900 + 300 * i, new), (50, new)], 16, 8, 2, 128, BF16, "token", 50 + i)
+        k, v = pool.cuda()
+        args = (q.cuda(), k, v, pool.table.cuda(), _ints(cu), _ints([900 + 300 * i + new, 50 + new]), new, 128 ** -0.5)
+        batches.append((args, native.paged_attention(*args), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, (args, _, stream) in enumerate(batches):
+            with torch.cuda.stream(stream):
+                outs[i].append(native.paged_attention(*args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, batches[i][1]) for x in outs[i])
+
+
 def test_results_do_not_depend_on_the_run_or_the_stream():
     pool, cu, q = _batch([(3000, 1), (777, 1), (20, 1)], 16, 32, 8, 128, BF16, "token", 41)
     k, v = pool.cuda()
@@ -364,7 +452,7 @@ def test_wrong_arguments_are_refused():
                    dict(cu_new=cu.long()), dict(seq_len=seq.cpu()), dict(block_table=t[:1]), dict(block_table=t.t()),
                    dict(max_new=0), dict(softmax_scale=float("nan")), dict(softmax_scale=-1.0), dict(window=-1), dict(sinks=-1),
                    dict(k_cache=c[:, :10], v_cache=c[:, :10]), dict(k_cache=c[..., :96], v_cache=c[..., :96]),
-                   dict(out=torch.zeros(4, 8, 64, dtype=BF16, device="cuda")), dict(q=q[..., ::2]),
+                   dict(out=torch.zeros(4, 8, 64, dtype=BF16, device="cuda")), dict(out=q), dict(q=q[..., ::2]),
                    dict(k_cache=c[..., 4:68], v_cache=c[..., 4:68], q=q[..., :64])):
         with pytest.raises(native.SpfError):
             native.paged_attention(change.pop("q", q), **{**ok, **change})
