@@ -296,22 +296,29 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     const int all_hi = pos0, all_lo = p.window > 0 ? pos0 + p.tile_tokens - p.window : 0;
     const int any_lo = p.window > 0 ? pos0 - p.window + 1 : 0;   // keys below it that are no sinks are seen by no row
 
-    // step u of this warp: 16 keys from key0(u); their page, -1 if absent
-    auto key0 = [&](int u) {
-      const int s = first + u, unit = s < span.sink_units ? s : span.win_first + s - span.sink_units;
-      return unit * (RR_TT * RR_NW) + warp * RR_TT;
+    // step u of this warp: 16 keys from `k0` that count up to `end`; `first_keys`: of the sinks
+    struct Step { int k0, end; bool first_keys; };
+    const bool plain = span.sink_units == 0 && span.embed == 0;
+    const int plain_k0 = span.win_key + first * (RR_TT * RR_NW) + warp * RR_TT;
+    auto step_of = [&](int u) {
+      if (plain) return Step{plain_k0 + u * (RR_TT * RR_NW), span.keys, false};
+      const int s = first + u, col = (s < span.sink_units ? s : s - span.sink_units) * (RR_TT * RR_NW) + warp * RR_TT;
+      if (s < span.sink_units || col < span.embed) return Step{col, span.sink_keys, true};
+      return Step{span.win_key + col, span.keys, false};
     };
+    // its page, -1 if absent
     auto page_of = [&](int u) -> int {
       if (u >= units) return -1;
-      const int k0 = key0(u);
-      if (k0 >= span.keys) return -1;
+      const Step x = step_of(u);
+      if (x.k0 >= x.end) return -1;
       if (!table) return 0;
-      const int pg = __ldg(table + (k0 >> p.page_shift));
+      const int pg = __ldg(table + (x.k0 >> p.page_shift));
       return pg >= 0 && pg < p.n_pages ? pg : -1;
     };
     auto issue = [&](int u, int page, int stage) {
       if (u < units) {
-        const int k0 = key0(u), valid = page >= 0 ? span.keys - k0 : 0;
+        const Step x = step_of(u);
+        const int k0 = x.k0, valid = page >= 0 ? x.end - k0 : 0;
         const int in_page = table ? k0 & ((1 << p.page_shift) - 1) : k0;
         const uint32_t ks = ring + stage * (2 * TILE_B), vs = ks + TILE_B;
         const uint16_t* kp = kb + (valid > 0 ? page * p.k_sp + in_page * p.k_st : 0);
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
         for (int i = lane; i < RR_TT * CH; i += 32) {
           const int row = i / CH, ch = i % CH;
           // keys that no row of the item sees are not read: whatever they hold, 0 times it must stay 0
-          const bool ok = row < valid && (k0 + row >= any_lo || k0 + row < p.sinks);
+          const bool ok = row < valid && (x.first_keys || k0 + row >= any_lo || k0 + row < p.sinks);
           cp_async16(ks + tile_off<D>(row, ch), kp + (ok ? row * p.k_st + ch * 8 : 0), ok);
           cp_async16(vs + tile_off<D>(row, ch), vp + (ok ? row * p.v_st + ch * 8 : 0), ok);
         }
@@ -346,7 +353,8 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
       cp_async_wait<2>();
       __syncwarp();
       if (page >= 0) {
-        const int k0 = key0(u);
+        const Step x = step_of(u);
+        const int k0 = x.k0;
         const uint32_t ks_base = ring + stage * (2 * TILE_B), vs_base = ks_base + TILE_B;
         float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -356,7 +364,7 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
           mma_16816<FP16>(s[0], qa[ks], b[0], b[1]);
           mma_16816<FP16>(s[1], qa[ks], b[2], b[3]);
         }
-        if (k0 >= all_lo && k0 + RR_TT - 1 <= all_hi) {
+        if (!x.first_keys && k0 >= all_lo && k0 + RR_TT - 1 <= all_hi) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -368,14 +376,14 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
             for (int e = 0; e < 4; ++e) {
               const int key = k0 + j * 8 + cq + (e & 1);
               const int hi = e < 2 ? hi0 : hi1, lo = e < 2 ? lo0 : lo1;
-              s[j][e] = key <= hi && (key >= lo || key < p.sinks) && key < span.keys ? s[j][e] * p.scale_log2 : -INFINITY;
+              s[j][e] = key <= hi && (key >= lo || key < p.sinks) && key < x.end ? s[j][e] * p.scale_log2 : -INFINITY;
             }
         }
-        float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-        float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1)); x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        float y0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        float y1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+        y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 1)); y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 2));
+        y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 1)); y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 2));
+        const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
         const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet: all weights are 0
         const float a0 = exp2f(m0 - f0), a1 = exp2f(m1 - f1);
         m0 = n0; m1 = n1;
@@ -467,6 +475,7 @@ void ragged_rows_config(RaggedParams& p) {
   p.tile_tokens = p.stream_tokens = RR_ROWS / p.chunk_heads;
   p.unit_shift = 6;
   static_assert(RR_TT * RR_NW == 64, "keys of a unit");
+  p.granule = RR_TT;      // a warp's step lies in one page
   p.n_ctas = 2 * 148;
 }
 

@@ -39,6 +39,8 @@ struct RaggedParams {
   int stream_rows, stream_tokens;            // an item's rows come in streams (one MMA tile each) of stream_tokens tokens
   int tile_rows, tile_tokens, unit_shift, n_ctas;  // tile_rows / stream_rows streams an item; log2 of the keys of a unit
   int only;                                  // requests of this launch: 0 all, 1 those of up to 16 rows per KV head, 2 the others
+  int granule;                               // keys (a power of two) at whose multiples a window's units may begin
+  int copy_rows;                             // keys of one TMA copy
   int few;                                   // every CTA finds its start itself (no schedule kernel)
   char* scratch;
 };
@@ -48,8 +50,10 @@ struct RaggedParams {
 // offset in the output, for the join.
 struct alignas(16) RaggedStart { int req, head, tile, first, units, item_units, taken, n_tok, heads, pad; long long out; };
 
-// units of one item: [0, sink_units) and then [win_first, win_first + total - sink_units)
-struct RaggedSpan { int total, sink_units, win_first, keys; };   // keys: exclusive end of the keys in view
+// Units of one item: [0, sink_units) are the keys from 0 on, of which those below sink_keys count; the others are the keys
+// from win_key on, up to `keys`.  Where the last units leave room, the window begins `embed` keys earlier and the first
+// `embed` columns hold the keys from 0 on instead (those below sink_keys count): four sinks cost no unit of their own.
+struct RaggedSpan { int total, sink_units, win_key, keys, sink_keys, embed; };
 
 // scratch: where the CTAs start, a stride per request, two partial tiles per CTA
 __host__ __device__ inline int ragged_starts_bytes(int n_ctas) { return (n_ctas * int(sizeof(RaggedStart)) + 255) & ~255; }
@@ -128,10 +132,15 @@ __device__ __forceinline__ RaggedSpan ragged_span(const RaggedParams& p, const R
   RaggedSpan s;
   s.keys = int(max(end, int64_t(0)));
   const int low = p.window > 0 ? max(first_pos - p.window + 1, 0) : 0;
-  const int rest = (1 << p.unit_shift) - 1, end_unit = (s.keys + rest) >> p.unit_shift;
-  s.win_first = min(low >> p.unit_shift, end_unit);
-  s.sink_units = min((p.sinks >> p.unit_shift) + ((p.sinks & rest) != 0), s.win_first);
-  s.total = max(s.sink_units + end_unit - s.win_first, 1);   // an item that sees nothing still has zeros to write
+  const int rest = (1 << p.unit_shift) - 1, grain = p.granule - 1;
+  s.win_key = min(low, s.keys) & ~grain;
+  s.sink_keys = min(p.sinks, s.win_key);
+  const int win_units = (s.keys - s.win_key + rest) >> p.unit_shift;
+  const int pad = (s.sink_keys + grain) & ~grain;
+  s.embed = pad <= (win_units << p.unit_shift) - (s.keys - s.win_key) ? pad : 0;
+  s.win_key -= s.embed;
+  s.sink_units = s.embed ? 0 : (s.sink_keys + rest) >> p.unit_shift;
+  s.total = max(s.sink_units + win_units, 1);   // an item that sees nothing still has zeros to write
   return s;
 }
 

@@ -10,7 +10,7 @@
 //               page that is not there is a copy from behind the pool, which fills zeros
 //   warps 1, 2  MMA issuers of the streams: S = Q K^T and O += P V (P from TMEM); the steps of the two leave in turn
 //               (a token goes back and forth), so that one stream's softmax runs under the other's products
-//   warp 3      rows of a V unit that no query of the item sees are set to zero before the unit is used: what lies
+//   warp 3      rows of V units at the edges that no query of the item sees are set to zero before the unit is used: what lies
 //               behind the sequence, between the sinks and the window, or in the future may hold NaN, and 0 * NaN
 //               would reach the output (scores of such keys are replaced, so K needs no such care)
 //   warps 4-7, 8-11  softmax of stream A, B: a thread owns a row; base-2 softmax in fp32 against a reference
@@ -38,7 +38,14 @@ struct alignas(16) RtPart {
   int units, units_a, key_a, key_b;           // units 0: no more parts
   int both, whole, slot, n_tok;               // stream B has rows; the item is whole, else its partial slot
   int heads, pos0, keys, low;                 // keys in [low, keys) or below sinks are seen by some row
+  int embed, sink_keys, sink_units, win_key;  // unit 0: columns below embed are keys from 0 on; the first sink_units units
+                                              // are sinks: of both count the keys below sink_keys
   long long out;                              // offset of the item's first token and head in the output
+  // some rows of V unit u must become zeros
+  __device__ bool edge(int u) const {
+    const int key = key0(u);
+    return key < low || key + 128 > keys;
+  }
   __device__ int key0(int u) const { return u < units_a ? key_a + u * 128 : key_b + (u - units_a) * 128; }
 };
 constexpr int RT_PARTS = 2;                          // announced parts
@@ -54,7 +61,7 @@ struct RtCfg {
   static constexpr int POLY = D == 128 ? 1 : 2;
   // barriers
   static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
-                       B_VREADY = B_VFULL + VST, B_VEMPTY = B_VREADY + VST, B_SFULL = B_VEMPTY + VST, B_PREADY = B_SFULL + 2,
+                       B_VEDGE = B_VFULL + VST, B_VEMPTY = B_VEDGE + VST, B_SFULL = B_VEMPTY + VST, B_PREADY = B_SFULL + 2,
                        B_ODONE = B_PREADY + 2, B_TOKEN = B_ODONE + 2, B_N = B_TOKEN + 2;
   static constexpr uint32_t O_TMEM = B_N * 8, O_ABORT = O_TMEM + 8, O_ABSENT = O_ABORT + 8,
                             O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_STRIDES = O_PART + RT_PARTS * sizeof(RtPart), O_DTAB = O_STRIDES + 32 * 4;
@@ -167,15 +174,17 @@ struct RtWalker {
     // an item whose start an earlier CTA runs through: that one took the last units, this part's are that many earlier
     const int from = whole ? (p.window > 0 ? 0 : done % span.total) : first == 0 ? span.total - units : first - taken;
     part.units = units; part.whole = whole; part.slot = first == 0 ? 1 : 0;
+    part.sink_units = min(max(span.sink_units - from, 0), units);
+    part.embed = from == 0 ? span.embed : 0;
+    part.sink_keys = span.sink_keys; part.win_key = span.win_key;
     if (from < span.sink_units) {             // sinks, then the window
-      part.units_a = min(span.sink_units - from, units);
+      part.units_a = part.sink_units;
       part.key_a = from * RT_UNIT;
-      part.key_b = span.win_first * RT_UNIT;
     } else {                                  // up to the end, then (a whole item) from the front
       part.units_a = min(span.total - from, units);
-      part.key_a = (span.win_first + from - span.sink_units) * RT_UNIT;
-      part.key_b = span.win_first * RT_UNIT;
+      part.key_a = span.win_key + (from - span.sink_units) * RT_UNIT;
     }
+    part.key_b = span.win_key;
   }
   int taken;    // units of the CTA's first item that the CTA where it starts runs through
 };
@@ -183,7 +192,8 @@ struct RtWalker {
 template <int D, bool FP16>
 __global__ void __launch_bounds__(RT_THREADS, 1)
 ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RaggedParams p) {
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k32,
+                  const __grid_constant__ CUtensorMap map_v32, const __grid_constant__ RaggedParams p) {
   using C = RtCfg<D>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t sbase = smem_addr(smem);
@@ -207,7 +217,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (int s = 0; s < RT_PARTS; ++s) { mbar_init(bar(C::B_PFULL + s), 1); mbar_init(bar(C::B_PEMPTY + s), 11); }
     for (int s = 0; s < C::KST; ++s) { mbar_init(bar(C::B_KFULL + s), 1); mbar_init(bar(C::B_KEMPTY + s), 2); }
     for (int s = 0; s < C::VST; ++s) {
-      mbar_init(bar(C::B_VFULL + s), 1); mbar_init(bar(C::B_VREADY + s), 1); mbar_init(bar(C::B_VEMPTY + s), 2);
+      mbar_init(bar(C::B_VFULL + s), 1); mbar_init(bar(C::B_VEDGE + s), 1); mbar_init(bar(C::B_VEMPTY + s), 2);
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(bar(C::B_QFULL + h), 1); mbar_init(bar(C::B_QEMPTY + h), 1);
@@ -243,13 +253,13 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   RtPart part = {};
   bool more = false;
   int id = 0;
-  const int page = p.table ? 1 << p.page_shift : RT_UNIT;
-  const int box = min(page, RT_UNIT), per_unit = RT_UNIT / box;      // rows of a copy, copies of a unit and 64 columns
-  const int my_page = lane % per_unit;
-  // this lane's page of unit u (the id; n_pages - behind the pool, zeros - where there is none)
+  const int box = p.copy_rows, per_unit = RT_UNIT / box;      // rows of a copy, copies of a unit and 64 columns
+  const int my_col = lane % per_unit * box;
+  // first key of this lane's copy of unit u, and its page (n_pages - behind the pool, zeros - where there is none)
+  auto key_of = [&](int u) { return u == 0 && my_col < part.embed ? my_col : part.key0(u) + my_col; };
   auto page_of = [&](int u) {
     if (!p.table || u >= part.units) return 0;
-    const int key = part.key0(u) + my_page * box;
+    const int key = key_of(u);
     if (key >= w.span.keys) return p.n_pages;
     const int got = __ldg(p.table + w.req * p.table_stride + (key >> p.page_shift));
     return got >= 0 && got < p.n_pages ? got : p.n_pages;
@@ -279,7 +289,8 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // ---------------------------------------------------------- producer (whole warp; lane 0 waits and announces)
       const int my_slab = lane / per_unit;
       const bool copies = my_slab < C::SLABS;
-      const uint32_t my_dst = uint32_t(my_slab) * RT_SLAB + uint32_t(my_page * box) * 128u;
+      const uint32_t my_dst = uint32_t(my_slab) * RT_SLAB + uint32_t(my_col) * 128u;
+      const int in_page = p.table ? (1 << p.page_shift) - 1 : -1;
       const uint32_t q_bytes = uint32_t(p.stream_tokens * p.chunk_heads) * 128u * C::SLABS;
       auto wait0 = [&](int b, int parity) {
         bool ok = true;
@@ -289,14 +300,30 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       auto load = [&](const CUtensorMap* map, int full, uint32_t tile, int key, int id, int kvh) {
         if (lane == 0) mbar_expect_tx(bar(full), C::TILE);
         __syncwarp();
-        if (copies) tma_load_4d(tile + my_dst, map, bar(full), my_slab * 64, p.table ? key & (page - 1) & ~(box - 1) : key, kvh, id);
+        if (copies) tma_load_4d(tile + my_dst, map, bar(full), my_slab * 64, key & in_page, kvh, id);
       };
+      // a unit of contiguous keys whose first columns are the keys from 0 on, 32 at a time
+      auto load_embedded = [&](const CUtensorMap* map, int full, uint32_t tile, int key, int embed, int kvh) {
+        if (lane == 0) mbar_expect_tx(bar(full), C::TILE);
+        __syncwarp();
+        const int col = (lane & 3) * 32, slab = lane >> 2;
+        if (slab < C::SLABS)
+          tma_load_4d(tile + uint32_t(slab) * RT_SLAB + uint32_t(col) * 128u, map, bar(full), slab * 64, col < embed ? col : key + col, kvh, 0);
+      };
+      int v_embed = 0;
+      bool v_edge = false;
+      uint32_t edges = 0, edge_last = 0;      // bits per V stage: parity of its edge units, whether its last unit was one
       int k_i = 0, v_i = 0, v_key = 0, v_id = 0, v_kvh = 0, pieces = 0;
       bool ok = true;
       auto load_v = [&]() {      // K runs one unit ahead of V
         const int s = v_i % C::VST;
         if (!wait0(C::B_VEMPTY + s, ((v_i / C::VST) & 1) ^ 1)) return false;
-        load(&map_v, C::B_VFULL + s, sbase + C::O_V + uint32_t(s) * C::TILE, v_key, v_id, v_kvh);
+        const uint32_t tile = sbase + C::O_V + uint32_t(s) * C::TILE;
+        const int full = (v_edge ? C::B_VEDGE : C::B_VFULL) + s;
+        if (v_embed) load_embedded(&map_v32, full, tile, v_key, v_embed, v_kvh);
+        else load(&map_v, full, tile, v_key, v_id, v_kvh);
+        edges ^= uint32_t(v_edge) << s;
+        edge_last = (edge_last & ~(1u << s)) | uint32_t(v_edge) << s;
         ++v_i;
         return true;
       };
@@ -331,7 +358,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (ok) ok = load_q(0) && (!part.both || load_q(1));
         if (!ok) break;
         for (int u = 0; u < part.units; ++u) {
-          const int key = part.key0(u), id_next = page_of(u + 1);
+          const int key = key_of(u), id_next = page_of(u + 1);
           const int s = k_i % C::KST;
           ok = wait0(C::B_KEMPTY + s, ((k_i / C::KST) & 1) ^ 1);
           if (!ok) break;
@@ -344,11 +371,15 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             absent_of[k_i % RT_ABSENT] = bits;
             __threadfence_block();
           }
-          load(&map_k, C::B_KFULL + s, sbase + C::O_K + uint32_t(s) * C::TILE, key, id, w.item.kvh);
+          const int embed = !p.table && u == 0 ? part.embed : 0;
+          if (embed) load_embedded(&map_k32, C::B_KFULL + s, sbase + C::O_K + uint32_t(s) * C::TILE, part.key_a, embed, w.item.kvh);
+          else load(&map_k, C::B_KFULL + s, sbase + C::O_K + uint32_t(s) * C::TILE, key, id, w.item.kvh);
           ++k_i;
           if (u > 0) ok = load_v();
           if (!ok) break;
-          v_key = key; v_id = id; v_kvh = w.item.kvh;
+          v_embed = embed;
+          v_edge = part.edge(u);
+          v_key = embed ? part.key_a : key; v_id = id; v_kvh = w.item.kvh;
           id = id_next;
         }
         if (ok) ok = load_v();
@@ -368,7 +399,11 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (int h = 0; h < 2; ++h)
           if (q_n[h] > 0) mbar_wait(bar(C::B_QFULL + h), (q_n[h] - 1) & 1, abort_flag, true);
         for (int j = max(0, k_i - C::KST); j < k_i; ++j) mbar_wait(bar(C::B_KFULL + j % C::KST), (j / C::KST) & 1, abort_flag, true);
-        for (int j = max(0, v_i - C::VST); j < v_i; ++j) mbar_wait(bar(C::B_VFULL + j % C::VST), (j / C::VST) & 1, abort_flag, true);
+        for (int j = max(0, v_i - C::VST); j < v_i; ++j) {
+          const int s = j % C::VST;
+          if (edge_last >> s & 1u) mbar_wait(bar(C::B_VEDGE + s), (edges >> s & 1u) ^ 1u, abort_flag, true);
+          else mbar_wait(bar(C::B_VFULL + s), (j / C::VST) & 1, abort_flag, true);
+        }
       }
     } else if (warp <= 2) {
       // ---------------------------------------------------------- MMA issuers
@@ -397,7 +432,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           for (int u = -1; ok && u < units; ++u) {
             const bool pv = u >= 0, qk = u + 1 < units;
             const int vs = (i + C::VST - 1) % C::VST, ks = i % C::KST;     // i: units of the CTA whose Q K^T has been issued
-            if (pv) ok = mbar_wait(bar(C::B_VREADY + vs), ((i - 1) / C::VST) & 1, abort_flag);
+            if (pv) ok = mbar_wait(bar(C::B_VFULL + vs), ((i - 1) / C::VST) & 1, abort_flag);
             if (ok && qk) ok = mbar_wait(bar(C::B_KFULL + ks), (i / C::KST) & 1, abort_flag);
             if (!ok) break;
             if (mine) {
@@ -427,8 +462,10 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
     } else {
       // ---------------------------------------------------------- V rows that no query of the item sees become zeros
+      // (such a unit's copies complete on a barrier of their own, and this warp's arrival makes the unit full)
       bool ok = true;
       int i = 0;
+      uint32_t edges = 0;       // a bit per stage: parity of its edge units
       for (int n = 0; ok; ++n) {
         ok = __all_sync(0xffffffffu, part_ready(n));
         if (!ok) break;
@@ -437,25 +474,25 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (lane == 0) mbar_arrive(bar(C::B_PEMPTY + n % RT_PARTS));
         if (part.units == 0) break;
         for (int u = 0; u < part.units; ++u, ++i) {
+          if (!part.edge(u)) continue;
           const int s = i % C::VST;
-          ok = mbar_wait(bar(C::B_VFULL + s), (i / C::VST) & 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(C::B_VEDGE + s), edges >> s & 1u, abort_flag));
           if (!ok) break;
+          edges ^= 1u << s;
           const int key = part.key0(u);
           const int tail = min(max(part.keys - key, 0), RT_UNIT);                                       // rows [tail, 128)
-          const int a = min(max(p.sinks - key, 0), RT_UNIT), b = min(max(part.low - key, 0), tail);     // and rows [a, b)
-          if (tail < RT_UNIT || a < b) {
-            const uint32_t base = sbase + C::O_V + uint32_t(s) * C::TILE;
-            for (int r = lane >> 3; r < RT_UNIT; r += 4)
-              if (r >= tail || (r >= a && r < b))
+          const int embed = u == 0 ? part.embed : 0;                                                    // rows [sink_keys, embed)
+          const int a = max(min(max(p.sinks - key, 0), RT_UNIT), embed), b = min(max(part.low - key, 0), tail);   // and [a, b)
+          const uint32_t base = sbase + C::O_V + uint32_t(s) * C::TILE;
+          for (int r = lane >> 3; r < RT_UNIT; r += 4)
+            if (r >= tail || (r >= a && r < b) || (r >= part.sink_keys && r < embed))
 #pragma unroll
-                for (int sl = 0; sl < C::SLABS; ++sl)
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
-                               ::"r"(base + uint32_t(sl) * RT_SLAB + uint32_t(r) * 128u + uint32_t(lane & 7) * 16u), "r"(0) : "memory");
-            fence_proxy_async();
-            __syncwarp();
-          }
-          if (lane == 0) mbar_arrive(bar(C::B_VREADY + s));
+              for (int sl = 0; sl < C::SLABS; ++sl)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                             ::"r"(base + uint32_t(sl) * RT_SLAB + uint32_t(r) * 128u + uint32_t(lane & 7) * 16u), "r"(0) : "memory");
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::B_VFULL + s));
         }
       }
     }
@@ -510,12 +547,16 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const uint32_t gone = absent_of[(seen_so_far >> 4) % RT_ABSENT];
         if (past || before || gone != 0u) {
           const Place x = place(part);
-          const int last = (x.in ? part.pos0 + x.tok : -1) - key;        // last column the row sees
-          const int a = max(p.sinks - key, 0), b = before ? last - p.window + 1 : 0;    // and not [a, b)
+          const int row_last = (x.in ? part.pos0 + x.tok : -1) - key;    // last column the row sees
+          const int last = u < part.sink_units ? min(row_last, part.sink_keys - 1 - key) : row_last;
+          const int a = max(p.sinks - key, 0), b = before ? row_last - p.window + 1 : 0;    // and not [a, b)
+          const int embed = u == 0 ? part.embed : 0, sinks = x.in ? part.sink_keys : 0;     // columns of the first keys, those that count
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             const uint32_t bad = (gone >> (2 * c) & 1u ? 0xffffu : 0u) | (gone >> (2 * c + 1) & 1u ? 0xffff0000u : 0u);
-            const uint32_t keep = low_bits(last + 1 - c * 32) & ~(low_bits(b - c * 32) & ~low_bits(a - c * 32)) & ~bad;
+            const uint32_t firsts = low_bits(embed - c * 32);
+            const uint32_t keep = ((low_bits(last + 1 - c * 32) & ~(low_bits(b - c * 32) & ~low_bits(a - c * 32)) & ~firsts) |
+                                   (low_bits(sinks - c * 32) & firsts)) & ~bad;
             if (__any_sync(0xffffffffu, keep != 0xffffffffu)) {
               float v[32];
               tmem_ld32(tS + c * 32, v);
@@ -656,6 +697,10 @@ void ragged_tc5_config(RaggedParams& p) {
   p.tile_tokens = 2 * p.stream_tokens;
   p.unit_shift = 7;
   static_assert(RT_UNIT == 128, "keys of a unit");
+  // A copy is a page or 128 keys; the unit of contiguous keys in which sinks stand first is copied 32 keys at a time
+  const int page = 1 << p.page_shift;
+  p.copy_rows = p.table && page < RT_UNIT ? page : RT_UNIT;
+  p.granule = p.table ? p.copy_rows : p.window > 0 && p.sinks > 0 ? 32 : 16;
   p.n_ctas = RT_CTAS;
 }
 
@@ -669,14 +714,14 @@ bool ragged_tc5_describable(const RaggedParams& p) {
 }
 
 // K or V as (d, token of the page, head, page); contiguous keys are one page
-static bool rt_map_kv(CUtensorMap* m, const RaggedParams& p, const void* base, int64_t sp, int64_t st, int64_t sh, int d) {
+static bool rt_map_kv(CUtensorMap* m, const RaggedParams& p, const void* base, int64_t sp, int64_t st, int64_t sh, int d, int rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   const int page = p.table ? 1 << p.page_shift : p.seq_one;
   const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(page), cuuint64_t(p.n_kv_heads), cuuint64_t(p.n_pages)};
   const cuuint64_t strides[3] = {cuuint64_t(st) * 2, cuuint64_t(p.n_kv_heads == 1 ? d : sh) * 2,
                                  cuuint64_t(!p.table || p.n_pages == 1 ? d : sp) * 2};
-  const cuuint32_t box[4] = {64, cuuint32_t(p.table && page < RT_UNIT ? page : RT_UNIT), 1, 1};
+  const cuuint32_t box[4] = {64, cuuint32_t(rows), 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   return fn(m, p.fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
             box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -698,13 +743,18 @@ static bool rt_map_q(CUtensorMap* m, const RaggedParams& p, int d) {
 
 template <int D, bool FP16>
 static int launch_tc5(const RaggedParams& p, cudaStream_t st) {
-  CUtensorMap mq, mk, mv;
-  if (!rt_map_q(&mq, p, D) || !rt_map_kv(&mk, p, p.k, p.k_sp, p.k_st, p.k_sh, D) || !rt_map_kv(&mv, p, p.v, p.v_sp, p.v_st, p.v_sh, D))
+  CUtensorMap mq, mk, mv, mk32, mv32;
+  if (!rt_map_q(&mq, p, D) || !rt_map_kv(&mk, p, p.k, p.k_sp, p.k_st, p.k_sh, D, p.copy_rows) ||
+      !rt_map_kv(&mv, p, p.v, p.v_sp, p.v_st, p.v_sh, D, p.copy_rows))
+    return SPF_ERR_SHAPE;
+  mk32 = mk; mv32 = mv;
+  if (!p.table && p.granule == 32 &&
+      (!rt_map_kv(&mk32, p, p.k, p.k_sp, p.k_st, p.k_sh, D, 32) || !rt_map_kv(&mv32, p, p.v, p.v_sp, p.v_st, p.v_sh, D, 32)))
     return SPF_ERR_SHAPE;
   const cudaError_t e = cudaFuncSetAttribute(ragged_tc5_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(RtCfg<D>::BYTES));
   if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
-  if (!p.few) return ragged_launch_after(ragged_tc5_kernel<D, FP16>, dim3(p.n_ctas), RT_THREADS, int(RtCfg<D>::BYTES), st, mq, mk, mv, p);
-  ragged_tc5_kernel<D, FP16><<<p.n_ctas, RT_THREADS, RtCfg<D>::BYTES, st>>>(mq, mk, mv, p);
+  if (!p.few) return ragged_launch_after(ragged_tc5_kernel<D, FP16>, dim3(p.n_ctas), RT_THREADS, int(RtCfg<D>::BYTES), st, mq, mk, mv, mk32, mv32, p);
+  ragged_tc5_kernel<D, FP16><<<p.n_ctas, RT_THREADS, RtCfg<D>::BYTES, st>>>(mq, mk, mv, mk32, mv32, p);
   return check_launch();
 }
 
