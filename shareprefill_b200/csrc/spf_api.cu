@@ -410,7 +410,7 @@ static bool few_rows(int group, int max_new) { return int64_t(group) * max_new <
 static int run_pass(RaggedParams p, bool tc5, int only, int max_new, int head_dim, cudaStream_t st) {
   p.only = only; p.head_dim = head_dim;
   if (tc5) ragged_tc5_config(p); else ragged_rows_config(p);
-  int rc = ragged_schedule(p, st);
+  int rc = ragged_schedule(p, max_new, st);
   if (rc == SPF_OK) rc = tc5 ? ragged_tc5_attention(p, head_dim, st) : ragged_rows_attention(p, head_dim, st);
   if (rc == SPF_OK) rc = ragged_merge(p, max_new, head_dim, st);
   return rc;

@@ -11,7 +11,7 @@ namespace spf {
 // by a scan over the tiles.
 // (blocks of 1024 threads, so of 32 starts, put the whole work on a few SMs: 15 us for 512 windowed tiles)
 constexpr int SCH_NT = 256, SCH_WARPS = SCH_NT / 32;
-constexpr int FEW_REQUESTS = 32, FEW_TILES = 512;
+constexpr int FEW_REQUESTS = 32, FEW_TILES = 512, FEW_SINGLES = 256;
 
 __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedParams p) {
   __shared__ long long upto[SPF_MAX_REQUESTS];   // inclusive sums over the requests
@@ -76,8 +76,10 @@ __global__ void __launch_bounds__(SCH_NT) ragged_schedule_kernel(const RaggedPar
   if (lane == 0) reinterpret_cast<RaggedStart*>(p.scratch)[c] = s;
 }
 
-int ragged_schedule(RaggedParams& p, cudaStream_t st) {
-  p.few = p.n_requests <= FEW_REQUESTS && p.n_rows / p.tile_tokens + p.n_requests <= FEW_TILES;
+int ragged_schedule(RaggedParams& p, int max_new, cudaStream_t st) {
+  p.few = 0;
+  if (p.n_requests <= FEW_REQUESTS && p.n_rows / p.tile_tokens + p.n_requests <= FEW_TILES) p.few = 1;
+  else if (p.n_requests <= FEW_SINGLES && max_new <= p.tile_tokens && p.tile_rows <= RAGGED_FEW_ROWS) p.few = 2;
   if (p.few) return SPF_OK;
   ragged_schedule_kernel<<<ceil_div(p.n_ctas, SCH_WARPS), SCH_NT, 0, st>>>(p);
   return check_launch();
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
   __shared__ int32_t sh_strides[FEW_REQUESTS];
   if (p.few) {
     if (warp == 0) {
-      const RaggedStart s = ragged_start_few(p, blockIdx.x, lane, sh_strides);
+      const RaggedStart s = p.few == 1 ? ragged_start_few(p, blockIdx.x, lane, sh_strides) : ragged_start_singles(p, blockIdx.x, lane);
       if (lane == 0) sh_start = s;
     }
     __syncthreads();

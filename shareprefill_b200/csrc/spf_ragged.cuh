@@ -41,7 +41,8 @@ struct RaggedParams {
   int only;                                  // requests of this launch: 0 all, 1 those of up to 16 rows per KV head, 2 the others
   int granule;                               // keys (a power of two) at whose multiples a window's units may begin
   int copy_rows;                             // keys of one TMA copy
-  int few;                                   // every CTA finds its start itself (no schedule kernel)
+  int few;                                   // every CTA finds its start itself (no schedule kernel): 1 few requests and tiles,
+                                             // 2 requests of one tile (what max_new says)
   char* scratch;
 };
 
@@ -105,12 +106,14 @@ __device__ __forceinline__ RaggedReq ragged_req_plain(const RaggedParams& p, int
 __device__ __forceinline__ RaggedReq ragged_req(const RaggedParams& p, int r, const int32_t* own) {
   RaggedReq q = ragged_req_plain(p, r);
   if (p.window > 0) {
-    if (p.few) q.stride = own[r]; else q.stride = __ldg(ragged_strides(p) + r);
+    if (p.few == 1) q.stride = own[r]; else if (p.few == 0) q.stride = __ldg(ragged_strides(p) + r);
   }
   return q;
 }
 
-__device__ __forceinline__ int ragged_tiles(const RaggedParams& p, int n) { return (n + p.tile_tokens - 1) / p.tile_tokens; }
+__device__ __forceinline__ int ragged_tiles(const RaggedParams& p, int n) {
+  return p.few == 2 ? n > 0 : (n + p.tile_tokens - 1) / p.tile_tokens;
+}
 
 // Tile `at` of a request's part of the line.  With a window a tile's keys are near its tokens only, and CTAs that run at
 // the same time should be at neighbouring tiles: `stride`, the tiles that a CTA runs through, makes the line go
@@ -252,7 +255,7 @@ __device__ __forceinline__ RaggedStart ragged_cut(const RaggedParams& p, int req
 }
 
 // The schedule of a short line (up to 32 requests, few tiles), found by one warp of every CTA for itself: a kernel less.
-// Leaves the strides in `strides` [32] and, for the join, the start and (CTA 0) the strides in the scratch.
+// Leaves the strides in `strides` [32] and, for the join, the start in the scratch.
 __device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, int c, int lane, int32_t* strides) {
   const int heads = p.n_kv_heads * p.head_chunks;
   RaggedReq q = {};
@@ -280,7 +283,6 @@ __device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, i
   if (p.window > 0) {
     q.stride = ragged_stride(per, tiles, sum);
     strides[lane] = q.stride;
-    if (c == 0 && lane < p.n_requests) ragged_strides(p)[lane] = q.stride;
   }
   RaggedStart s = {};
   if (u < all) {
@@ -290,6 +292,39 @@ __device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, i
     o.n = __shfl_sync(0xffffffffu, q.n, at); o.seq = __shfl_sync(0xffffffffu, q.seq, at); o.stride = __shfl_sync(0xffffffffu, q.stride, at);
     const long long a_head = __shfl_sync(0xffffffffu, sum, at), end = __shfl_sync(0xffffffffu, upto, at);
     s = ragged_cut(p, at, o, end - a_head * heads, a_head, u, per, all, lane);
+  }
+  if (lane == 0) reinterpret_cast<RaggedStart*>(p.scratch)[c] = s;
+  return s;
+}
+
+// The same for requests of one tile each (single tokens; a decode batch of 64 requests up to 8K: 226 us with the schedule
+// kernel, 218 without): a lane adds up the units of its run of requests, and those of the run in
+// which the CTA starts are looked at again, one a lane.
+__device__ __forceinline__ RaggedStart ragged_start_singles(const RaggedParams& p, int c, int lane) {
+  const int heads = p.n_kv_heads * p.head_chunks, run = (p.n_requests + 31) / 32;
+  auto units_of = [&](int r, RaggedReq& q) {
+    q = ragged_req_plain(p, r);
+    return q.n > 0 ? ragged_span(p, q, 0).total : 0;
+  };
+  long long sum = 0;
+  RaggedReq q;
+#pragma unroll 4
+  for (int i = 0; i < run; ++i)
+    if (lane * run + i < p.n_requests) sum += units_of(lane * run + i, q);
+  long long upto = warp_scan_ll(sum * heads, lane);
+  const long long all = __shfl_sync(0xffffffffu, upto, 31), per = max(div_ll(all + p.n_ctas - 1, p.n_ctas), 1ll), u = per * c;
+  RaggedStart s = {};
+  if (u < all) {
+    const int at = __ffs(__ballot_sync(0xffffffffu, upto > u)) - 1;
+    const long long before = __shfl_sync(0xffffffffu, upto - sum * heads, at);
+    const int r = at * run + lane, mine = lane < run && r < p.n_requests ? units_of(r, q) : 0;
+    upto = before + warp_scan_ll((long long)mine * heads, lane);
+    const int own = __ffs(__ballot_sync(0xffffffffu, upto > u)) - 1;
+    RaggedReq o;
+    o.row0 = __shfl_sync(0xffffffffu, q.row0, own);
+    o.n = __shfl_sync(0xffffffffu, q.n, own); o.seq = __shfl_sync(0xffffffffu, q.seq, own); o.stride = 1;
+    const long long a_head = __shfl_sync(0xffffffffu, mine, own), end = __shfl_sync(0xffffffffu, upto, own);
+    s = ragged_cut(p, at * run + own, o, end - a_head * heads, a_head, u, per, all, lane);
   }
   if (lane == 0) reinterpret_cast<RaggedStart*>(p.scratch)[c] = s;
   return s;
@@ -307,7 +342,7 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 #endif  // __CUDACC__
 
 // decides whether the CTAs find their starts themselves, launches the schedule kernel if not
-int ragged_schedule(RaggedParams& p, cudaStream_t st);
+int ragged_schedule(RaggedParams& p, int max_new, cudaStream_t st);
 int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t st);
 // up to 16 packed rows an item: bandwidth bound (single tokens); also what TMA cannot describe
 void ragged_rows_config(RaggedParams& p);

@@ -192,6 +192,19 @@ def test_offsets_and_lengths_that_lie_are_clipped():
         _check_batch(got, spec, pool, cu, q, dim ** -0.5, 0, 0, BF16)
 
 
+@pytest.mark.parametrize("requests", [5, 40, 300])
+def test_a_request_longer_than_max_new_says_leaves_the_others_right(requests):
+    # 16 rows a tile are two tokens of eight heads: three tokens are more than one tile where one token was promised
+    spec = [(10 + 7 * i, 3 if i == 3 else 1) for i in range(requests)]
+    pool, cu, q = _batch(spec, 16, 8, 1, 64, BF16, "token", requests)
+    k, v = pool.cuda()
+    got = native.paged_attention(q.cuda(), k, v, pool.table.cuda(), _ints(cu), _ints([c + n for c, n in spec]), 1, 0.125)
+    for r, (c, n) in enumerate(spec):
+        if r != 3:
+            out, mass = R.attention(q[cu[r]:cu[r + 1]], *pool.rows[r], c, 0.125)
+            R.check(got[cu[r]:cu[r + 1]], out, mass, BF16, c + n, 5.0, f"request {r}")
+
+
 @pytest.mark.parametrize("new", [1, 200])
 def test_cache_of_more_than_32_bits_of_elements(new):
     page, heads, kv_heads, dim = 64, 8, 8, 128
