@@ -3,14 +3,14 @@
  *
  * The reference (opas-lab/SharePrefill) is pure Python and has no FFI; every entry
  * point below replaces a Python function of the reference's prefill attention path,
- * cited as file:line within that project.
+ * cited as file:line within that project, but for those that say they have no counterpart there.
  *
  * Conventions
  *   - Batch is 1 per call (the reference's sharing state assumes it,
- *     attn/attention_sharing.py:42-44); callers loop over the batch.
+ *     attn/attention_sharing.py:42-44); callers loop over the batch.  The paged group takes batches.
  *   - All pointers are DEVICE pointers unless marked "host".  The caller owns every
  *     buffer (inputs, outputs, scratch, sharing state); nothing here allocates.
- *   - q/k/v/avg tensors are bf16 with the head dimension contiguous; token and head
+ *   - q/k/v/avg tensors are bf16 (paged and windowed operators: bf16 or fp16) with the head dimension contiguous; token and head
  *     strides are given in ELEMENTS and must be multiples of 8 (16-byte rows).
  *   - `stream` is a cudaStream_t passed as void*; work is enqueued, never synchronised.
  *   - Every function returns SPF_OK (0) or a negative spf_status; nothing throws,

@@ -14,7 +14,9 @@ namespace spf {
 // ceil((c + n) / P), and the ids it lacks come from the free ring in the order of the requests.  One
 // cluster: every CTA scans all requests (a few numbers each) into shared memory, then the CTAs share the
 // rows and the table's new entries.  Between the two lies a cluster barrier, so an output may be the
-// array that an input was.
+// array that an input was.  Bound by latency: 6.4 us for 8 requests, 13 us for 512 requests and 37K rows (0.3 MB), of
+// which the scan and the rows' binary searches in shared memory are most; a single CTA would write the rows at
+// an eighth of the rate, and a grid of more needs a second launch for the scan.
 constexpr int PLAN_CTAS = 8, PLAN_NT = 512, PLAN_WARPS = PLAN_NT / 32;
 
 __device__ __forceinline__ long long warp_scan_long(long long v, int lane) {   // inclusive
