@@ -34,7 +34,7 @@ extern "C" {
 #define SPF_MAX_BLOCKS 8192
 #define SPF_MAX_HEADS 256
 #define SPF_MAX_REQUESTS 4096       /* requests of one paged batch */
-#define SPF_MAX_KEYS (1 << 30)      /* tokens of one sequence */
+#define SPF_MAX_KEYS (1 << 28)      /* tokens of one sequence */
 
 typedef enum spf_status {
   SPF_OK = 0,

@@ -38,7 +38,7 @@ struct alignas(16) RtPart {
   int units, units_a, key_a, key_b;           // units 0: no more parts
   int both, whole, slot, n_tok;               // stream B has rows; the item is whole, else its partial slot
   int heads, pos0, keys, low;                 // keys in [low, keys) or below sinks are seen by some row
-  int embed, sink_keys, sink_units, win_key;  // unit 0: columns below embed are keys from 0 on; the first sink_units units
+  int embed, sink_keys, sink_units, pad;      // unit 0: columns below embed are keys from 0 on; the first sink_units units
                                               // are sinks: of both count the keys below sink_keys
   long long out;                              // offset of the item's first token and head in the output
   // some rows of V unit u must become zeros
@@ -60,11 +60,13 @@ struct RtCfg {
   // 147 / 140 / 207 us
   static constexpr int POLY = D == 128 ? 1 : 2;
   // barriers
-  static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
+  static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 2,
+                       B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
                        B_VEDGE = B_VFULL + VST, B_VEMPTY = B_VEDGE + VST, B_SFULL = B_VEMPTY + VST, B_PREADY = B_SFULL + 2,
                        B_ODONE = B_PREADY + 2, B_TOKEN = B_ODONE + 2, B_N = B_TOKEN + 2;
   static constexpr uint32_t O_TMEM = B_N * 8, O_ABORT = O_TMEM + 8, O_ABSENT = O_ABORT + 8,
-                            O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_STRIDES = O_PART + RT_PARTS * sizeof(RtPart), O_DTAB = O_STRIDES + 32 * 4;
+                            O_PART = (O_ABSENT + RT_ABSENT * 4 + 15) & ~15u, O_STRIDES = O_PART + RT_PARTS * sizeof(RtPart),
+                            O_DTAB = O_STRIDES + 32 * 4;
   static constexpr int DT_K = 16, DT_V = DT_K + 8 * KST, DT_N = DT_V + 8 * VST;   // descriptors: 8 per tile, Q_A, Q_B, K.., V..
   static_assert(O_DTAB + DT_N * 8 <= RT_CTRL, "control region too small");
   static_assert(DT_N <= RT_THREADS, "a thread per descriptor");
@@ -176,7 +178,7 @@ struct RtWalker {
     part.units = units; part.whole = whole; part.slot = first == 0 ? 1 : 0;
     part.sink_units = min(max(span.sink_units - from, 0), units);
     part.embed = from == 0 ? span.embed : 0;
-    part.sink_keys = span.sink_keys; part.win_key = span.win_key;
+    part.sink_keys = span.sink_keys;
     if (from < span.sink_units) {             // sinks, then the window
       part.units_a = part.sink_units;
       part.key_a = from * RT_UNIT;

@@ -58,7 +58,7 @@ def plan(cached, new, table, width, ring, head, count, n_rows, page):
         c, n = max(c, 0), max(n, 0)
         held, total = -(-c // page), -(-(c + n) // page)
         end += n
-        fits = total <= width and end <= n_rows and c + n <= 1 << 30
+        fits = total <= width and end <= n_rows and c + n <= 1 << 28
         wanted += total - held if fits else 0
         ok = fits and (total == held or wanted <= count)
         if ok:

@@ -181,6 +181,35 @@ def test_rows_without_keys_absent_pages_and_rows_behind_the_batch(new):
     assert bool((got[cu[3]:] == 7).all()), "rows behind the batch were touched"
 
 
+@pytest.mark.parametrize("new,page,window,sinks", [(1, 16, 90, 20), (50, 16, 90, 20), (50, 64, 90, 70), (200, 32, 120, 5), (60, 128, 100, 150)])
+def test_absent_pages_among_sinks_and_window(new, page, window, sinks):
+    heads, kv_heads, dim, dtype = 8, 2, 64, FP16
+    spec = [(400, new), (700, new)]
+    pool, cu, q = _batch(spec, page, heads, kv_heads, dim, dtype, "token", new)
+    k, v = pool.cuda()
+    table, present = pool.table.clone(), []
+    for r, gone in enumerate(([0, 2], [0, (700 - 60) // page, (700 - 20) // page])):
+        present.append(torch.ones(spec[r][0] + new, dtype=torch.bool))
+        for i in gone:
+            table[r, i] = -1
+            present[r][i * page:(i + 1) * page] = False
+    got = native.paged_attention(q.cuda(), k, v, table.cuda(), _ints(cu), _ints([c + n for c, n in spec]), new, 0.125, window, sinks)
+    _check_batch(got, spec, pool, cu, q, 0.125, window, sinks, dtype, present)
+
+
+def test_sinks_and_windows_of_every_relation():
+    # window edges and sinks on, before and behind the places where units, pages and copies begin
+    dim, g = 64, torch.Generator().manual_seed(71)
+    for new, keys in ((1, 400), (30, 400), (400, 400)):
+        q = torch.randn(new, 4, dim, generator=g).to(BF16)
+        k, v = (torch.randn(keys, 2, dim, generator=g).to(BF16) for _ in range(2))
+        for window in (1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 200, 399, 400, 401):
+            for sinks in (0, 1, 16, 31, 32, 33, 64, 127, 129, 390):
+                out, mass = R.attention(q, k, v, keys - new, 0.125, window, sinks)
+                got = native.window_attention(q.cuda(), k.cuda(), v.cuda(), 0.125, window, sinks)
+                R.check(got, out, mass, BF16, keys, 5.0, f"{new} new, window {window}, sinks {sinks}")
+
+
 def test_offsets_and_lengths_that_lie_are_clipped():
     page, heads, kv_heads, dim = 16, 8, 2, 64
     spec = [(30, 2)]

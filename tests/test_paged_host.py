@@ -26,7 +26,7 @@ def test_paged_attention_refusals():
     for bad in (dict(q=PTR + 8), dict(k=PTR + 2), dict(out=PTR + 4), dict(scratch=PTR + 1), dict(qn=1020), dict(kt=252),
                 dict(vh=4), dict(vp=4097)):
         assert _attention(**bad) == -3, bad
-    for bad in (dict(dtype=2), dict(dtype=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0),
+    for bad in (dict(dtype=2), dict(dtype=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0), dict(scale=1e-60), dict(scale=1e39),
                 dict(window=-1), dict(sinks=-1), dict(rows=-1), dict(pages=0), dict(req=0), dict(most=0), dict(tw=0), dict(ts=3),
                 dict(bytes=1)):
         assert _attention(**bad) == -4, bad
