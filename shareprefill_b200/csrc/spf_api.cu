@@ -432,7 +432,7 @@ int64_t spf_paged_scratch_bytes(int max_new, int n_q_heads, int n_kv_heads, int 
   if (max_new <= 0 || check_ragged(n_q_heads, n_kv_heads, head_dim, SPF_BF16, 1.0, 0, 0) != SPF_OK) return 0;
   RaggedParams p;
   std::memset(&p, 0, sizeof(p));
-  p.group = n_q_heads / n_kv_heads;
+  p.group = n_q_heads / n_kv_heads; p.head_dim = head_dim;
   ragged_rows_config(p);
   const int64_t rows = ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim);
   if (few_rows(p.group, max_new)) return rows;

@@ -7,6 +7,7 @@ library is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import NamedTuple, Optional
 
@@ -514,6 +515,12 @@ def paged_write(k, v, slot_map, k_cache, v_cache) -> None:
     _launched(1)
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(max_new: int, heads: int, kv_heads: int, dim: int) -> int:
+    """spf_paged_scratch_bytes; at least one line, so that a refused shape reaches the call that names it"""
+    return max(int(load().spf_paged_scratch_bytes(max_new, heads, kv_heads, dim)), 32)
+
+
 def _c_int(x) -> int:
     """x as a C int; what is larger than any length is the largest one (ctypes would drop its upper bits)."""
     return min(int(x), 0x7fffffff)
@@ -553,8 +560,8 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
         raise SpfError(f"paged_attention: {r} lengths, {cu_new.numel()} offsets; head size {d} of q, {hd} of the cache")
     out = _attention_out(q, out)
     max_new = _c_int(max_new)
-    need = lib.spf_paged_scratch_bytes(max_new, h, hkv, d)
-    scratch = torch.empty(need or 32, dtype=torch.uint8, device=dev)
+    need = _scratch_bytes(max_new, h, hkv, d)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
     _check(lib.spf_paged_attention(qp, qn, qh, n, h, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1],
                                    vs[2], pages, page_size, hkv, d, _DTYPE_CODE[dtype], block_table.data_ptr(), step, width,
                                    cu_new.data_ptr(), seq_len.data_ptr(), r, max_new, softmax_scale, _c_int(window), _c_int(sinks),
@@ -580,8 +587,8 @@ def window_attention(q, k, v, softmax_scale: float, window: int, sinks: int = 0,
         raise SpfError(f"window_attention: q/k/v must all be bfloat16 or all float16 on one device (got {dtype}, {k.dtype}, "
                        f"{v.dtype} on {dev}, {k.device}, {v.device})")
     out = _attention_out(q, out)
-    need = lib.spf_paged_scratch_bytes(n or 1, h, hkv, d)
-    scratch = torch.empty(need or 32, dtype=torch.uint8, device=dev)
+    need = _scratch_bytes(n or 1, h, hkv, d)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
     _check(lib.spf_window_attention(qp, qn, qh, kp, kn, kh, vp, vn, vh, n, keys, h, hkv, d, _DTYPE_CODE[dtype], softmax_scale,
                                     _c_int(window), _c_int(sinks), out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)),
            "spf_window_attention")
