@@ -142,8 +142,8 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 // The parts of items that a CTA runs through, in order, and the order of each part's units.
 // A CTA that runs through the START of its last item takes the item's LAST units, and the next CTAs, which begin
 // with the rest of it, take the units from the front; a whole item without a window starts at the unit whose
-// number is that of units done, and wraps.  So CTAs that have done equally many units stand at about the same
-// key of their items, and what one of them fetched the others find in L2.  (In the order of the keys, the last
+// number is that of units done (modulo those of the whole sequence), and wraps.  So CTAs that have done equally many
+// units stand at about the same key of their items, and what one of them fetched the others find in L2.  (In the order of the keys, the last
 // 2K chunk of a 34K prompt of 32 heads read its 143 MB of K and V 15 times from HBM: 2.1 GB.)
 struct RtWalker {
   int req, head, tile, first, left, units, done;
@@ -174,7 +174,11 @@ struct RtWalker {
   __device__ void order(const RaggedParams& p, RtPart& part) const {
     const bool whole = units == span.total;
     // an item whose start an earlier CTA runs through: that one took the last units, this part's are that many earlier
-    const int from = whole ? (p.window > 0 ? 0 : done % span.total) : first == 0 ? span.total - units : first - taken;
+    int from = first == 0 ? span.total - units : first - taken;
+    if (whole) {
+      from = p.window > 0 ? 0 : done % max((q.seq + RT_UNIT - 1) / RT_UNIT, 1);
+      if (from >= span.total) from = 0;
+    }
     part.units = units; part.whole = whole; part.slot = first == 0 ? 1 : 0;
     part.sink_units = min(max(span.sink_units - from, 0), units);
     part.embed = from == 0 ? span.embed : 0;
