@@ -55,10 +55,10 @@ struct RtCfg {
   static constexpr int SLABS = D / 64, KSTEPS = D / 16;
   static constexpr uint32_t TILE = RT_SLAB * SLABS;
   static constexpr int KST = D == 128 ? 3 : 6, VST = D == 128 ? 2 : 5;
-  // pairs of exponentials out of eight that go to the FMA pipe.  Measured with 1 / 2 / 3: at D = 128 the last 2K chunk of
-  // a 34K prompt takes 1030 / 1055 / 1287 us (3 spills), at D = 64, where the products take half the time, a mixed batch
-  // 147 / 140 / 207 us
+  // pairs of exponentials out of eight that go to the FMA pipe.  The last 2K chunk of a 34K prompt with 1 / 2 / 3: at
+  // D = 128 1030 / 1055 / 1287 us (3 spills), at D = 64 748 / 735 / 751 us
   static constexpr int POLY = D == 128 ? 1 : 2;
+  static constexpr bool P_BESIDE = D == 64;        // columns 384 .. 511 are free
   // barriers
   static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 2,
                        B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST,
@@ -415,7 +415,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // ---------------------------------------------------------- MMA issuers
       if (lane == 0) {
         const int h = warp - 1;
-        const uint32_t ts = tmem + (h == 0 ? 0u : 128u), to = tmem + 256u + uint32_t(h) * D;
+        const uint32_t ts = tmem + (h == 0 ? 0u : 128u), to = tmem + 256u + uint32_t(h) * D, tp = C::P_BESIDE ? tmem + 384u + uint32_t(h) * 64u : ts;
         constexpr uint32_t ID_QK = rt_idesc(FP16, 128, false), ID_PV = rt_idesc(FP16, D, true);
         auto fetch = [&](int first, RtSteps& o) {
           const ulonglong2* src = reinterpret_cast<const ulonglong2*>(dtab + first);
@@ -450,7 +450,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               if (!ok) break;
               tc_fence_after();
               if (pv) {
-                rt_mma_pv(to, ts, vd, ID_PV, u > 0 ? 1u : 0u);
+                rt_mma_pv(to, tp, vd, ID_PV, u > 0 ? 1u : 0u);
                 ++np;
                 if (!qk) tc_commit(bar(C::B_ODONE + h));
               }
@@ -512,6 +512,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // units does not need is looked up (in shared memory) or computed again where it is used.
     const int h = (warp - 4) >> 2;
     const uint32_t tS = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(h * 128);
+    auto p_tmem = [&]() { return tS + (C::P_BESIDE ? 384u - uint32_t(h) * 64u : 0u); };     // 384 + 64 h, or S itself
     auto o_tmem = [&]() { return tmem + (uint32_t((warp & 3) * 32) << 16) + 256u + uint32_t(h) * D; };
     // this thread's row: token of the item, head of the chunk, and whether the item has it
     struct Place { int tok, head; bool in; };
@@ -591,8 +592,9 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (m_used == -INFINITY) m_used = mb;
           fresh = __any_sync(0xffffffffu, m_used == -INFINITY);
         }
-        // P of the row, held in registers until its sum has been looked at: S stays in TMEM for the case that the reference
-        // has to move, and no more than three quarters of it are in registers
+        // S must stay in TMEM until the row's sum has been looked at, for the case that the reference has to move.  At D = 64
+        // there is room for P beside it; at D = 128 P is held in registers and then written over S.  Either way no more than
+        // three quarters of S are in registers.
         uint32_t pk0[16], pk1[16], pk2[16], pk3[16];
         float blk;
         bool moved = u == 0;
@@ -605,11 +607,15 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           tc_wait_ld();
           tmem_ld32_raw(tS + 64, s2);
           exp_pack_poly<C::POLY, FP16>(s0, p.scale_log2, ref, pk0, l0);
+          if (C::P_BESIDE) tmem_st16(p_tmem(), pk0);
           tmem_ld32_raw(tS + 96, s3);
           exp_pack_poly<C::POLY, FP16>(s1, p.scale_log2, ref, pk1, l1);
+          if (C::P_BESIDE) tmem_st16(p_tmem() + 16, pk1);
           tc_wait_ld();
           exp_pack_poly<C::POLY, FP16>(s2, p.scale_log2, ref, pk2, l2);
+          if (C::P_BESIDE) tmem_st16(p_tmem() + 32, pk2);
           exp_pack_poly<C::POLY, FP16>(s3, p.scale_log2, ref, pk3, l3);
+          if (C::P_BESIDE) tmem_st16(p_tmem() + 48, pk3);
           blk = (l0 + l1) + (l2 + l3);
           if (moved || !__any_sync(0xffffffffu, !(blk <= SUM_LIMIT))) break;
           moved = true;
@@ -630,7 +636,9 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tmem_st32(o_tmem() + c * 32, v);
           }
         }
-        tmem_st16(tS + 0, pk0); tmem_st16(tS + 16, pk1); tmem_st16(tS + 32, pk2); tmem_st16(tS + 48, pk3);
+        if (!C::P_BESIDE) {
+          tmem_st16(p_tmem(), pk0); tmem_st16(p_tmem() + 16, pk1); tmem_st16(p_tmem() + 32, pk2); tmem_st16(p_tmem() + 48, pk3);
+        }
         l_sum += blk;
         tc_wait_st();
         tc_fence_before();
