@@ -655,16 +655,21 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const float inv = m_used != -INFINITY && l_sum > 0.f ? 1.f / l_sum : 0.f;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + (x.in ? part.out + (int64_t(x.tok) * p.n_q_heads + x.head) * D : 0);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float v[32];
-          tmem_ld32(o_tmem() + c * 32, v);
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t r0[32], r1[32];
+          tmem_ld32_raw(o_tmem() + c * 64, r0);
+          tmem_ld32_raw(o_tmem() + c * 64 + 32, r1);
+          tc_wait_ld();
           if (x.in) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 4; ++j) {
               uint32_t o[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[e] = pack_half2<FP16>(v[16 * j + 2 * e] * inv, v[16 * j + 2 * e + 1] * inv);
-              store_32(dst + c * 32 + j * 16, o);
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t* v = j < 2 ? r0 + 16 * j : r1 + 16 * (j - 2);
+                o[e] = pack_half2<FP16>(__uint_as_float(v[2 * e]) * inv, __uint_as_float(v[2 * e + 1]) * inv);
+              }
+              store_32(dst + c * 64 + j * 16, o);
             }
           }
         }
