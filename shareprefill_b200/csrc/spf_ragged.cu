@@ -252,14 +252,13 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
   __shared__ RaggedStart sh_start;
   __shared__ int32_t sh_strides[FEW_REQUESTS];
+  ragged_wait_before();
   if (p.few) {
     if (warp == 0) {
       const RaggedStart s = p.few == 1 ? ragged_start_few(p, blockIdx.x, lane, sh_strides) : ragged_start_singles(p, blockIdx.x, lane);
       if (lane == 0) sh_start = s;
     }
     __syncthreads();
-  } else {
-    ragged_wait_before();
   }
   const RaggedStart start = p.few ? sh_start : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
   int left = start.units, req = start.req, head = start.head, tile = start.tile, first = start.first;
@@ -490,9 +489,7 @@ static int launch_rows(const RaggedParams& p, cudaStream_t st) {
   static_assert(SMEM >= RR_NW * (16 * (D + 8) + 32) * 4, "the join of the warps must fit in the rings");
   const cudaError_t e = cudaFuncSetAttribute(ragged_rows_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
-  if (!p.few) return ragged_launch_after(ragged_rows_kernel<D, FP16>, dim3(p.n_ctas), RR_NT, SMEM, st, p);
-  ragged_rows_kernel<D, FP16><<<p.n_ctas, RR_NT, SMEM, st>>>(p);
-  return check_launch();
+  return ragged_launch_after(ragged_rows_kernel<D, FP16>, dim3(p.n_ctas), RR_NT, SMEM, st, p);
 }
 
 int ragged_rows_attention(const RaggedParams& p, int head_dim, cudaStream_t st) {

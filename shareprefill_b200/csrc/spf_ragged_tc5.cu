@@ -207,6 +207,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (skewed || *reinterpret_cast<volatile unsigned int*>(&g_tc5_timeouts) > 16u) {
     if (threadIdx.x == 0) {
       if (skewed) atomicAdd(&g_tc5_timeouts, 1000u);
+      ragged_wait_before();
       reinterpret_cast<RaggedStart*>(p.scratch)[blockIdx.x] = RaggedStart{};      // nothing for the join to read
     }
     return;
@@ -271,7 +272,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     return got >= 0 && got < p.n_pages ? got : p.n_pages;
   };
   if (warp == 0) {
-    if (!p.few) ragged_wait_before();
+    ragged_wait_before();
     const RaggedStart start = p.few ? ragged_start_few(p, blockIdx.x, lane, sh_strides)
                                     : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
     __syncwarp();
@@ -772,9 +773,7 @@ static int launch_tc5(const RaggedParams& p, cudaStream_t st) {
     return SPF_ERR_SHAPE;
   const cudaError_t e = cudaFuncSetAttribute(ragged_tc5_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(RtCfg<D>::BYTES));
   if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
-  if (!p.few) return ragged_launch_after(ragged_tc5_kernel<D, FP16>, dim3(p.n_ctas), RT_THREADS, int(RtCfg<D>::BYTES), st, mq, mk, mv, mk32, mv32, p);
-  ragged_tc5_kernel<D, FP16><<<p.n_ctas, RT_THREADS, RtCfg<D>::BYTES, st>>>(mq, mk, mv, mk32, mv32, p);
-  return check_launch();
+  return ragged_launch_after(ragged_tc5_kernel<D, FP16>, dim3(p.n_ctas), RT_THREADS, int(RtCfg<D>::BYTES), st, mq, mk, mv, mk32, mv32, p);
 }
 
 int ragged_tc5_attention(const RaggedParams& p, int head_dim, cudaStream_t st) {
