@@ -343,6 +343,16 @@ int spf_window_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h,
                          double softmax_scale, int window, int sinks, void* out,
                          void* scratch, int64_t scratch_bytes, void* stream);
 
+/* spf_packed_call: one of the four calls above with its arguments as 64-bit words, in the order of its parameters (pointers
+ * and integers as they are, the scale by its bits, the stream last).  For bindings in which every argument of a foreign
+ * call costs; ctypes takes 3 us to convert the 32 of spf_paged_attention, 0.7 us for them as one string of bytes.
+ * words: host.  An int parameter whose word does not fit is SPF_ERR_RANGE. */
+#define SPF_PACKED_PAGED_PLAN 0
+#define SPF_PACKED_PAGED_WRITE 1
+#define SPF_PACKED_PAGED_ATTENTION 2
+#define SPF_PACKED_WINDOW_ATTENTION 3
+int spf_packed_call(int function, const void* words);
+
 /* ---------------------------------------------------------------- bounded device-side waits
  * The tcgen05 kernels never spin without a limit: a wait (on an mbarrier) that has been spinning for
  * longer than the wait limit makes its CTA drain and return - its rows of the output stay unwritten -

@@ -504,6 +504,40 @@ int spf_window_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, 
   return run_ragged(p, n_new, head_dim, scratch_bytes, static_cast<cudaStream_t>(stream));
 }
 
+int spf_packed_call(int function, const void* words) {
+  // kinds of the parameters: p pointer, l 64-bit integer, d double, i int
+  static const char* const kinds[4] = {"ppiiplipipppppppip", "pllpllpiiiplllpllliip", "plliiplllplll" "iiiii" "plippii" "diipplp",
+                                       "pllpllplliiiiiidiipplp"};
+  if (!words) return SPF_ERR_NULL;
+  if (function < 0 || function > 3) return SPF_ERR_RANGE;
+  int64_t w[32];
+  const int n = int(std::strlen(kinds[function]));
+  std::memcpy(w, words, size_t(n) * 8);
+  for (int i = 0; i < n; ++i)
+    if (kinds[function][i] == 'i' && w[i] != int64_t(int(w[i]))) return SPF_ERR_RANGE;
+  auto p = [&](int i) { return reinterpret_cast<void*>(w[i]); };
+  auto i32 = [&](int i) { return static_cast<int32_t*>(p(i)); };
+  auto i = [&](int k) { return int(w[k]); };
+  double d;
+  switch (function) {
+    case SPF_PACKED_PAGED_PLAN:
+      return spf_paged_plan(i32(0), i32(1), i(2), i(3), i32(4), w[5], i(6), i32(7), i(8), i32(9), i32(10), i32(11), i32(12),
+                            static_cast<int64_t*>(p(13)), i32(14), i32(15), i(16), p(17));
+    case SPF_PACKED_PAGED_WRITE:
+      return spf_paged_write(p(0), w[1], w[2], p(3), w[4], w[5], static_cast<int64_t*>(p(6)), i(7), i(8), i(9), p(10), w[11], w[12],
+                             w[13], p(14), w[15], w[16], w[17], i(18), i(19), p(20));
+    case SPF_PACKED_PAGED_ATTENTION:
+      std::memcpy(&d, &w[25], 8);
+      return spf_paged_attention(p(0), w[1], w[2], i(3), i(4), p(5), w[6], w[7], w[8], p(9), w[10], w[11], w[12], i(13), i(14), i(15),
+                                 i(16), i(17), i32(18), w[19], i(20), i32(21), i32(22), i(23), i(24), d, i(26), i(27), p(28), p(29),
+                                 w[30], p(31));
+    default:
+      std::memcpy(&d, &w[15], 8);
+      return spf_window_attention(p(0), w[1], w[2], p(3), w[4], w[5], p(6), w[7], w[8], i(9), i(10), i(11), i(12), i(13), i(14), d,
+                                  i(16), i(17), p(18), p(19), w[20], p(21));
+  }
+}
+
 int spf_device_timeouts(void) {
   const unsigned int n = tc5_timeout_count() + est_tc5_timeout_count() + ragged_tc5_timeout_count();
   g_known_timeouts.store(n, std::memory_order_relaxed);

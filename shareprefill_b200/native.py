@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import os
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -72,6 +73,7 @@ SIGNATURES = {
                                  _P, _P, _I, _I, _D, _I, _I, _P, _P, _L, _P]),
     "spf_window_attention": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _I, _D, _I, _I, _P, _P, _L,
                                   _P]),
+    "spf_packed_call": (_I, [_I, C.c_char_p]),
     "spf_update_pivots": (_I, [_P, _P, _P, _I, _I, _I, _D, _P]),
 }
 
@@ -394,6 +396,12 @@ def decode_attention(q, k, v, softmax_scale, out=None):
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
 
 
+# spf_packed_call: function number and arguments as words (bytes that Struct.pack makes)
+_PLAN, _WRITE, _PAGED, _WINDOW = range(4)
+_plan_words, _write_words = struct.Struct("18q").pack, struct.Struct("21q").pack
+_paged_words, _window_words = struct.Struct("25qd6q").pack, struct.Struct("15qd6q").pack
+
+
 class PagedPlan(NamedTuple):
     """What ``paged_plan`` found out: the row offsets, lengths, slots and positions of a step."""
     cu_new: torch.Tensor        # int32 [R + 1]
@@ -465,10 +473,11 @@ def paged_plan(cached_len, new_len, block_table, free_ring, ring_state, n_rows: 
     slot_map = slots.view(torch.int64)
     at = words.data_ptr()
     ints = at + 8 * n_rows
-    _check(load().spf_paged_plan(cached_len.data_ptr(), new_len.data_ptr(), r, _c_int(page_size), block_table.data_ptr(), step, width,
-                                 free_ring.data_ptr(), free_ring.numel(), ring_state.data_ptr(), ring_state_out.data_ptr(),
-                                 ints, ints + 4 * (r + 1), at, ints + 4 * (3 * r + 1), ints + 4 * (2 * r + 1), n_rows,
-                                 _raw_stream(dev)), "spf_paged_plan")
+    rc = load().spf_packed_call(_PLAN, _plan_words(
+        cached_len.data_ptr(), new_len.data_ptr(), r, _c_int(page_size), block_table.data_ptr(), step, width, free_ring.data_ptr(),
+        free_ring.numel(), ring_state.data_ptr(), ring_state_out.data_ptr(), ints, ints + 4 * (r + 1), at, ints + 4 * (3 * r + 1),
+        ints + 4 * (2 * r + 1), n_rows, _raw_stream(dev)))
+    _check(rc, "spf_paged_plan")
     _launched(1)
     return PagedPlan(cu_new, seq_len, slot_map, positions, refused, ring_state_out)
 
@@ -509,9 +518,10 @@ def paged_write(k, v, slot_map, k_cache, v_cache) -> None:
         raise SpfError(f"paged_write: rows {tuple(k.shape)} and {tuple(v.shape)} do not match caches {tuple(k_cache.shape)}")
     if slot_map.dtype is not torch.int64 or not slot_map.is_contiguous() or slot_map.numel() != n or slot_map.device != dev:
         raise SpfError(f"slot_map must be a contiguous int64 tensor of {n} slots on {dev}")
-    _check(load().spf_paged_write(kp, kn, kh, vp, vn, vh, slot_map.data_ptr(), n, h, d, k_cache.data_ptr(), ks[0], ks[1], ks[2],
-                                  v_cache.data_ptr(), vs[0], vs[1], vs[2], pages, page_size, _raw_stream(dev)),
-           "spf_paged_write")
+    rc = load().spf_packed_call(_WRITE, _write_words(
+        kp, kn, kh, vp, vn, vh, slot_map.data_ptr(), n, h, d, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1],
+        vs[2], pages, page_size, _raw_stream(dev)))
+    _check(rc, "spf_paged_write")
     _launched(1)
 
 
@@ -549,7 +559,6 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
     if ctx is not None:
         with ctx:
             return paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new, softmax_scale, window, sinks, out)
-    lib = load()
     qp, qn, qh = _rows(q, "q")
     (pages, page_size, hkv, hd), ks, vs = _paged_views(k_cache, v_cache, dtype, dev, "paged_attention")
     n, h, d = q.shape
@@ -562,10 +571,11 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
     max_new = _c_int(max_new)
     need = _scratch_bytes(max_new, h, hkv, d)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-    _check(lib.spf_paged_attention(qp, qn, qh, n, h, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1],
-                                   vs[2], pages, page_size, hkv, d, _DTYPE_CODE[dtype], block_table.data_ptr(), step, width,
-                                   cu_new.data_ptr(), seq_len.data_ptr(), r, max_new, softmax_scale, _c_int(window), _c_int(sinks),
-                                   out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)), "spf_paged_attention")
+    rc = load().spf_packed_call(_PAGED, _paged_words(
+        qp, qn, qh, n, h, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2], pages, page_size, hkv, d,
+        _DTYPE_CODE[dtype], block_table.data_ptr(), step, width, cu_new.data_ptr(), seq_len.data_ptr(), r, max_new, softmax_scale,
+        _c_int(window), _c_int(sinks), out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)))
+    _check(rc, "spf_paged_attention")
     _launched(2)
     return out
 
@@ -578,7 +588,6 @@ def window_attention(q, k, v, softmax_scale: float, window: int, sinks: int = 0,
     if ctx is not None:
         with ctx:
             return window_attention(q, k, v, softmax_scale, window, sinks, out)
-    lib = load()
     (qp, qn, qh), (kp, kn, kh), (vp, vn, vh) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
     (n, h, d), (keys, hkv, hd) = q.shape, k.shape
     if k.shape != v.shape or hd != d:
@@ -589,9 +598,10 @@ def window_attention(q, k, v, softmax_scale: float, window: int, sinks: int = 0,
     out = _attention_out(q, out)
     need = _scratch_bytes(n or 1, h, hkv, d)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-    _check(lib.spf_window_attention(qp, qn, qh, kp, kn, kh, vp, vn, vh, n, keys, h, hkv, d, _DTYPE_CODE[dtype], softmax_scale,
-                                    _c_int(window), _c_int(sinks), out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)),
-           "spf_window_attention")
+    rc = load().spf_packed_call(_WINDOW, _window_words(
+        qp, qn, qh, kp, kn, kh, vp, vn, vh, n, keys, h, hkv, d, _DTYPE_CODE[dtype], softmax_scale, _c_int(window), _c_int(sinks),
+        out.data_ptr(), scratch.data_ptr(), need, _raw_stream(dev)))
+    _check(rc, "spf_window_attention")
     _launched(2)
     return out
 

@@ -56,6 +56,35 @@ def test_window_plan_and_write_refusals():
     assert write(pages=0) == -4 and write(rows=-1) == -4 and write(kc=PTR + 8) == -3
 
 
+def test_packed_calls_are_the_calls():
+    import ctypes
+    import struct
+    lib = native.load()
+    kinds = {ctypes.c_void_p: "q", ctypes.c_int: "q", ctypes.c_int64: "q", ctypes.c_double: "d"}
+    for number, name in enumerate(("spf_paged_plan", "spf_paged_write", "spf_paged_attention", "spf_window_attention")):
+        types = native.SIGNATURES[name][1]
+        pack = struct.Struct("".join(kinds[t] for t in types)).pack
+        good = [PTR if t is ctypes.c_void_p else 0.1 if t is ctypes.c_double else 128 for t in types]
+        ints = [i for i, t in enumerate(types) if t is ctypes.c_int]
+        seen = set()
+        for change in [()] + [(i, v) for i in range(len(types)) for v in (-1, 0, 3, 1 << 40)]:
+            args = list(good)
+            if change:
+                if change[0] in ints and change[1] == 1 << 40:
+                    args[change[0]] = change[1]
+                    assert lib.spf_packed_call(number, pack(*args)) == -4
+                    continue
+                args[change[0]] = change[1] if types[change[0]] is not ctypes.c_double else float(change[1])
+            args[ints[-1]] = -1                       # whatever else it is, nothing is launched
+            if name in ("spf_paged_attention", "spf_window_attention"):
+                args[-2] = 0                          # scratch of no bytes
+            flat = getattr(lib, name)(*args)
+            assert lib.spf_packed_call(number, pack(*args)) == flat <= 0, (name, change)      # no rows: nothing to do
+            seen.add(flat)
+        assert len(seen) >= 2, name
+    assert lib.spf_packed_call(0, None) == -1 and lib.spf_packed_call(4, b"") == -4 and lib.spf_packed_call(-1, b"") == -4
+
+
 def test_scratch_grows_with_the_tile_not_with_the_lengths():
     lib = native.load()
     one, many = lib.spf_paged_scratch_bytes(1, 32, 8, 128), lib.spf_paged_scratch_bytes(1 << 20, 32, 8, 128)
