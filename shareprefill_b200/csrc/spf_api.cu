@@ -408,9 +408,16 @@ static int check_ragged(int n_q_heads, int n_kv_heads, int head_dim, int dtype, 
 // describe (strides of 0 in expanded views) go to the first kernel whole.
 static bool few_rows(int group, int max_new) { return int64_t(group) * max_new <= RAGGED_FEW_ROWS; }
 
+// Single tokens with a worker per warp instead of one per CTA: from this many items on, at D = 128.  us with a worker per CTA /
+// per warp, 32q/8kv: 64 requests up to 32 keys 18.6 / 16.9, 500 keys 39.6 / 32.1, 3000 91.1 / 90.3, 8192 215.9 / 215.9; 96
+// requests up to 500 keys 56.2 / 42.4; 32 requests up to 500 keys 27.5 / 23.0, but 3000 keys 50.1 / 52.4 and 8192 keys 112.5 /
+// 114.0.  At D = 64 (96 requests): 500 keys 34.5 / 33.6, 8192 keys 184.6 / 192.2.
+constexpr int SOLO_ITEMS = 512;
+
 static int run_pass(RaggedParams p, bool tc5, int only, int max_new, int head_dim, cudaStream_t st) {
   p.only = only; p.head_dim = head_dim;
-  if (tc5) ragged_tc5_config(p); else ragged_rows_config(p);
+  const bool solo = head_dim == 128 && few_rows(p.group, max_new) && p.n_requests * p.n_kv_heads >= SOLO_ITEMS;
+  if (tc5) ragged_tc5_config(p); else ragged_rows_config(p, solo);
   int rc = ragged_schedule(p, max_new, st);
   if (rc == SPF_OK) rc = tc5 ? ragged_tc5_attention(p, head_dim, st) : ragged_rows_attention(p, head_dim, st);
   if (rc == SPF_OK) rc = ragged_merge(p, max_new, head_dim, st);
@@ -433,7 +440,7 @@ int64_t spf_paged_scratch_bytes(int max_new, int n_q_heads, int n_kv_heads, int 
   RaggedParams p;
   std::memset(&p, 0, sizeof(p));
   p.group = n_q_heads / n_kv_heads; p.head_dim = head_dim;
-  ragged_rows_config(p);
+  ragged_rows_config(p, head_dim == 128);
   const int64_t rows = ragged_scratch_bytes(p.n_ctas, p.tile_rows, head_dim);
   if (few_rows(p.group, max_new)) return rows;
   ragged_tc5_config(p);

@@ -243,27 +243,38 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
   }
 }
 
-template <int D, bool FP16>
-__global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p) {
-  constexpr int CH = D / 8, TILE_B = RR_TT * D * 2;
+// SOLO: every warp is a worker with a part of the line of its own (in units of 16 keys) and no one to join with; for
+// batches with so many items that a CTA would run through several, one chain of loads after the other.
+template <int D, bool FP16, bool SOLO>
+__global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(const RaggedParams p) {
+  constexpr int CH = D / 8, TILE_B = RR_TT * D * 2, UNIT = SOLO ? RR_TT : RR_TT * RR_NW;
   extern __shared__ __align__(128) uint8_t rsm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(rsm) + warp * (RR_STAGES * 2 * TILE_B);
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
   __shared__ RaggedStart sh_start;
-  __shared__ int32_t sh_strides[FEW_REQUESTS];
+  __shared__ int32_t sh_strides[SOLO ? RR_NW : 1][FEW_REQUESTS];
+  const int worker = SOLO ? blockIdx.x * RR_NW + warp : blockIdx.x, part_col = SOLO ? 0 : warp * RR_TT;
+  int32_t* strides = sh_strides[SOLO ? warp : 0];
   ragged_wait_before();
-  if (p.few) {
-    if (warp == 0) {
-      const RaggedStart s = p.few == 1 ? ragged_start_few(p, blockIdx.x, lane, sh_strides) : ragged_start_singles(p, blockIdx.x, lane);
-      if (lane == 0) sh_start = s;
+  RaggedStart start;
+  if (!p.few) {
+    start = reinterpret_cast<const RaggedStart*>(p.scratch)[worker];
+  } else {
+    if (SOLO || warp == 0) {
+      start = p.few == 1 ? ragged_start_few(p, worker, lane, strides) : ragged_start_singles(p, worker, lane);
+      if (!SOLO && lane == 0) sh_start = start;
     }
-    __syncthreads();
+    if (SOLO) {
+      __syncwarp();
+    } else {
+      __syncthreads();
+      start = sh_start;
+    }
   }
-  const RaggedStart start = p.few ? sh_start : reinterpret_cast<const RaggedStart*>(p.scratch)[blockIdx.x];
   int left = start.units, req = start.req, head = start.head, tile = start.tile, first = start.first;
   if (left == 0) return;
-  RaggedReq q = ragged_req(p, req, sh_strides);
+  RaggedReq q = ragged_req(p, req, strides);
 
   while (true) {
     const RaggedSpan span = ragged_span(p, q, tile);
@@ -302,10 +313,10 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     // step u of this warp: 16 keys from `k0` that count up to `end`; `first_keys`: of the sinks
     struct Step { int k0, end; bool first_keys; };
     const bool plain = span.sink_units == 0 && span.embed == 0;
-    const int plain_k0 = span.win_key + first * (RR_TT * RR_NW) + warp * RR_TT;
+    const int plain_k0 = span.win_key + first * UNIT + part_col;
     auto step_of = [&](int u) {
-      if (plain) return Step{plain_k0 + u * (RR_TT * RR_NW), span.keys, false};
-      const int s = first + u, col = (s < span.sink_units ? s : s - span.sink_units) * (RR_TT * RR_NW) + warp * RR_TT;
+      if (plain) return Step{plain_k0 + u * UNIT, span.keys, false};
+      const int s = first + u, col = (s < span.sink_units ? s : s - span.sink_units) * UNIT + part_col;
       if (s < span.sink_units || col < span.embed) return Step{col, span.sink_keys, true};
       return Step{span.win_key + col, span.keys, false};
     };
@@ -416,6 +427,29 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     cp_async_wait<0>();
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    const bool whole = units == span.total;
+    float* part = ragged_part(p, worker, first == 0 ? 1 : 0, D);
+    if (SOLO) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!(half ? in1 : in0)) continue;
+        const int r = half ? r1 : r0;
+        const float l = half ? l1 : l0, inv = l > 0.f ? 1.f / l : 0.f;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, half ? t_r1 : t_r0, half ? h_r1 : h_r0, D) + cq;
+        if (!whole && (lane & 3) == 0) { part[r] = half ? m1 : m0; part[RR_ROWS + r] = l; }
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          const float x = o[j][2 * half], y = o[j][2 * half + 1];
+          if (whole) *reinterpret_cast<uint32_t*>(dst + j * 8) = pack_half2<FP16>(x * inv, y * inv);
+          else *reinterpret_cast<float2*>(part + 2 * RR_ROWS + r * D + j * 8 + cq) = make_float2(x, y);
+        }
+      }
+      left -= units;
+      if (left == 0) return;
+      first = 0;
+      if (!ragged_next(p, req, head, tile, q, strides)) return;
+      continue;
+    }
     __syncthreads();
 
     // join the warps through shared memory (the rings are drained)
@@ -435,8 +469,6 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     }
     __syncthreads();
     const float* all = reinterpret_cast<const float*>(rsm);
-    const bool whole = units == span.total;
-    float* part = ragged_part(p, blockIdx.x, first == 0 ? 1 : 0, D);
     for (int idx = threadIdx.x; idx < item.n_tok * p.chunk_heads * (D / 2); idx += RR_NT) {
       const int r = idx / (D / 2), d = (idx % (D / 2)) * 2, t = r / p.chunk_heads, h = r - t * p.chunk_heads;
       if (h >= item.heads) continue;
@@ -464,37 +496,41 @@ __global__ void __launch_bounds__(RR_NT) ragged_rows_kernel(const RaggedParams p
     left -= units;
     if (left == 0) return;
     first = 0;
-    if (!ragged_next(p, req, head, tile, q, sh_strides)) return;
+    if (!ragged_next(p, req, head, tile, q, strides)) return;
     __syncthreads();   // the buffers become rings again
   }
 }
 
 // As many CTAs as fit: at D = 128 two per SM (96 KiB of rings, 236 registers), at D = 64 three (156 registers).  A decode
 // batch of 64 requests up to 8K with D = 64 takes 145 / 129 / 173 us with 2 / 3 / 4 per SM, 133 with four of 128 registers.
-void ragged_rows_config(RaggedParams& p) {
+void ragged_rows_config(RaggedParams& p, bool solo) {
   p.tile_rows = RR_ROWS;
   p.head_chunks = ceil_div(p.group, RR_ROWS);
   p.chunk_heads = ceil_div(p.group, p.head_chunks);
   p.stream_rows = RR_ROWS;
   p.tile_tokens = p.stream_tokens = RR_ROWS / p.chunk_heads;
-  p.unit_shift = 6;
-  static_assert(RR_TT * RR_NW == 64, "keys of a unit");
+  p.solo = solo;
+  p.unit_shift = solo ? 4 : 6;
+  static_assert(RR_TT == 16 && RR_NW == 4, "keys of a unit");
   p.granule = RR_TT;      // a warp's step lies in one page
-  p.n_ctas = (p.head_dim == 64 ? 3 : 2) * 148;
+  p.n_ctas = (p.head_dim == 64 ? 3 : 2) * 148 * (solo ? RR_NW : 1);
 }
 
-template <int D, bool FP16>
+template <int D, bool FP16, bool SOLO>
 static int launch_rows(const RaggedParams& p, cudaStream_t st) {
   constexpr int SMEM = rr_smem_bytes<D>();
   static_assert(SMEM >= RR_NW * (16 * (D + 8) + 32) * 4, "the join of the warps must fit in the rings");
-  const cudaError_t e = cudaFuncSetAttribute(ragged_rows_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  const cudaError_t e = cudaFuncSetAttribute(ragged_rows_kernel<D, FP16, SOLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
-  return ragged_launch_after(ragged_rows_kernel<D, FP16>, dim3(p.n_ctas), RR_NT, SMEM, st, p);
+  return ragged_launch_after(ragged_rows_kernel<D, FP16, SOLO>, dim3(SOLO ? p.n_ctas / RR_NW : p.n_ctas), RR_NT, SMEM, st, p);
 }
 
 int ragged_rows_attention(const RaggedParams& p, int head_dim, cudaStream_t st) {
-  if (head_dim == 128) return p.fp16 ? launch_rows<128, true>(p, st) : launch_rows<128, false>(p, st);
-  return p.fp16 ? launch_rows<64, true>(p, st) : launch_rows<64, false>(p, st);
+  if (head_dim == 128) {
+    if (p.solo) return p.fp16 ? launch_rows<128, true, true>(p, st) : launch_rows<128, false, true>(p, st);
+    return p.fp16 ? launch_rows<128, true, false>(p, st) : launch_rows<128, false, false>(p, st);
+  }
+  return p.fp16 ? launch_rows<64, true, false>(p, st) : launch_rows<64, false, false>(p, st);
 }
 
 }  // namespace spf

@@ -41,6 +41,7 @@ struct RaggedParams {
   int only;                                  // requests of this launch: 0 all, 1 those of up to 16 rows per KV head, 2 the others
   int granule;                               // keys (a power of two) at whose multiples a window's units may begin
   int copy_rows;                             // keys of one TMA copy
+  int solo;                                  // bandwidth-bound kernel: a worker (of n_ctas) per warp
   int few;                                   // every CTA finds its start itself (no schedule kernel): 1 few requests and tiles,
                                              // 2 requests of one tile (what max_new says)
   char* scratch;
@@ -345,7 +346,8 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 int ragged_schedule(RaggedParams& p, int max_new, cudaStream_t st);
 int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t st);
 // up to 16 packed rows an item: bandwidth bound (single tokens); also what TMA cannot describe
-void ragged_rows_config(RaggedParams& p);
+// solo: a worker per warp instead of one per CTA (n_ctas counts the workers)
+void ragged_rows_config(RaggedParams& p, bool solo);
 int ragged_rows_attention(const RaggedParams& p, int head_dim, cudaStream_t st);
 // items of two 128-row MMA tiles on tcgen05 (spf_ragged_tc5.cu); SPF_ERR_SHAPE where TMA cannot describe the tensors
 void ragged_tc5_config(RaggedParams& p);

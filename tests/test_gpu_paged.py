@@ -125,6 +125,9 @@ CASES = [
     ([(3000, 64)] + [(i * 37, 1) for i in range(40)], 16, 8, 2, 128, BF16, 0, 0, "token"),
     ([(i * 29, 1 + 41 * (i % 3)) for i in range(45)], 32, 8, 2, 64, BF16, 90, 2, "head"),
     ([(700, 5), (0, 5), (33, 5)], 64, 16, 2, 128, FP16, 0, 0, "token"),                # all bring as many
+    ([(i * i % 700, i % 7 > 0) for i in range(70)], 16, 16, 8, 128, BF16, 0, 0, "token"),      # a worker per warp
+    ([(i * 13 % 900, 1 + i % 2) for i in range(260)], 16, 16, 2, 128, FP16, 120, 20, "head"),
+    ([(3000 + i, 1) for i in range(300)], 64, 2, 2, 128, BF16, 0, 0, "token"),
     ([(5, 2), (900, 1)], 16, 12, 1, 128, BF16, 0, 0, "token"),                         # 12 rows and 24
 ]
 

@@ -88,7 +88,7 @@ def test_packed_calls_are_the_calls():
 def test_scratch_grows_with_the_tile_not_with_the_lengths():
     lib = native.load()
     one, many = lib.spf_paged_scratch_bytes(1, 32, 8, 128), lib.spf_paged_scratch_bytes(1 << 20, 32, 8, 128)
-    assert 0 < one <= 16 << 20 and 0 < many <= 64 << 20
+    assert 0 < one <= 32 << 20 and 0 < many <= 64 << 20
     assert lib.spf_paged_scratch_bytes(0, 32, 8, 128) == 0 and lib.spf_paged_scratch_bytes(1, 32, 5, 128) == 0
 
 
