@@ -223,8 +223,8 @@ int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t 
 // The rows of an item are the 16 rows of mma.sync m16n8k16 tiles.  A unit is 64 keys, 16 per warp; every
 // warp streams its tiles through a private ring of cp.async stages and keeps its own running maximum, sum
 // and output; the warps meet when the CTA's part of the item ends.  Bound by HBM: 64 tokens of 32 heads over 8 KV heads
-// and up to 8K keys (1.33 GB) take 208 us, 6.4 TB/s; one token of 28 heads over 128K keys 50 us, 5.4 TB/s, of which 4 us are
-// launch and start and 3 the end.  Three stages of 16 keys per warp and two CTAs per SM keep 128 KiB of an SM in flight.
+// and up to 8K keys (1.33 GB) take 207 - 217 us, 6.1 - 6.4 TB/s; one token of 28 heads over 128K keys 49 us, 5.5 TB/s, of which
+// 4 us are launch and start and 3 the end.  Three stages of 16 keys per warp and two CTAs per SM keep 128 KiB of an SM in flight.
 constexpr int RR_NT = 128, RR_NW = RR_NT / 32, RR_TT = 16, RR_STAGES = 3, RR_ROWS = 16;
 
 template <int D>
@@ -243,6 +243,15 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
   }
 }
 
+__device__ __forceinline__ void cp_async16_all(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src));
+}
+__device__ __forceinline__ float ex2(float x) {      // 2^x; results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // SOLO: every warp is a worker with a part of the line of its own (in units of 16 keys) and no one to join with; for
 // batches with so many items that a CTA would run through several, one chain of loads after the other.
 template <int D, bool FP16, bool SOLO>
@@ -252,6 +261,9 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(rsm) + warp * (RR_STAGES * 2 * TILE_B);
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
+  constexpr int ROWS_AT_ONCE = 32 / CH;         // a warp copies this many rows of a tile at a time
+  const int lane_row = lane / CH, lane_ch = lane % CH;
+  const uint32_t lane_off = tile_off<D>(lane_row, lane_ch);
   __shared__ RaggedStart sh_start;
   __shared__ int32_t sh_strides[SOLO ? RR_NW : 1][FEW_REQUESTS];
   const int worker = SOLO ? blockIdx.x * RR_NW + warp : blockIdx.x, part_col = SOLO ? 0 : warp * RR_TT;
@@ -337,13 +349,27 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
         const uint32_t ks = ring + stage * (2 * TILE_B), vs = ks + TILE_B;
         const uint16_t* kp = kb + (valid > 0 ? page * p.k_sp + in_page * p.k_st : 0);
         const uint16_t* vp = vb + (valid > 0 ? page * p.v_sp + in_page * p.v_st : 0);
+        // A tile of keys that all count is copied without a question per row (rows eight apart lie alike in the swizzled tile).
+        // With that and the rescaling left out where no maximum moved, a tile takes 334 instructions of a warp instead of
+        // 597: 64 requests up to 8K 233 -> 224 us in a long run, where the power limit counts
+        if (valid >= RR_TT && (x.first_keys || k0 >= any_lo)) {
+          kp += lane_row * p.k_st + lane_ch * 8;
+          vp += lane_row * p.v_st + lane_ch * 8;
 #pragma unroll
-        for (int i = lane; i < RR_TT * CH; i += 32) {
-          const int row = i / CH, ch = i % CH;
-          // keys that no row of the item sees are not read: whatever they hold, 0 times it must stay 0
-          const bool ok = row < valid && (x.first_keys || k0 + row >= any_lo || k0 + row < p.sinks);
-          cp_async16(ks + tile_off<D>(row, ch), kp + (ok ? row * p.k_st + ch * 8 : 0), ok);
-          cp_async16(vs + tile_off<D>(row, ch), vp + (ok ? row * p.v_st + ch * 8 : 0), ok);
+          for (int r = 0; r < RR_TT; r += ROWS_AT_ONCE) {
+            const uint32_t at = (lane_off ^ (uint32_t(r & 7) << 4)) + r * (D * 2);
+            cp_async16_all(ks + at, kp);
+            cp_async16_all(vs + at, vp);
+            kp += ROWS_AT_ONCE * p.k_st; vp += ROWS_AT_ONCE * p.v_st;
+          }
+        } else {
+#pragma unroll 1
+          for (int row = lane_row; row < RR_TT; row += ROWS_AT_ONCE) {
+            // keys that no row of the item sees are not read: whatever they hold, 0 times it must stay 0
+            const bool ok = row < valid && (x.first_keys || k0 + row >= any_lo || k0 + row < p.sinks);
+            cp_async16(ks + tile_off<D>(row, lane_ch), kp + (ok ? row * p.k_st + lane_ch * 8 : 0), ok);
+            cp_async16(vs + tile_off<D>(row, lane_ch), vp + (ok ? row * p.v_st + lane_ch * 8 : 0), ok);
+          }
         }
       }
       cp_async_commit();
@@ -378,41 +404,39 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
           mma_16816<FP16>(s[0], qa[ks], b[0], b[1]);
           mma_16816<FP16>(s[1], qa[ks], b[2], b[3]);
         }
-        if (!x.first_keys && k0 >= all_lo && k0 + RR_TT - 1 <= all_hi) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][e] *= p.scale_log2;
-        } else {
+        if (x.first_keys || k0 < all_lo || k0 + RR_TT - 1 > all_hi) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int key = k0 + j * 8 + cq + (e & 1);
               const int hi = e < 2 ? hi0 : hi1, lo = e < 2 ? lo0 : lo1;
-              s[j][e] = key <= hi && (key >= lo || key < p.sinks) && key < x.end ? s[j][e] * p.scale_log2 : -INFINITY;
+              s[j][e] = key <= hi && (key >= lo || key < p.sinks) && key < x.end ? s[j][e] : -INFINITY;
             }
         }
         float y0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
         float y1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
         y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 1)); y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 2));
         y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 1)); y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 2));
-        const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
+        const float n0 = fmaxf(m0, y0 * p.scale_log2), n1 = fmaxf(m1, y1 * p.scale_log2);
         const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet: all weights are 0
-        const float a0 = exp2f(m0 - f0), a1 = exp2f(m1 - f1);
-        m0 = n0; m1 = n1;
+        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {      // rare once a few tiles have been seen
+          const float a0 = ex2(m0 - f0), a1 = ex2(m1 - f1);
+          l0 *= a0; l1 *= a1;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) { o[j][0] *= a0; o[j][1] *= a0; o[j][2] *= a1; o[j][3] *= a1; }
+          m0 = n0; m1 = n1;
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          s[j][0] = exp2f(s[j][0] - f0); s[j][1] = exp2f(s[j][1] - f0);
-          s[j][2] = exp2f(s[j][2] - f1); s[j][3] = exp2f(s[j][3] - f1);
+          s[j][0] = ex2(fmaf(s[j][0], p.scale_log2, -f0)); s[j][1] = ex2(fmaf(s[j][1], p.scale_log2, -f0));
+          s[j][2] = ex2(fmaf(s[j][2], p.scale_log2, -f1)); s[j][3] = ex2(fmaf(s[j][3], p.scale_log2, -f1));
         }
-        l0 = l0 * a0 + (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
-        l1 = l1 * a1 + (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
+        l0 += (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
+        l1 += (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
         // the weights are rounded to the inputs' type for the product, their sum is taken before that
         const uint32_t pa[4] = {pack_half2<FP16>(s[0][0], s[0][1]), pack_half2<FP16>(s[0][2], s[0][3]),
                                 pack_half2<FP16>(s[1][0], s[1][1]), pack_half2<FP16>(s[1][2], s[1][3])};
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j) { o[j][0] *= a0; o[j][1] *= a0; o[j][2] *= a1; o[j][3] *= a1; }
 #pragma unroll
         for (int jj = 0; jj < D / 16; ++jj) {
           uint32_t b[4];
