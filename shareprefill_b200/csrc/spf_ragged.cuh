@@ -263,21 +263,18 @@ __device__ __forceinline__ RaggedStart ragged_start_few(const RaggedParams& p, i
   q.stride = 1;
   if (lane < p.n_requests) q = ragged_req_plain(p, lane);
   const int tiles = ragged_tiles(p, q.n);
-  long long sum = 0;
-  if (__any_sync(0xffffffffu, tiles > 1)) {
-    for (int r = 0; r < p.n_requests; ++r) {
-      RaggedReq o;
-      o.row0 = 0; o.stride = 1;
-      o.n = __shfl_sync(0xffffffffu, q.n, r); o.seq = __shfl_sync(0xffffffffu, q.seq, r);
-      const int n_tiles = ragged_tiles(p, o.n);
-      int part = 0;
+  long long sum = tiles == 1 ? ragged_span(p, q, 0).total : 0;
+  for (unsigned many = __ballot_sync(0xffffffffu, tiles > 1); many; many &= many - 1) {     // the warp adds up a request's tiles
+    const int r = __ffs(many) - 1;
+    RaggedReq o;
+    o.row0 = 0; o.stride = 1;
+    o.n = __shfl_sync(0xffffffffu, q.n, r); o.seq = __shfl_sync(0xffffffffu, q.seq, r);
+    const int n_tiles = ragged_tiles(p, o.n);
+    int part = 0;
 #pragma unroll 4
-      for (int t = lane; t < n_tiles; t += 32) part += ragged_span(p, o, t).total;
-      const long long all = warp_sum_ll(part);
-      if (lane == r) sum = all;
-    }
-  } else if (tiles == 1) {
-    sum = ragged_span(p, q, 0).total;
+    for (int t = lane; t < n_tiles; t += 32) part += ragged_span(p, o, t).total;
+    const long long all = warp_sum_ll(part);
+    if (lane == r) sum = all;
   }
   const long long upto = warp_scan_ll(sum * heads, lane), all = __shfl_sync(0xffffffffu, upto, 31);
   const long long per = max(div_ll(all + p.n_ctas - 1, p.n_ctas), 1ll), u = per * c;
