@@ -478,6 +478,36 @@ def test_results_do_not_depend_on_the_run_or_the_stream():
         assert torch.equal(first, again)
 
 
+@pytest.mark.parametrize("requests,new", [(2, 1), (40, 1), (300, 1), (3, 90), (45, 30)])
+def test_lengths_and_queries_written_by_the_kernel_just_before(requests, new):
+    # the attention kernels are launched under the end of the kernel before: what that one writes must be seen
+    steps = []
+    pool = _batch([(400, new)] * requests, 16, 8, 2, 128, BF16, "token", 77)[0]
+    k, v = pool.cuda()
+    table = pool.table.cuda()
+    for i in range(3):
+        spec = [((37 * r + 131 * i) % 400, 1 + (r + i) % new) for r in range(requests)]
+        cu = [0]
+        for _, n in spec:
+            cu.append(cu[-1] + n)
+        q = torch.randn(requests * new, 8, 128, device="cuda").to(BF16)
+        data = (q, _ints(cu), _ints([c + n for c, n in spec]))
+        torch.cuda.synchronize()
+        want = [native.paged_attention(data[0], k, v, table, data[1], data[2], new, 0.1, window)[:cu[-1]] for window in (0, 50)]
+        torch.cuda.synchronize()
+        steps.append((data, want))
+    live = [x.clone() for x in steps[0][0]]
+    got = []
+    for i in range(30):
+        for which in ((0, 1, 2), (2, 0, 1), (1, 2, 0))[i // 3 % 3]:      # each of them once the last to be written
+            live[which].copy_(steps[i % 3][0][which])
+        got.append(native.paged_attention(live[0], k, v, table, live[1], live[2], new, 0.1, 50 * (i % 2)))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        want = steps[i % 3][1][i % 2]
+        assert torch.equal(x[:len(want)], want), i
+
+
 def test_a_device_that_is_not_the_current_one():
     if torch.cuda.device_count() < 2:
         pytest.skip("one GPU")
