@@ -1,4 +1,5 @@
 // C ABI of libspf_b200.so: argument validation and dispatch.  See include/spf_b200.h.
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdlib>
@@ -402,11 +403,29 @@ static int check_ragged(int n_q_heads, int n_kv_heads, int head_dim, int dtype, 
   return SPF_OK;
 }
 
-// Requests of up to 16 rows per KV head (single tokens) go to the bandwidth-bound kernel, others to the tcgen05 one, each
-// in its own pass over the batch where it may hold both.  (All through the tcgen05 kernel, whose 128-row tiles such
-// requests leave nearly empty, a batch of 14 tokens and two chunks of 509 takes 131 us instead of 117.)  Tensors that TMA cannot
-// describe (strides of 0 in expanded views) go to the first kernel whole.
+// Batches whose requests all bring up to 16 rows per KV head (single tokens) go to the bandwidth-bound kernel, others to the
+// tcgen05 one.  Tensors that TMA cannot describe (strides of 0 in expanded views) go to the first kernel whole.
 static bool few_rows(int group, int max_new) { return int64_t(group) * max_new <= RAGGED_FEW_ROWS; }
+
+// Chunks and single tokens in one batch: a pass of each kernel over its own requests, or all of them through the tcgen05
+// kernel, whose 128-row tiles single tokens leave nearly empty.  The second pass costs 10 - 30 us, a token in the wrong kernel
+// 0.04 us per 1000 keys of a KV head.  The host knows neither lengths nor which requests are which: of n_rows what passes one token
+// a request is taken for as few chunks as can hold it, and a token for half of the table or its window, and 512 keys for its
+// tile.  us in two passes
+// / one, two chunks of 509 behind up to 16K keys and 4, 16, 20, 24 and 28 tokens with a window of 4096, 32q/8kv, D = 128:
+// 120.3 / 89.5, 152.4 / 135.5, 162.1 / 154.7, 173.3 / 173.0, 183.4 / 185.7; D = 64: 92.4 / 75.6, 119.2 / 112.9, 125.8 / 122.8, 131.1
+// / 136.2, 136.5 / 148.5.  Without a window, D = 128: 4 tokens 238 / 220, 12 300 / 296, 20 343 / 369; 64 of them 594 / 745; 64 with
+// 2K keys 155 / 148 (D = 64 113 / 133); 254 with 500 keys 169 / 211.
+constexpr int64_t MIXED_KEYS_128 = 920 * 1024, MIXED_KEYS_64 = 700 * 1024, TILE_KEYS = 512;
+
+static bool two_passes(const RaggedParams& p, int max_new, int head_dim) {
+  if (p.n_requests < 2 || p.group > RAGGED_FEW_ROWS || p.n_rows >= int64_t(p.n_requests) * max_new) return false;
+  // (max_new >= 2: one token of at most 16 heads is a matter of the first kernel)
+  const int64_t over = std::max(p.n_rows - p.n_requests, 0), chunks = (over + max_new - 2) / (max_new - 1);
+  int64_t keys = (int64_t(p.table_width) << p.page_shift) / 2;
+  if (p.window > 0) keys = std::min(keys, int64_t(p.window) + p.sinks);
+  return (p.n_requests - chunks) * p.n_kv_heads * (keys + TILE_KEYS) > (head_dim == 128 ? MIXED_KEYS_128 : MIXED_KEYS_64);
+}
 
 // Single tokens with a worker per warp instead of one per CTA: from this many items on, at D = 128.  us with a worker per CTA /
 // per warp, 32q/8kv: 64 requests up to 32 keys 18.6 / 16.9, 500 keys 39.6 / 32.1, 3000 91.1 / 90.3, 8192 215.9 / 215.9; 96
@@ -428,9 +447,7 @@ static int run_ragged(RaggedParams& p, int max_new, int head_dim, int64_t scratc
   if (scratch_bytes < spf_paged_scratch_bytes(max_new, p.n_q_heads, p.n_kv_heads, head_dim)) return SPF_ERR_RANGE;
   if (few_rows(p.group, max_new) || !ragged_tc5_describable(p)) return run_pass(p, false, 0, max_new, head_dim, st);
   if (timeouts_tripped()) return SPF_ERR_TIMEOUT;
-  // some request brings less than max_new tokens, perhaps few enough
-  const bool mixed = p.n_requests > 1 && p.group <= RAGGED_FEW_ROWS && p.n_rows < int64_t(p.n_requests) * max_new;
-  if (!mixed) return run_pass(p, true, 0, max_new, head_dim, st);
+  if (!two_passes(p, max_new, head_dim)) return run_pass(p, true, 0, max_new, head_dim, st);
   const int rc = run_pass(p, false, 1, RAGGED_FEW_ROWS / p.group, head_dim, st);
   return rc == SPF_OK ? run_pass(p, true, 2, max_new, head_dim, st) : rc;
 }

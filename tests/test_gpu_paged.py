@@ -161,6 +161,25 @@ def test_paged_attention_matches_the_statement(case):
     _check_batch(got, spec, pool, cu, q, scale, window, sinks, dtype)
 
 
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("spec,heads,kv_heads,dim,dtype,window,sinks", [
+    ([(700, 90), (40, 200), (0, 3), (5, 0)] + [(i * 29 % 600, 1) for i in range(20)], 8, 2, 128, BF16, 0, 0),
+    ([(300, 7), (900, 6), (0, 1), (33, 5)] + [(i * 17, 1) for i in range(20)], 28, 4, 64, FP16, 0, 0),
+    ([(2300, 40), (2500, 1)] + [(i * 7, 1) for i in range(60)], 16, 8, 64, BF16, 2100, 4),
+])
+def test_chunks_and_single_tokens_in_one_pass_or_two(spec, heads, kv_heads, dim, dtype, window, sinks, wide):
+    # a table that could hold long sequences makes a batch of tokens and chunks run through both kernels
+    pool, cu, q = _batch(spec, 16, heads, kv_heads, dim, dtype, "token", 31)
+    k, v = pool.cuda()
+    table = torch.nn.functional.pad(pool.table, (0, 6000 if wide else 0), value=-1).cuda()
+    out = torch.full((cu[-1] + 3, heads, dim), 7.0, dtype=dtype, device="cuda")
+    padded = torch.cat([q, q[:3]]).cuda()
+    lengths = _ints([c + n for c, n in spec])
+    native.paged_attention(padded, k, v, table, _ints(cu), lengths, max(n for _, n in spec), dim ** -0.5, window, sinks, out)
+    _check_batch(out, spec, pool, cu, q, dim ** -0.5, window, sinks, dtype)
+    assert (out[cu[-1]:] == 7.0).all()
+
+
 @pytest.mark.parametrize("new", [1, 3, 90])
 def test_rows_without_keys_absent_pages_and_rows_behind_the_batch(new):
     page, heads, kv_heads, dim, dtype = 16, 8, 2, 128, BF16
