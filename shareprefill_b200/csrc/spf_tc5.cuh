@@ -173,7 +173,7 @@ __device__ __forceinline__ uint32_t bf16x2_from(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));   // first source -> upper half
   return d;
 }
-// p = 2^(s*scale - m) for 32 scores: packed to bf16 (or fp16) pairs, unrounded values summed into `sum`.
+// p = 2^(s*scale - m) for 32 scores: packed to bf16 pairs, unrounded values summed into `sum`.
 // POLY of every 8 element pairs are taken off the exponential unit (16 exponentials per clock and
 // SM): their 2^y comes from a range reduction and a degree-3 polynomial on the FMA pipe
 // (relative error 7.5e-5, far below the bf16 rounding of P).
@@ -181,12 +181,7 @@ __device__ __forceinline__ uint32_t bf16x2_from(float lo, float hi) {
 //                                   exceeds the row's true maximum, so 2^-57 is noise against l >= 1
 //   n = round(128u - 57) by the 1.5 * 2^23 trick;  f = 128u - 57 - n in [-0.5, 0.5]
 //   2^y = poly(f) * 2^n             n is added to the exponent field of poly(f)
-__device__ __forceinline__ uint32_t f16x2_from(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-template <int POLY, bool FP16 = false>
+template <int POLY>
 __device__ __forceinline__ void exp_pack_poly(const uint32_t (&r)[32], float scale, float m, uint32_t (&pk)[16], float& sum) {
   const unsigned long long sc2 = f2_pack(scale, scale), nm2 = f2_pack(-m, -m);
   const float sc128 = scale * 0.0078125f, b128 = (57.f - m) * 0.0078125f;
@@ -220,7 +215,7 @@ __device__ __forceinline__ void exp_pack_poly(const uint32_t (&r)[32], float sca
       p0 = fast_exp2(y0); p1 = fast_exp2(y1);
     }
     acc[(j >> 1) & 3] = f2_add(acc[(j >> 1) & 3], f2_pack(p0, p1));
-    pk[j >> 1] = FP16 ? f16x2_from(p0, p1) : bf16x2_from(p0, p1);
+    pk[j >> 1] = bf16x2_from(p0, p1);
   }
   float a0, a1;
   f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a0, a1);

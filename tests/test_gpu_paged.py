@@ -310,6 +310,24 @@ def test_values_that_no_query_sees_may_be_anything(new):
         R.check(got, out, mass, BF16, keys, 5.0)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,keys,window,sinks", [(64, 64, 0, 0), (300, 300, 0, 0), (40, 700, 0, 0), (300, 700, 90, 0), (300, 700, 70, 20),
+                                                   (3, 600, 50, 4), (200, 200, 1, 0)])
+def test_large_values_of_keys_that_a_token_does_not_see_have_no_weight(new, keys, window, sinks, dim):
+    # every key is hidden from some tokens of a tile and seen by others, and every third has a value 10^30 times
+    # as large: a weight of 2^-57 where there should be none would show
+    g = torch.Generator().manual_seed(new + keys + dim)
+    q = torch.randn(new, 8, dim, generator=g).to(BF16)
+    k, v = (torch.randn(keys, 2, dim, generator=g).to(BF16) for _ in range(2))
+    hidden_first = torch.arange(keys) % 3 == 1
+    hidden_first &= torch.arange(keys) > keys - new          # the first token sees none of them in its future
+    v[hidden_first] *= 1e30
+    out, mass = R.attention(q, k, v, keys - new, dim ** -0.5, window, sinks)
+    assert float(mass[0].max()) < 10 and (window == 1 or float(mass.max()) > 1e20)
+    got = native.window_attention(q.cuda(), k.cuda(), v.cuda(), dim ** -0.5, window, sinks)
+    R.check(got, out, mass, BF16, keys, 1e31)
+
+
 @pytest.mark.parametrize("new", [1, 200])
 @pytest.mark.parametrize("gain", [30.0, 1e4])
 def test_peaked_scores_and_expanded_caches(new, gain):
