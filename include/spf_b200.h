@@ -314,8 +314,9 @@ int spf_paged_write(const void* k, int64_t k_stride_n, int64_t k_stride_h,
  *   q: [n_rows][H][D], out: [n_rows][H][D] contiguous; caches as for spf_paged_write; dtype of all: SPF_BF16
  *   or SPF_FP16.  max_new: an upper bound of new_r, read on the host; it selects the kernel, and rows of a
  *   request past it need not be computed.  cu_new and seq_len are clipped to the batch on the device.
- *   Keys that a request does not see are not read, or not used, whatever they hold (NaN included), except that
- *   a NaN or infinity in a VALUE row that some token of a chunk sees can reach the chunk's other tokens.
+ *   Keys that a token does not see have the weight 0, whatever they hold (NaN included), except that
+ *   a NaN or infinity in a VALUE row that some token of a chunk sees can reach the chunk's other tokens.  A score of NaN or
+ *   +infinity of a key that a row sees makes the row NaN; a score of -infinity is a weight of 0.
  *   out and scratch start on 32-byte boundaries and overlap no input.  There is no backward pass.
  *   scratch: spf_paged_scratch_bytes() bytes, overwritten; calls that may run at the same
  *   time need their own.

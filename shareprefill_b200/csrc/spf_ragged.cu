@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
     }
     const int64_t at = place(row);
     if (at < 0) return;                        // what was read of such a row was never written, and is not used
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at + x4 + j * 4 * LANES) =
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(MRG_NT) ragged_merge_kernel(const RaggedParams
       total += sum_of[w] * a;
       x += acc_of[w][2 * threadIdx.x] * a; y += acc_of[w][2 * threadIdx.x + 1] * a;
     }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
     reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at)[threadIdx.x] = pack_half2<FP16>(x * inv, y * inv);
   }
 }
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
       for (int half = 0; half < 2; ++half) {
         if (!(half ? in1 : in0)) continue;
         const int r = half ? r1 : r0;
-        const float l = half ? l1 : l0, inv = l > 0.f ? 1.f / l : 0.f;
+        const float l = half ? l1 : l0, inv = l == 0.f ? 0.f : 1.f / l;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, half ? t_r1 : t_r0, half ? h_r1 : h_r0, D) + cq;
         if (!whole && (lane & 3) == 0) { part[r] = half ? m1 : m0; part[RR_ROWS + r] = l; }
 #pragma unroll
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
         x += t.x * sc; y += t.y * sc;
       }
       if (whole) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + ragged_out(p, q, item, t, h, D) + d) =
             pack_half2<FP16>(x * inv, y * inv);
       } else {

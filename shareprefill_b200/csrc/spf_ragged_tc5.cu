@@ -136,6 +136,12 @@ __device__ __forceinline__ void store_32(void* dst, const uint32_t (&v)[8]) {
                ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
+// NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // P = 2^(s * scale - m) for 32 scores, packed in pairs; the unrounded weights are added to `sum`.  POLY of every 8 pairs
 // are taken off the exponential unit (16 exponentials per clock and SM): a range reduction and a cubic on the FMA pipe.
 //   u = sat((y + 127) / 255)        y = s * scale - m
@@ -146,8 +152,11 @@ __device__ __forceinline__ void store_32(void* dst, const uint32_t (&v)[8]) {
 // 0, and u = 1 those of infinity.  So a masked score (-infinity) has the weight 0, whatever the value of its key - with 2^-57,
 // where a range of [-57, 71] ended, a value of 1e20 that a token must not see was 690 in its output - and a score far above
 // m shows in the sum.  Weights between 2^-127 and 2^-126 are rounded at will.
+// Saturation makes 0 of NaN too: the sum becomes NaN where one of the polynomial's scores is (1% at D = 128; a mixed batch
+// at D = 64 107.3 -> 110.7 us; sums of the scores and the smallest of them took as long).
 template <int POLY, bool FP16>
 __device__ __forceinline__ void rt_weights(const uint32_t (&r)[32], float scale, float m, uint32_t (&pk)[16], float& sum) {
+  float top = -INFINITY;
   const unsigned long long sc2 = f2_pack(scale, scale), nm2 = f2_pack(-m, -m);
   const float sc255 = scale * (1.f / 255.f), b255 = (127.f - m) * (1.f / 255.f);
   constexpr float MAGIC = 12582912.f - 127.f;      // 1.5 * 2^23 - 127
@@ -159,6 +168,7 @@ __device__ __forceinline__ void rt_weights(const uint32_t (&r)[32], float scale,
   for (int j = 0; j < 32; j += 2) {
     float p0, p1;
     if (((j >> 1) & 7) < POLY) {
+      top = max3_nan(top, __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
       const float u0 = __saturatef(fmaf(__uint_as_float(r[j]), sc255, b255));
       const float u1 = __saturatef(fmaf(__uint_as_float(r[j + 1]), sc255, b255));
       const unsigned long long u = f2_pack(u0, u1);
@@ -184,7 +194,7 @@ __device__ __forceinline__ void rt_weights(const uint32_t (&r)[32], float scale,
   }
   float a0, a1;
   f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a0, a1);
-  sum += a0 + a1;
+  sum = top == top ? sum + (a0 + a1) : top;
 }
 
 // the n lowest bits (n below 0: none, above 32: all)
@@ -642,6 +652,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (fresh) {
           const float mb = row_max_log2();
           if (m_used == -INFINITY) m_used = mb;
+          if (mb == INFINITY) l_sum = NAN;       // infinity less itself
           fresh = __any_sync(0xffffffffu, m_used == -INFINITY);
         }
         // S must stay in TMEM until the row's sum has been looked at, for the case that the reference has to move.  At D = 64
@@ -652,23 +663,22 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         bool moved = u == 0;
         while (true) {
           const float ref = m_used == -INFINITY ? 0.f : m_used;
-          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+          blk = 0.f;
           uint32_t s0[32], s1[32], s2[32], s3[32];
           tmem_ld32_raw(tS + 0, s0);
           tmem_ld32_raw(tS + 32, s1);
           tc_wait_ld();
           tmem_ld32_raw(tS + 64, s2);
-          rt_weights<C::POLY, FP16>(s0, p.scale_log2, ref, pk0, l0);
+          rt_weights<C::POLY, FP16>(s0, p.scale_log2, ref, pk0, blk);
           if (C::P_BESIDE) tmem_st16(p_tmem(), pk0);
           tmem_ld32_raw(tS + 96, s3);
-          rt_weights<C::POLY, FP16>(s1, p.scale_log2, ref, pk1, l1);
+          rt_weights<C::POLY, FP16>(s1, p.scale_log2, ref, pk1, blk);
           if (C::P_BESIDE) tmem_st16(p_tmem() + 16, pk1);
           tc_wait_ld();
-          rt_weights<C::POLY, FP16>(s2, p.scale_log2, ref, pk2, l2);
+          rt_weights<C::POLY, FP16>(s2, p.scale_log2, ref, pk2, blk);
           if (C::P_BESIDE) tmem_st16(p_tmem() + 32, pk2);
-          rt_weights<C::POLY, FP16>(s3, p.scale_log2, ref, pk3, l3);
+          rt_weights<C::POLY, FP16>(s3, p.scale_log2, ref, pk3, blk);
           if (C::P_BESIDE) tmem_st16(p_tmem() + 48, pk3);
-          blk = (l0 + l1) + (l2 + l3);
           if (moved || !__any_sync(0xffffffffu, !(blk <= SUM_LIMIT))) break;
           moved = true;
           const float mb = row_max_log2();
@@ -677,6 +687,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             alpha = exp2f(m_used - mb);
             m_used = mb;
             l_sum *= alpha;
+            if (mb == INFINITY) l_sum = NAN;
           }
           // S of this unit is complete, hence so is every earlier P V of the stream: O is stable
 #pragma unroll 1
@@ -704,7 +715,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       tc_fence_after();
       const Place x = place(part);
       if (part.whole) {
-        const float inv = m_used != -INFINITY && l_sum > 0.f ? 1.f / l_sum : 0.f;
+        const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;     // (no key: 0; a NaN stays one)
         uint16_t* dst = static_cast<uint16_t*>(p.out) + (x.in ? part.out + (int64_t(x.tok) * p.n_q_heads + x.head) * D : 0);
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {

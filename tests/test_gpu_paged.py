@@ -328,6 +328,35 @@ def test_large_values_of_keys_that_a_token_does_not_see_have_no_weight(new, keys
     R.check(got, out, mass, BF16, keys, 1e31)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("new,keys,heads,dim", [(1, 300, 4, 128), (1, 9000, 4, 64), (64, 200, 4, 128), (64, 200, 4, 64), (200, 9000, 2, 128), (200, 9000, 2, 64)])
+def test_scores_that_are_not_finite_are_seen_wherever_their_key_stands(new, keys, heads, dim, dtype):
+    # a key of NaN makes every row NaN that sees it, an infinite score too; a score of -infinity is a weight of 0
+    g = torch.Generator().manual_seed(new + keys + dim)
+    q = torch.randn(new, heads, dim, generator=g).to(dtype)
+    k, v = (torch.randn(keys, 1, dim, generator=g).to(dtype) for _ in range(2))
+    q[:, 0::2, 0], q[:, 1::2, 0] = 1.0, -1.0                # heads to which a key's infinity is +infinity and -infinity
+    before, scale = keys - new, dim ** -0.5
+    out, mass = R.attention(q, k, v, before, scale)
+    dq, dk, dv = q.cuda(), k.cuda(), v.cuda()
+    for at in [*range(before - 20, before + new, 3), *range(68), keys - 1]:
+        sees = before + torch.arange(new) >= at
+        for bad in (float("nan"), float("inf")):
+            dk.copy_(k)
+            dk[at, 0, 0] = bad
+            got = native.window_attention(dq, dk, dv, scale, 0).cpu()
+            spoiled = sees[:, None] & (torch.tensor([True, False] * (heads // 2)) | (bad != bad))
+            assert bool((got.isnan().all(-1) == spoiled).all()), f"{bad} at {at}"
+            fine = got.double().nan_to_num(0.0)
+            fine[spoiled] = out[spoiled]
+            if bad == bad and keys < 1000:
+                present = torch.ones(keys, dtype=torch.bool)
+                present[at] = False
+                want, weight = R.attention(q[:, 1::2], k, v, before, scale, present=present)
+                R.check(fine[:, 1::2], want, weight, dtype, keys, 5.0, f"-inf at {at}")
+            R.check(fine[~sees], out[~sees], mass[~sees], dtype, keys, 5.0, f"rows before {at}") if not bool(sees.all()) else None
+
+
 @pytest.mark.parametrize("new", [1, 200])
 @pytest.mark.parametrize("gain", [30.0, 1e4])
 def test_peaked_scores_and_expanded_caches(new, gain):
