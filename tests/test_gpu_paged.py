@@ -357,6 +357,30 @@ def test_scores_that_are_not_finite_are_seen_wherever_their_key_stands(new, keys
             R.check(fine[~sees], out[~sees], mass[~sees], dtype, keys, 5.0, f"rows before {at}") if not bool(sees.all()) else None
 
 
+@pytest.mark.parametrize("new,dim", [(1, 64), (1, 128), (5, 64), (5, 128)])
+def test_fp16_weights_far_below_the_largest_still_add_up(new, dim):
+    # one key 17 nats (2^24.5) above 30000 others that hold a thousandth of the mass together, and only they have values.
+    # 64 requests over the same pages, so that a request's keys stay with one CTA.
+    page, heads, kv_heads, keys, requests, scale = 16, 32, 8, 30000, 64, 0.125
+    g = torch.Generator().manual_seed(new + dim)
+    q = (0.3 * torch.randn(new, heads, dim, generator=g)).to(FP16)
+    k = torch.randn(keys, kv_heads, dim, generator=g).to(FP16)
+    v = (1 + 0.1 * torch.randn(keys, kv_heads, dim, generator=g)).to(FP16)
+    q[:, :, 0], k[:, :, 0] = 8.0, 0.0
+    k[0], v[0] = 0.0, 0.0
+    k[0, :, 0] = 17.0
+    out, mass = R.attention(q, k, v, keys - new, scale)
+    assert 5e-4 < float(out.min()) and float(out.max()) < 5e-3
+    table = torch.arange(keys // page).to(torch.int32).expand(requests, -1).contiguous()
+    got = native.paged_attention(q.repeat(requests, 1, 1).cuda(), k.view(-1, page, kv_heads, dim).cuda(), v.view(-1, page, kv_heads, dim).cuda(),
+                                 table.cuda(), _ints([i * new for i in range(requests + 1)]), _ints([keys] * requests), new, scale)
+    # as R.tolerance, but the largest weight of a unit is 2^8 or more, so that multiples of 2^-24 are 2^-33 of it per key
+    u = 2 ** -11
+    tol = u * (mass + out.abs()) * (1 + 2 ** -6) + 2 ** -11 * mass + keys * 2 ** -33 * float(v.abs().max())
+    off = (got.view(requests, new, heads, dim).double().cpu() - out).abs() / tol
+    assert float(off.max()) <= 1.0, f"{float(off.max()):.3g} times the tolerance"
+
+
 @pytest.mark.parametrize("new", [1, 200])
 @pytest.mark.parametrize("gain", [30.0, 1e4])
 def test_peaked_scores_and_expanded_caches(new, gain):
