@@ -127,8 +127,11 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_NT) pag
 
 int launch_paged_plan(const PlanParams& p, cudaStream_t st) {
   const int smem = (3 * p.n_requests + 1) * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // 48 KiB are granted without asking, to this and the kernel's static shared memory together.  (Always the same limit: with the
+  // call's own size, a call from another thread could lower it between this and the launch.)
+  if (smem > 32 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * SPF_MAX_REQUESTS + 1) * 4);
     if (e != cudaSuccess) { note_cuda_error(e); return SPF_ERR_LAUNCH; }
   }
   paged_plan_kernel<<<PLAN_CTAS, PLAN_NT, smem, st>>>(p);

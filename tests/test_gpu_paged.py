@@ -1,5 +1,8 @@
 """Paged cache and windowed attention on the GPU against the 64-bit statements of tests/paged_reference.py."""
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -10,6 +13,7 @@ from shareprefill_b200 import native
 pytestmark = pytest.mark.gpu
 
 BF16, FP16 = torch.bfloat16, torch.float16
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def _ints(x):
@@ -67,6 +71,22 @@ def test_plan_in_place_state_odd_lengths_and_padded_table_rows():
     assert p.ring_state.data_ptr() == state.data_ptr() and state.tolist() == want["ring_state"] == [1, 2]
     assert table.tolist() == want["table"] and p.slot_map.tolist() == want["slot_map"]
     assert p.seq_len.tolist() == [17, 0, 17] and p.refused.tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("requests", [4073, 4074, 4075, 4095])
+def test_plan_of_nearly_the_most_requests_in_a_fresh_process(requests):
+    # (a call with more requests before it in the process would raise the kernel's limit of shared memory for this one)
+    program = f"""
+import torch
+from shareprefill_b200 import native
+i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+r = {requests}
+table = torch.full((r, 1), -1, dtype=torch.int32, device="cuda")
+p = native.paged_plan(i([0] * r), i([1] * r), table, torch.arange(r, dtype=torch.int32, device="cuda"), i([0, r]), r, 16)
+assert p.slot_map.tolist() == [16 * x for x in range(r)] and p.ring_state.tolist() == [0, 0] and not p.refused.any()
+"""
+    done = subprocess.run([sys.executable, "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_plan_with_extreme_lengths_refuses_and_stays_inside():
