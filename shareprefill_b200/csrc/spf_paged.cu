@@ -39,7 +39,8 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_NT) pag
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = int(cluster.block_rank());
   const int cap = p.ring_capacity, ps = 1 << p.page_shift;
-  const int head = ((p.ring_state[0] % cap) + cap) % cap, count = min(max(p.ring_state[1], 0), cap);
+  const int turn = p.ring_state[0] % cap, head = turn < 0 ? turn + cap : turn;
+  const int count = min(max(p.ring_state[1], 0), cap);
   if (tid == 0) { cu[0] = 0; taken_max = 0; }
   long long carry_rows = 0, carry_pages = 0;
   for (int r0 = 0; r0 < p.n_requests; r0 += PLAN_NT) {

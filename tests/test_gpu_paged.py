@@ -89,6 +89,18 @@ assert p.slot_map.tolist() == [16 * x for x in range(r)] and p.ring_state.tolist
     assert done.returncode == 0, done.stderr[-2000:]
 
 
+def test_plan_from_the_end_of_a_ring_of_more_than_2_to_the_30_ids():
+    # head + capacity is more than an int holds
+    cap = (1 << 30) + 16
+    ring = torch.empty(cap, dtype=torch.int32, device="cuda")
+    ring[-2:], ring[:3] = _ints([7, 5]), _ints([9, 4, 6])
+    for head in (cap - 2, -2):
+        table = torch.full((2, 3), -1, dtype=torch.int32, device="cuda")
+        p = native.paged_plan(_ints([0, 0]), _ints([33, 17]), table, ring, _ints([head, 5]), 50, 16)
+        assert table.tolist() == [[7, 5, 9], [4, 6, -1]] and p.ring_state.tolist() == [3, 0] and p.refused.tolist() == [0, 0]
+        assert p.slot_map.tolist() == [16 * page + i for page, n in ((7, 16), (5, 16), (9, 1), (4, 16), (6, 1)) for i in range(n)]
+
+
 def test_plan_with_extreme_lengths_refuses_and_stays_inside():
     page, top = 16, 2 ** 31 - 1
     table = torch.full((4, 3), -1, dtype=torch.int32, device="cuda")
