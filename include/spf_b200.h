@@ -282,7 +282,7 @@ int spf_decode_attention(const void* q, int64_t q_stride_h,
  * and per packed row of the n_rows: slot_map (page * page_size + offset, -1 for rows of refused requests,
  * of negative page ids and behind the last request) and positions (place in the sequence; 0 behind the
  * last request).  Any output may be the buffer of the input it follows (seq_len = cached_len,
- * ring_state_out = ring_state).  n_requests <= SPF_MAX_REQUESTS.
+ * ring_state_out = ring_state).  n_requests <= SPF_MAX_REQUESTS, n_rows <= SPF_MAX_KEYS (also of the attention below).
  */
 int spf_paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_requests, int page_size,
                    int32_t* block_table, int64_t table_stride, int table_width,

@@ -358,7 +358,7 @@ int spf_paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_requ
   if (page_shift_of(page_size) < 0) return SPF_ERR_SHAPE;
   if (n_requests <= 0 || n_rows < 0 || table_width <= 0 || table_stride < table_width || ring_capacity <= 0)
     return SPF_ERR_RANGE;
-  if (n_requests > SPF_MAX_REQUESTS) return SPF_ERR_TOO_LARGE;
+  if (n_requests > SPF_MAX_REQUESTS || n_rows > SPF_MAX_KEYS) return SPF_ERR_TOO_LARGE;
   PlanParams p;
   p.cached_len = cached_len; p.new_len = new_len; p.n_requests = n_requests; p.page_shift = page_shift_of(page_size);
   p.table = block_table; p.table_stride = table_stride; p.table_width = table_width;

@@ -134,3 +134,9 @@ def test_sliding_window_layers_refuse_what_they_cannot_do():
     module.training = True
     with pytest.raises(native.SpfError, match="dropout"):
         forward(module, x, x[:, :2], x[:, :2], None, sliding_window=4)
+
+
+def test_plans_of_more_rows_than_a_batch_may_have_are_refused():
+    # (the kernel's row counter would pass 32 bits just below 2^31 rows)
+    for rows in ((1 << 28) + 1, (1 << 31) - 4097, (1 << 31) - 1):
+        assert native.load().spf_paged_plan(PTR, PTR, 2, 16, PTR, 4, 4, PTR, 8, PTR, PTR, PTR, PTR, PTR, PTR, PTR, rows, None) == -6
