@@ -318,6 +318,7 @@ int spf_paged_write(const void* k, int64_t k_stride_n, int64_t k_stride_h,
  *   a NaN or infinity in a VALUE row that some token of a chunk sees can reach the chunk's other tokens.  A score of NaN or
  *   +infinity of a key that a row sees makes the row NaN; a score of -infinity is a weight of 0.
  *   out and scratch start on 32-byte boundaries and overlap no input.  There is no backward pass.
+ *   More than 2^31 runs of 64 or 128 keys for a CTA (minutes to hours of work) are SPF_ERR_TOO_LARGE.
  *   scratch: spf_paged_scratch_bytes() bytes, overwritten; calls that may run at the same
  *   time need their own.
  */

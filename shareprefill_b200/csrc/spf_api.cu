@@ -433,10 +433,22 @@ static bool two_passes(const RaggedParams& p, int max_new, int head_dim) {
 // 114.0.  At D = 64 (96 requests): 500 keys 34.5 / 33.6, 8192 keys 184.6 / 192.2.
 constexpr int SOLO_ITEMS = 512;
 
+// A CTA counts the units that it runs through in 32 bits, and so does the search for its start over 128 tiles at a time.
+// (The bound takes every request for as long as its table; what it refuses would run for minutes to hours.)
+static int64_t line_keys(const RaggedParams& p) { return p.table ? int64_t(p.table_width) << p.page_shift : p.seq_one; }
+static bool line_fits(const RaggedParams& p) {
+  int64_t keys = line_keys(p);
+  if (p.window > 0) keys = std::min(keys, int64_t(p.window) + p.sinks + p.tile_tokens);
+  const int64_t units = (keys >> p.unit_shift) + 3, items = (int64_t(p.n_rows / p.tile_tokens) + p.n_requests) * p.n_kv_heads * p.head_chunks;
+  return units < (int64_t(1) << 24) && double(units) * double(items) < 2147483647.0 * p.n_ctas;
+}
+
 static int run_pass(RaggedParams p, bool tc5, int only, int max_new, int head_dim, cudaStream_t st) {
   p.only = only; p.head_dim = head_dim;
-  const bool solo = head_dim == 128 && few_rows(p.group, max_new) && p.n_requests * p.n_kv_heads >= SOLO_ITEMS;
+  const bool solo = head_dim == 128 && few_rows(p.group, max_new) && p.n_requests * p.n_kv_heads >= SOLO_ITEMS &&
+                    line_keys(p) <= SPF_MAX_KEYS / 2;       // (units of 16 keys)
   if (tc5) ragged_tc5_config(p); else ragged_rows_config(p, solo);
+  if (!line_fits(p)) return SPF_ERR_TOO_LARGE;
   int rc = ragged_schedule(p, max_new, st);
   if (rc == SPF_OK) rc = tc5 ? ragged_tc5_attention(p, head_dim, st) : ragged_rows_attention(p, head_dim, st);
   if (rc == SPF_OK) rc = ragged_merge(p, max_new, head_dim, st);

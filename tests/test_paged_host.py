@@ -140,3 +140,12 @@ def test_plans_of_more_rows_than_a_batch_may_have_are_refused():
     # (the kernel's row counter would pass 32 bits just below 2^31 rows)
     for rows in ((1 << 28) + 1, (1 << 31) - 4097, (1 << 31) - 1):
         assert native.load().spf_paged_plan(PTR, PTR, 2, 16, PTR, 4, 4, PTR, 8, PTR, PTR, PTR, PTR, PTR, PTR, PTR, rows, None) == -6
+
+
+def test_more_work_than_a_call_can_count_is_refused():
+    # a causal prompt of 2^28 tokens is 2^40 units of keys, 2^33 a CTA; with a window it is a line that fits
+    lib = native.load()
+    for heads, n in ((64, 1 << 28), (8, 1 << 28), (64, 1 << 26)):
+        assert lib.spf_window_attention(PTR, 1 << 14, 128, PTR, 1 << 14, 128, PTR, 1 << 14, 128, n, n, heads, 8, 128, 0, 0.1, 0, 0, PTR, PTR,
+                                        1 << 40, None) == -6
+    assert _attention(rows=1 << 24, req=4096, most=1 << 12, tw=1 << 24, ts=1 << 24, bytes=1 << 40) == -6
