@@ -309,10 +309,10 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
       const uint16_t* q1 = qb + t_r1 * p.q_sn + h_r1 * p.q_sh;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        qa[ks][0] = in0 ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16)) : 0u;
-        qa[ks][1] = in1 ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16)) : 0u;
-        qa[ks][2] = in0 ? __ldg(reinterpret_cast<const uint32_t*>(q0 + ks * 16 + 8)) : 0u;
-        qa[ks][3] = in1 ? __ldg(reinterpret_cast<const uint32_t*>(q1 + ks * 16 + 8)) : 0u;
+        qa[ks][0] = in0 ? *reinterpret_cast<const uint32_t*>(q0 + ks * 16) : 0u;
+        qa[ks][1] = in1 ? *reinterpret_cast<const uint32_t*>(q1 + ks * 16) : 0u;
+        qa[ks][2] = in0 ? *reinterpret_cast<const uint32_t*>(q0 + ks * 16 + 8) : 0u;
+        qa[ks][3] = in1 ? *reinterpret_cast<const uint32_t*>(q1 + ks * 16 + 8) : 0u;
       }
     }
     // row r sees keys <= hi that are >= lo or < sinks (rows past the item's end: none)
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
       const Step x = step_of(u);
       if (x.k0 >= x.end) return -1;
       if (!table) return 0;
-      const int pg = __ldg(table + (x.k0 >> p.page_shift));
+      const int pg = table[x.k0 >> p.page_shift];
       return pg >= 0 && pg < p.n_pages ? pg : -1;
     };
     auto issue = [&](int u, int page, int stage) {

@@ -82,10 +82,10 @@ inline int ragged_launch_after(void (*kernel)(A...), dim3 grid, int threads, int
 }
 __device__ __forceinline__ void ragged_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Lengths, offsets and strides, which the kernel before may have written.  A load through the read-only path may be moved
-// above the wait; a plain one may not, but is not moved past any copy either (windowed 32K prompt 1158 -> 1173 us).  Queries
-// and entries of the block table may go the read-only path: where they lie follows from a start that is
-// known behind the wait only.
+// Lengths, offsets, strides, queries and the block table may be what the kernel before writes while this one is already there,
+// so none of them is read through the read-only path, which is for what stays the same as long as a kernel lives.  Queries and
+// the table are read by plain loads, whose addresses are known behind the wait only; the others like this, so that they are not
+// moved above the wait (nor past any copy: windowed 32K prompt 1158 -> 1173 us).
 __device__ __forceinline__ int32_t ragged_load(const int32_t* x) {
   int32_t y;
   asm volatile("ld.global.b32 %0, [%1];" : "=r"(y) : "l"(x));

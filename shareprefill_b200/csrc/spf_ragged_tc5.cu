@@ -329,7 +329,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (!p.table || u >= part.units) return 0;
     const int key = key_of(u);
     if (key >= w.span.keys) return p.n_pages;
-    const int got = __ldg(p.table + w.req * p.table_stride + (key >> p.page_shift));
+    const int got = p.table[w.req * p.table_stride + (key >> p.page_shift)];
     return got >= 0 && got < p.n_pages ? got : p.n_pages;
   };
   if (warp == 0) {

@@ -630,6 +630,49 @@ def test_lengths_and_queries_written_by_the_kernel_just_before(requests, new):
         assert torch.equal(x[:len(want)], want), i
 
 
+@pytest.mark.parametrize("requests,new,dim", [(1, 1, 128), (40, 1, 64), (300, 1, 128), (3, 90, 128), (45, 30, 64)])
+def test_tables_and_queries_written_by_the_kernel_just_before(requests, new, dim):
+    g = torch.Generator().manual_seed(requests)
+    k, v = (torch.randn(64, 16, 2, dim, generator=g).to(BF16).cuda() for _ in range(2))
+    cu, seq = _ints([i * new for i in range(requests + 1)]), _ints([new + (37 * r) % 300 for r in range(requests)])
+    steps = []
+    for i in range(3):
+        table = torch.randint(0, 64, (requests, 25), generator=g).to(torch.int32).cuda()
+        q = torch.randn(requests * new, 8, dim, generator=g).to(BF16).cuda()
+        torch.cuda.synchronize()
+        steps.append((table, q, native.paged_attention(q, k, v, table, cu, seq, new, 0.1)))
+        torch.cuda.synchronize()
+    table, q = steps[0][0].clone(), steps[0][1].clone()
+    got = []
+    for i in range(30):
+        for which in ((0, 1), (1, 0))[i // 3 % 2]:
+            (table, q)[which].copy_(steps[i % 3][which])
+        got.append(native.paged_attention(q, k, v, table, cu, seq, new, 0.1))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, steps[i % 3][2]), i
+
+
+@pytest.mark.parametrize("new,dim", [(1, 128), (3, 64), (90, 128), (700, 64)])
+def test_windowed_inputs_written_by_the_kernel_just_before(new, dim):
+    g = torch.Generator().manual_seed(new)
+    steps = []
+    for i in range(3):
+        data = [torch.randn(n, heads, dim, generator=g).to(BF16).cuda() for n, heads in ((new, 8), (900, 2), (900, 2))]
+        torch.cuda.synchronize()
+        steps.append((data, native.window_attention(*data, 0.1, 200, 3)))
+        torch.cuda.synchronize()
+    live = [x.clone() for x in steps[0][0]]
+    got = []
+    for i in range(30):
+        for which in ((0, 1, 2), (2, 0, 1), (1, 2, 0))[i // 3 % 3]:      # each of them once the last to be written
+            live[which].copy_(steps[i % 3][0][which])
+        got.append(native.window_attention(*live, 0.1, 200, 3))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, steps[i % 3][1]), i
+
+
 def test_a_device_that_is_not_the_current_one():
     if torch.cuda.device_count() < 2:
         pytest.skip("one GPU")
