@@ -390,7 +390,8 @@ def decode_attention(q, k, v, softmax_scale, out=None):
 
 # ---------------------------------------------------------------------------- paged cache, sliding window
 # caches: [n_pages, page_size, Hkv, D] views of bfloat16 or float16 (any page/token/head strides that are
-# multiples of 8).  Every call runs on its tensors' device and that device's current stream; scratch is
+# multiples of 8).  There is no backward pass: tensors that require a gradient are refused where gradients are enabled.
+# Every call runs on its tensors' device and that device's current stream; scratch is
 # taken from torch's allocator per call, so calls and captured graphs never share it.
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
@@ -432,6 +433,14 @@ def _elsewhere(dev, what: str):
     if dev.type != "cuda":
         raise SpfError(f"{what} needs CUDA tensors: there is no CPU fallback")
     return None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _no_grad(what: str, *tensors):
+    """These operators have no backward pass: refuse what would silently drop a gradient."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise SpfError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def _raw_stream(dev) -> int:
@@ -506,6 +515,7 @@ def _rows(t: torch.Tensor, name: str):
 def paged_write(k, v, slot_map, k_cache, v_cache) -> None:
     """``k_cache[slot] = k[row]``, ``v_cache[slot] = v[row]`` for the rows of ``slot_map`` (int64 ``[rows]``, as
     ``paged_plan`` returns it); slots outside the cache are skipped, slots of one call must differ."""
+    _no_grad("paged_write", k, v, k_cache, v_cache)
     dev = k.device
     ctx = _elsewhere(dev, "paged_write")
     if ctx is not None:
@@ -554,6 +564,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
     block_table, cu_new, seq_len: as ``paged_plan`` leaves them; max_new: at least the largest number of new tokens of
     a request; window: keys a token sees including its own (0: all), sinks: first tokens that stay visible.  Rows
     that see nothing are zero, rows behind the last request stay as they were in ``out``."""
+    _no_grad("paged_attention", q, k_cache, v_cache)
     dev, dtype = q.device, q.dtype
     ctx = _elsewhere(dev, "paged_attention")
     if ctx is not None:
@@ -583,6 +594,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
 def window_attention(q, k, v, softmax_scale: float, window: int, sinks: int = 0, out=None):
     """q ``[n, H, D]``: the last n of the N tokens of k/v ``[N, Hkv, D]`` -> ``[n, H, D]``; a token sees the last
     ``window`` keys up to its own (0: all) and the first ``sinks``."""
+    _no_grad("window_attention", q, k, v)
     dev, dtype = q.device, q.dtype
     ctx = _elsewhere(dev, "window_attention")
     if ctx is not None:

@@ -149,3 +149,23 @@ def test_more_work_than_a_call_can_count_is_refused():
         assert lib.spf_window_attention(PTR, 1 << 14, 128, PTR, 1 << 14, 128, PTR, 1 << 14, 128, n, n, heads, 8, 128, 0, 0.1, 0, 0, PTR, PTR,
                                         1 << 40, None) == -6
     assert _attention(rows=1 << 24, req=4096, most=1 << 12, tw=1 << 24, ts=1 << 24, bytes=1 << 40) == -6
+
+
+def test_gradients_are_refused_not_dropped():
+    from types import SimpleNamespace
+
+    from shareprefill_b200.attention import shareprefill_attention_forward as forward
+    q, c, i = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    g, gc = q.clone().requires_grad_(), c.clone().requires_grad_()
+    module = SimpleNamespace(training=True, attention_dropout=0.0, scaling=0.1)
+    x = torch.zeros(1, 4, 9, 64, dtype=torch.bfloat16, requires_grad=True)
+    calls = [lambda: native.paged_attention(g, c, c, i[:, None], i, i, 1, 0.1), lambda: native.paged_attention(q, gc, c, i[:, None], i, i, 1, 0.1),
+             lambda: native.paged_attention(q, c, gc, i[:, None], i, i, 1, 0.1), lambda: native.window_attention(g, q, q, 0.1, 4),
+             lambda: native.window_attention(q, g, q, 0.1, 4), lambda: native.window_attention(q, q, g, 0.1, 4),
+             lambda: native.paged_write(g, q, i.long(), c, c), lambda: native.paged_write(q, q, i.long(), c, gc),
+             lambda: forward(module, x, x[:, :2], x[:, :2], None, sliding_window=4)]
+    for call in calls:
+        with pytest.raises(native.SpfError, match="no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(native.SpfError, match="CUDA"):
+            call()
