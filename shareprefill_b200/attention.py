@@ -88,7 +88,8 @@ def sliding_window_attention(module, query_states, key_states, value_states, win
     """A layer with a sliding window: ``[1,H,N,D]`` -> ``[1,N,H,D]``, every token sees the last ``window`` keys up to its
     own.  The reference refuses such layers (attn/shareprefill_attn.py:160-184); they need no block selection.  A prompt brings
     all its keys, a decode step one query and the keys that its cache kept (all, or at least the last ``window``).
-    Batch 1: padding is not visible at this interface."""
+    Batch 1: padding is not visible at this interface.  Refused are more keys than tokens were seen, as far as a patched
+    model knows their number: buffers of a fixed size that are not full yet."""
     bsz, _, q_len, head_dim = query_states.shape
     if bsz != 1:
         raise NotImplementedError("sliding-window layers are served with batch size 1")
@@ -99,6 +100,10 @@ def sliding_window_attention(module, query_states, key_states, value_states, win
         raise native.SpfError(f"sliding window: the B200 kernels have no attention dropout (got {dropout})")
     if window < 1:
         raise native.SpfError(f"sliding window must be at least 1 (got {window})")
+    tokens = getattr(getattr(module, "attention_sharing", None), "tokens_so_far", None)
+    if tokens is not None and key_states.shape[2] > tokens:
+        raise NotImplementedError(f"sliding window: {key_states.shape[2]} keys of {tokens} tokens; a cache whose buffer has places that no "
+                                  "token has filled (a static cache) is not supported by windowed layers")
     out = native.window_attention(_token_major(query_states[0]), _token_major(key_states[0]), _token_major(value_states[0]),
                                   getattr(module, "scaling", 1.0 / math.sqrt(head_dim)), window)
     return out[None]
@@ -124,7 +129,7 @@ def shareprefill_attention_forward(module, query_states, key_states, value_state
     """Hugging Face attention interface: q ``[B,H,N,D]``, k/v ``[B,Hkv,N,D]`` ->
     ``(attn_output [B,N,H,D] contiguous, attn_weights or None)``.  ``attention_mask``,
     ``scaling`` and ``dropout`` are ignored as in the reference (the scale is read from
-    ``module.scaling``).  Layers that pass ``sliding_window`` go to ``sliding_window_attention``."""
+    ``module.scaling``).  Layers that pass ``sliding_window`` go to ``sliding_window_attention``; they refuse a mask."""
     sliding_window = kwargs.pop("sliding_window", None)
     gqa_interleave = kwargs.pop("gqa_interleave", False)
     if sliding_window is not None:
@@ -133,6 +138,9 @@ def shareprefill_attention_forward(module, query_states, key_states, value_state
         for name in ("s_aux", "softcap"):      # what some models with windowed layers change the softmax by
             if kwargs.get(name) is not None:
                 raise NotImplementedError(f"{name} is not supported by the B200 kernels")
+        causal = kwargs.get("is_causal")
+        if attention_mask is not None or not (getattr(module, "is_causal", True) if causal is None else causal):
+            raise NotImplementedError("windowed layers are causal and take no attention mask")
         return sliding_window_attention(module, query_states, key_states, value_states, int(sliding_window)), None
     return shareprefill_attention_core(module, query_states, key_states, value_states,
                                        gqa_interleave=gqa_interleave)

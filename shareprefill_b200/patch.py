@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import functools
 import importlib
+import inspect
 import logging
 
 from . import native
@@ -102,13 +103,24 @@ def shareprefill_patch(model, config: SharePrefillConfig):
     model.model._use_sdpa = False
 
     original = model.forward.__func__
+    signature = inspect.signature(original)
+
+    def tokens_so_far(self, args, kwargs):
+        """Tokens in the cache and in this forward; None where the arguments do not say."""
+        given = signature.bind_partial(self, *args, **kwargs).arguments
+        given = {**given, **given.get("kwargs", {})}
+        new = given.get("input_ids") if given.get("input_ids") is not None else given.get("inputs_embeds")
+        cache = given.get("past_key_values")
+        if new is None or (cache is not None and not hasattr(cache, "get_seq_length")):
+            return None
+        return (int(cache.get_seq_length()) if cache is not None else 0) + new.shape[1]
 
     @functools.wraps(original)
     def forward_with_reset(self, *args, **kwargs):
         # a kernel of the previous forward that gave up on a bounded wait left rows unwritten: say so
         # here, where a synchronisation costs nothing (the previous forward's result has been used)
         native.raise_on_device_timeouts()
-        self.reset_attention_sharing()
+        self.reset_attention_sharing().tokens_so_far = tokens_so_far(self, args, kwargs)
         return original(self, *args, **kwargs)
 
     model.forward = forward_with_reset.__get__(model, model.__class__)

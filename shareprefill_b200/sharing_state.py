@@ -78,6 +78,7 @@ class AttentionSharing:
         self._needs_reset = True
         self.last_pattern: Optional[BlockPattern] = None
         self.on_stage = None   # optional callable(stage_name), e.g. to record CUDA events
+        self.tokens_so_far: Optional[int] = None   # tokens of the sequence up to the forward's last, where the model knows it
 
     def _mark(self, stage: str):
         if self.on_stage is not None:

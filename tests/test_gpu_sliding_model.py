@@ -4,7 +4,7 @@ import json
 import pytest
 import torch
 
-from shareprefill_b200 import SharePrefill
+from shareprefill_b200 import SharePrefill, native
 from shareprefill_b200.workloads import synthetic_lookup
 
 pytestmark = pytest.mark.gpu
@@ -58,4 +58,36 @@ def test_decoding_behind_a_sliding_cache_matches_eager(tmp_path):
     want = logits(model)
     got = logits(_patched(model, tmp_path))
     err = (got - want).abs()
+    assert err.max() < 0.15 and err.mean() < 0.01, (err.max().item(), err.mean().item())
+
+
+@pytest.mark.parametrize("prompt,cached,refused", [(150, "static", False), (30, "static", True), (30, "dynamic", False), (1, "static", True), (1, "dynamic", False)])
+def test_caches_of_a_fixed_size_are_served_when_full_and_refused_before(tmp_path, prompt, cached, refused):
+    from transformers import DynamicCache, Qwen2Config, Qwen2ForCausalLM, StaticCache
+    cfg = Qwen2Config(vocab_size=128, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, max_position_embeddings=4096, use_sliding_window=True, sliding_window=WINDOW,
+                      max_window_layers=0, attn_implementation="eager")
+    assert set(cfg.layer_types) == {"sliding_attention"}
+    torch.manual_seed(0)
+    model = Qwen2ForCausalLM(cfg).to(torch.bfloat16).cuda().eval()
+    ids = torch.randint(0, 128, (1, prompt + 5), generator=torch.Generator().manual_seed(4)).cuda()
+
+    def logits():
+        cache = StaticCache(config=cfg, max_cache_len=400) if cached == "static" else DynamicCache(config=cfg)
+        with torch.no_grad():
+            out = [model(ids[:, :prompt], past_key_values=cache).logits[:, -1].float()]
+            for i in range(prompt, prompt + 5):
+                out.append(model(ids[:, i:i + 1], None, None, cache).logits[:, -1].float())      # (also by position)
+        return torch.stack(out)
+
+    want = logits()
+    p = tmp_path / "l.json"
+    p.write_text(json.dumps(synthetic_lookup(2, 4, 2, group_size=2)))
+    model = SharePrefill(model_name="tiny", sharing_lookup_path=str(p), block_size=64, min_budget=4096)(model)
+    if refused:
+        # a prompt of 30 tokens meets 70 keys; one token could pass for a step behind 69
+        with pytest.raises((NotImplementedError, native.SpfError), match="sliding window"):
+            logits()
+        return
+    err = (logits() - want).abs()
     assert err.max() < 0.15 and err.mean() < 0.01, (err.max().item(), err.mean().item())

@@ -169,3 +169,25 @@ def test_gradients_are_refused_not_dropped():
             call()
         with torch.no_grad(), pytest.raises(native.SpfError, match="CUDA"):
             call()
+
+
+def test_sliding_window_layers_refuse_masks_other_orders_and_buffers_that_are_not_full():
+    from types import SimpleNamespace
+
+    from shareprefill_b200.attention import shareprefill_attention_forward as forward
+    x = torch.zeros(1, 4, 9, 64, dtype=torch.bfloat16)
+    module = SimpleNamespace(training=False, attention_dropout=0.0, scaling=0.1)
+    with pytest.raises(NotImplementedError, match="mask"):
+        forward(module, x, x[:, :2], x[:, :2], torch.zeros(1, 1, 9, 9), sliding_window=4)
+    with pytest.raises(NotImplementedError, match="causal"):
+        forward(module, x, x[:, :2], x[:, :2], None, sliding_window=4, is_causal=False)
+    for causal in (True, None):
+        with pytest.raises(native.SpfError, match="CUDA"):
+            forward(module, x, x[:, :2], x[:, :2], None, sliding_window=4, is_causal=causal)
+    with pytest.raises(NotImplementedError, match="causal"):
+        forward(SimpleNamespace(**vars(module), is_causal=False), x, x[:, :2], x[:, :2], None, sliding_window=4)
+    for tokens, error, words in ((5, NotImplementedError, "5 tokens"), (8, NotImplementedError, "8 tokens"), (9, native.SpfError, "CUDA"),
+                                 (40, native.SpfError, "CUDA"), (None, native.SpfError, "CUDA")):
+        module.attention_sharing = SimpleNamespace(tokens_so_far=tokens)
+        with pytest.raises(error, match=words):
+            forward(module, x[:, :, :1], x[:, :2], x[:, :2], None, sliding_window=8)
