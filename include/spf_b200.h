@@ -294,7 +294,7 @@ int spf_paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_requ
  * k_cache, v_cache [n_pages][page_size][Hkv][D], all with the given strides in elements (multiples of 8; D
  * contiguous; a cache stored head-major is the same with other strides).  Rows whose slot lies outside
  * [0, n_pages * page_size) are skipped.  Slots of one call must differ: of two rows with the same slot
- * either may be found there, in whole or in part.
+ * either may be found there, in whole or in part.  Caches with a stride of 0 (expanded views) are SPF_ERR_RANGE.
  */
 int spf_paged_write(const void* k, int64_t k_stride_n, int64_t k_stride_h,
                     const void* v, int64_t v_stride_n, int64_t v_stride_h,

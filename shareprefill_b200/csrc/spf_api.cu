@@ -383,6 +383,11 @@ int spf_paged_write(const void* k, int64_t k_stride_n, int64_t k_stride_h, const
       !strides_ok(v_stride_n, v_stride_h) || !strides_ok(k_stride_page, k_stride_token) || k_stride_head % 8 ||
       !strides_ok(v_stride_page, v_stride_token) || v_stride_head % 8)
     return SPF_ERR_ALIGN;
+  // several elements in one place (an expanded view) would be written in no order
+  const bool heads = n_kv_heads > 1, pages = n_pages > 1;
+  if (k_stride_token == 0 || v_stride_token == 0 || (heads && (k_stride_head == 0 || v_stride_head == 0)) ||
+      (pages && (k_stride_page == 0 || v_stride_page == 0)))
+    return SPF_ERR_RANGE;
   WriteParams p;
   p.k = WriteTensor{static_cast<const uint16_t*>(k), k_stride_n, k_stride_h, static_cast<uint16_t*>(k_cache),
                     k_stride_page, k_stride_token, k_stride_head};

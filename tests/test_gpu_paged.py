@@ -136,6 +136,20 @@ def test_write_puts_rows_in_their_slots_and_nothing_else(rows, kv_heads, dim, pa
     assert torch.equal(k_cache, want_k) and torch.equal(v_cache, want_v)
 
 
+def test_write_refuses_expanded_caches_and_takes_one_page_or_head_of_any_stride():
+    rows = torch.randn(16, 2, 64, device="cuda").to(BF16)
+    slots = torch.arange(16, device="cuda")
+    cache = torch.zeros(2, 16, 2, 64, dtype=BF16, device="cuda")
+    for view in (cache[:1].expand(2, -1, -1, -1), cache[:, :1].expand(-1, 16, -1, -1), cache[:, :, :1].expand(-1, -1, 2, -1)):
+        for pair in ((view, cache), (cache, view)):
+            with pytest.raises(native.SpfError):
+                native.paged_write(rows, rows, slots, *pair)
+    assert not cache.any()
+    one = cache.as_strided((1, 16, 1, 64), (0, 128, 0, 1))
+    native.paged_write(rows[:, :1], rows[:, :1], slots, one, one)
+    assert torch.equal(cache[0, :, :1], rows[:, :1]) and not cache[1].any() and not cache[:, :, 1].any()
+
+
 # ------------------------------------------------------------------------------------- attention
 CASES = [
     # (cached, new) per request, page, heads, kv heads, head size, type, window, sinks, cache layout

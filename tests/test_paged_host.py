@@ -191,3 +191,10 @@ def test_sliding_window_layers_refuse_masks_other_orders_and_buffers_that_are_no
         module.attention_sharing = SimpleNamespace(tokens_so_far=tokens)
         with pytest.raises(error, match=words):
             forward(module, x[:, :, :1], x[:, :2], x[:, :2], None, sliding_window=8)
+
+
+def test_writes_into_expanded_caches_are_refused():
+    def write(kp=4096, kt=256, kh=128, vp=4096, vt=256, vh=128, heads=2, pages=0):
+        return native.load().spf_paged_write(PTR, 256, 128, PTR, 256, 128, PTR, 4, heads, 128, PTR, kp, kt, kh, PTR, vp, vt, vh, pages or 3, 16, None)
+    for name in ("kp", "kt", "kh", "vp", "vt", "vh"):
+        assert write(**{name: 0}) == -4, name
