@@ -420,8 +420,10 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
         y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 1)); y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 2));
         const float n0 = fmaxf(m0, y0 * p.scale_log2), n1 = fmaxf(m1, y1 * p.scale_log2);
         const float f0 = n0 == -INFINITY ? 0.f : n0, f1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet: all weights are 0
-        // fp16: the largest weight is 2^15, so that multiples of 2^-24 lose 2^-40 of it per key (the factor cancels in o / l)
-        const float g0 = FP16 ? f0 - 15.f : f0, g1 = FP16 ? f1 - 15.f : f1;
+        // The largest weight is 2^LIFT; the factor cancels in o / l.  fp16: multiples of 2^-24 lose 2^-40 of it per key; bf16: o
+        // does not overflow with values up to 3.4e38
+        constexpr float LIFT = FP16 ? 15.f : -32.f;
+        const float g0 = f0 - LIFT, g1 = f1 - LIFT;
         if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {      // rare once a few tiles have been seen
           const float a0 = ex2(m0 - f0), a1 = ex2(m1 - f1);
           l0 *= a0; l1 *= a1;

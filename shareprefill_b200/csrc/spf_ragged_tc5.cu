@@ -567,12 +567,14 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   } else {
     // ------------------------------------------------------------ softmax warpgroups
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(RT_REGS_SOFTMAX));
-    // P must stay inside its type's range: a unit's sum of P above this moves the reference point to the unit's maximum.
-    // In fp16 weights are 2^ROOM times what the reference point says: the largest is 2^8 (128 of them stay below the limit)
-    // and what multiples of 2^-24 lose is 2^-33 of it per key, not 2^-25, which over 100K keys behind one that all tokens
-    // look at was 0.4% of the mass.  The factor cancels in O / l, and all parts of an item have it.
-    constexpr float SUM_LIMIT = FP16 ? 61440.f : 1180591620717411303424.f;   // 15/16 of 2^16, 2^70
-    constexpr float MARGIN = FP16 ? 0.f : 64.f, ROOM = FP16 ? 8.f : 0.f;
+    // Weights are 2^LIFT times what the reference point says, and a unit's sum of them above SUM_LIMIT moves the point to the
+    // unit's maximum.  The factor cancels in O / l, and all parts of an item have it.
+    //   bf16: O, the sum of weight times value, must not overflow with values up to 3.4e38, so weights are 2^-32 and less at
+    //         first, and a unit's sum stays below 2^-8 (without this a score that rose by 2^60 overflowed with values of 1e25)
+    //   fp16: P reaches 65504 only, and the multiples of 2^-24 that small weights are rounded to should be small against the
+    //         largest weight: at 2^8 (128 of them are below the limit) they lose 2^-33 of it per key, not 2^-25, which over
+    //         100K keys behind one that all tokens look at was 0.4% of the mass
+    constexpr float SUM_LIMIT = FP16 ? 61440.f : 0.00390625f, MARGIN = FP16 ? 0.f : 12.f, LIFT = FP16 ? 8.f : -32.f;
     // The 128 scores of a row and the constants of the exponentials leave about twenty registers: what the loop over
     // units does not need is looked up (in shared memory) or computed again where it is used.
     const int h = (warp - 4) >> 2;
@@ -665,7 +667,7 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         float blk;
         bool moved = u == 0;
         while (true) {
-          const float ref = m_used == -INFINITY ? 0.f : m_used - ROOM;
+          const float ref = m_used == -INFINITY ? 0.f : m_used - LIFT;
           blk = 0.f;
           uint32_t s0[32], s1[32], s2[32], s3[32];
           tmem_ld32_raw(tS + 0, s0);

@@ -427,6 +427,28 @@ def test_fp16_weights_far_below_the_largest_still_add_up(new, dim):
     assert float(off.max()) <= 1.0, f"{float(off.max()):.3g} times the tolerance"
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,keys,heads", [(1, 300, 4), (1, 5000, 4), (40, 300, 4), (200, 5000, 2)])
+def test_values_up_to_the_largest_of_the_type_do_not_overflow(new, keys, heads, dim):
+    # scores that rise along the sequence by 2^60 in all (the tcgen05 kernel keeps a row's reference point while it can), and
+    # values of 3e38, of which two do not add up in fp32
+    g = torch.Generator().manual_seed(keys + dim)
+    before, scale = keys - new, 0.125
+    q = torch.randn(new, heads, dim, generator=g).to(BF16)
+    k, v = (torch.randn(keys, 1, dim, generator=g).to(BF16) for _ in range(2))
+    q[:, :, 0], k[:, :, 0] = 8.0, torch.linspace(0, 41, keys).to(BF16)[:, None]
+    for size in (1e-20, 1e25, 3e38):
+        big = (v.sign() * size).to(BF16) if size > 1e30 else (v.double() * size).to(BF16)
+        big[:, :, 1] = torch.tensor(size, dtype=BF16)                 # the same value everywhere: their mean is it
+        for rising in (True, False):
+            if not rising:
+                k[:, :, 0] = 0.0
+            out, mass = R.attention(q, k, big, before, scale)
+            got = native.window_attention(q.cuda(), k.cuda(), big.cuda(), scale, 0)
+            R.check(got, out, mass, BF16, keys, 5.0, f"{size} {rising}")
+        k[:, :, 0] = torch.linspace(0, 41, keys).to(BF16)[:, None]
+
+
 @pytest.mark.parametrize("new", [1, 200])
 @pytest.mark.parametrize("gain", [30.0, 1e4])
 def test_peaked_scores_and_expanded_caches(new, gain):
