@@ -435,12 +435,10 @@ def _elsewhere(dev, what: str):
     return None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _no_grad(what: str, *tensors):
+def _no_grad(what: str):
     """These operators have no backward pass: refuse what would silently drop a gradient."""
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise SpfError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+        raise SpfError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def _raw_stream(dev) -> int:
@@ -515,7 +513,8 @@ def _rows(t: torch.Tensor, name: str):
 def paged_write(k, v, slot_map, k_cache, v_cache) -> None:
     """``k_cache[slot] = k[row]``, ``v_cache[slot] = v[row]`` for the rows of ``slot_map`` (int64 ``[rows]``, as
     ``paged_plan`` returns it); slots outside the cache are skipped, slots of one call must differ."""
-    _no_grad("paged_write", k, v, k_cache, v_cache)
+    if k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad:
+        _no_grad("paged_write")
     dev = k.device
     ctx = _elsewhere(dev, "paged_write")
     if ctx is not None:
@@ -564,7 +563,8 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
     block_table, cu_new, seq_len: as ``paged_plan`` leaves them; max_new: at least the largest number of new tokens of
     a request; window: keys a token sees including its own (0: all), sinks: first tokens that stay visible.  Rows
     that see nothing are zero, rows behind the last request stay as they were in ``out``."""
-    _no_grad("paged_attention", q, k_cache, v_cache)
+    if q.requires_grad or k_cache.requires_grad or v_cache.requires_grad:
+        _no_grad("paged_attention")
     dev, dtype = q.device, q.dtype
     ctx = _elsewhere(dev, "paged_attention")
     if ctx is not None:
@@ -594,7 +594,8 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: 
 def window_attention(q, k, v, softmax_scale: float, window: int, sinks: int = 0, out=None):
     """q ``[n, H, D]``: the last n of the N tokens of k/v ``[N, Hkv, D]`` -> ``[n, H, D]``; a token sees the last
     ``window`` keys up to its own (0: all) and the first ``sinks``."""
-    _no_grad("window_attention", q, k, v)
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _no_grad("window_attention")
     dev, dtype = q.device, q.dtype
     ctx = _elsewhere(dev, "window_attention")
     if ctx is not None:
