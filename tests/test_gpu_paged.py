@@ -101,6 +101,20 @@ def test_plan_from_the_end_of_a_ring_of_more_than_2_to_the_30_ids():
         assert p.slot_map.tolist() == [16 * page + i for page, n in ((7, 16), (5, 16), (9, 1), (4, 16), (6, 1)) for i in range(n)]
 
 
+def test_plan_may_put_its_outputs_where_its_inputs_were():
+    lib, page, rows = native.load(), 16, 40
+    cached, new = [15, 0, 16, 100], [2, 17, 0, 9]
+    table = [[4, -1, -1], [-1] * 3, [6, -1, -1], [-1] * 3]
+    want = R.plan(cached, new, table, 3, [9, 8, 7, 5], 2, 4, rows, page)
+    seq, fresh, t, ring, state = _ints(cached), _ints(new), _ints(table), _ints([9, 8, 7, 5]), _ints([2, 4])
+    cu, slots, positions = _ints([0] * 5), torch.empty(rows, dtype=torch.int64, device="cuda"), _ints([0] * rows)
+    assert lib.spf_paged_plan(seq.data_ptr(), fresh.data_ptr(), 4, page, t.data_ptr(), 3, 3, ring.data_ptr(), 4, state.data_ptr(), state.data_ptr(),
+                              cu.data_ptr(), seq.data_ptr(), slots.data_ptr(), positions.data_ptr(), fresh.data_ptr(), rows,
+                              torch.cuda.current_stream().cuda_stream) == 0
+    got = dict(table=t, cu_new=cu, seq_len=seq, refused=fresh, slot_map=slots, positions=positions, ring_state=state)
+    assert {name: x.tolist() for name, x in got.items()} == want
+
+
 def test_plan_with_extreme_lengths_refuses_and_stays_inside():
     page, top = 16, 2 ** 31 - 1
     table = torch.full((4, 3), -1, dtype=torch.int32, device="cuda")
@@ -601,6 +615,33 @@ def test_a_whole_step_captured_and_replayed():
                 R.check(out[at:at + n], want, mass, dtype, 100, 5.0, f"{new} request {r}")
             at += n
     assert seq.tolist() == [len(h[0]) for h in history]
+
+
+@pytest.mark.parametrize("requests", [20, 60])
+def test_captured_batches_of_tokens_and_chunks_in_two_passes(requests):
+    # a wide table sends tokens and chunks through both kernels; 60 requests are scheduled by a kernel of their own
+    page, heads, kv_heads, dim = 16, 8, 2, 64
+    spec = [(i * 23 % 500, 1 if i % 9 else 30 + i) for i in range(requests)]
+    pool, cu, q = _batch(spec, page, heads, kv_heads, dim, BF16, "token", requests)
+    k, v = pool.cuda()
+    table = torch.nn.functional.pad(pool.table, (0, 12000), value=-1).cuda()
+    live = dict(q=torch.zeros_like(q).cuda(), cu=_ints([0] * (requests + 1)), seq=_ints([0] * requests))
+    most = max(n for _, n in spec)
+    for window in (0, 90):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            native.paged_attention(live["q"], k, v, table, live["cu"], live["seq"], most, 0.125, window, 2)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = native.paged_attention(live["q"], k, v, table, live["cu"], live["seq"], most, 0.125, window, 2)
+        for cut in (0, 1):
+            lens = [max(c + n - cut * 7, n) for c, n in spec]
+            live["q"].copy_(q), live["cu"].copy_(_ints(cu)), live["seq"].copy_(_ints(lens))
+            graph.replay()
+            for r, (_, n) in enumerate(spec):
+                want, mass = R.attention(q[cu[r]:cu[r + 1]], *(x[:lens[r]] for x in pool.rows[r]), lens[r] - n, 0.125, window, 2)
+                R.check(out[cu[r]:cu[r + 1]], want, mass, BF16, lens[r], 5.0, f"request {r} window {window} cut {cut}")
 
 
 @pytest.mark.parametrize("new", [1, 60])
