@@ -55,9 +55,10 @@ struct RtCfg {
   static constexpr int SLABS = D / 64, KSTEPS = D / 16;
   static constexpr uint32_t TILE = RT_SLAB * SLABS;
   static constexpr int KST = D == 128 ? 3 : 6, VST = D == 128 ? 2 : 5;
-  // pairs of exponentials out of eight that go to the FMA pipe.  The last 2K chunk of a 34K prompt with 1 / 2 / 3: at
-  // D = 128 1030 / 1055 / 1287 us (3 spills), at D = 64 748 / 735 / 751 us
-  static constexpr int POLY = D == 128 ? 1 : 2;
+  // Pairs of exponentials out of eight that go to the FMA pipe.  At D = 128 the products take as long as the exponentials and
+  // none need go there: the last 2K chunk of a 34K prompt with 0 / 1 / 2 of them takes 1022 / 1028 / 1230 us (2 spills), the
+  // windowed 32K prompt 1172 / 1190 / 1390.  At D = 64, 0 / 1 / 2 / 3: 779 / 735 / 738 / 783 and 935 / 929 / 967 / 1006 us.
+  static constexpr int POLY = D == 128 ? 0 : 1;
   static constexpr bool P_BESIDE = D == 64;        // columns 384 .. 511 are free
   // barriers
   static constexpr int B_PFULL = 0, B_PEMPTY = B_PFULL + RT_PARTS, B_QFULL = B_PEMPTY + RT_PARTS, B_QEMPTY = B_QFULL + 2,
@@ -152,10 +153,9 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // 0, and u = 1 those of infinity.  So a masked score (-infinity) has the weight 0, whatever the value of its key - with 2^-57,
 // where a range of [-57, 71] ended, a value of 1e20 that a token must not see was 690 in its output - and a score far above
 // m shows in the sum.  Weights between 2^-127 and 2^-126 are rounded at will.
-// Saturation makes 0 of NaN too: the sum becomes NaN where one of the polynomial's scores is (1% at D = 128; a mixed batch
-// at D = 64 107.3 -> 110.7 us; sums of the scores and the smallest of them took as long).
+// Saturation makes 0 of NaN too, so `nan` says whether one of the polynomial's scores is NaN (it costs 1 - 2% at D = 64).
 template <int POLY, bool FP16>
-__device__ __forceinline__ void rt_weights(const uint32_t (&r)[32], float scale, float m, uint32_t (&pk)[16], float& sum) {
+__device__ __forceinline__ void rt_weights(const uint32_t (&r)[32], float scale, float m, uint32_t (&pk)[16], float& sum, bool& nan) {
   float top = -INFINITY;
   const unsigned long long sc2 = f2_pack(scale, scale), nm2 = f2_pack(-m, -m);
   const float sc255 = scale * (1.f / 255.f), b255 = (127.f - m) * (1.f / 255.f);
@@ -194,7 +194,8 @@ __device__ __forceinline__ void rt_weights(const uint32_t (&r)[32], float scale,
   }
   float a0, a1;
   f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a0, a1);
-  sum = top == top ? sum + (a0 + a1) : top;
+  sum += a0 + a1;
+  if (POLY > 0) nan |= top != top;
 }
 
 // the n lowest bits (n below 0: none, above 32: all)
@@ -669,21 +670,23 @@ ragged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         while (true) {
           const float ref = m_used == -INFINITY ? 0.f : m_used - LIFT;
           blk = 0.f;
+          bool nan = false;
           uint32_t s0[32], s1[32], s2[32], s3[32];
           tmem_ld32_raw(tS + 0, s0);
           tmem_ld32_raw(tS + 32, s1);
           tc_wait_ld();
           tmem_ld32_raw(tS + 64, s2);
-          rt_weights<C::POLY, FP16>(s0, p.scale_log2, ref, pk0, blk);
+          rt_weights<C::POLY, FP16>(s0, p.scale_log2, ref, pk0, blk, nan);
           if (C::P_BESIDE) tmem_st16(p_tmem(), pk0);
           tmem_ld32_raw(tS + 96, s3);
-          rt_weights<C::POLY, FP16>(s1, p.scale_log2, ref, pk1, blk);
+          rt_weights<C::POLY, FP16>(s1, p.scale_log2, ref, pk1, blk, nan);
           if (C::P_BESIDE) tmem_st16(p_tmem() + 16, pk1);
           tc_wait_ld();
-          rt_weights<C::POLY, FP16>(s2, p.scale_log2, ref, pk2, blk);
+          rt_weights<C::POLY, FP16>(s2, p.scale_log2, ref, pk2, blk, nan);
           if (C::P_BESIDE) tmem_st16(p_tmem() + 32, pk2);
-          rt_weights<C::POLY, FP16>(s3, p.scale_log2, ref, pk3, blk);
+          rt_weights<C::POLY, FP16>(s3, p.scale_log2, ref, pk3, blk, nan);
           if (C::P_BESIDE) tmem_st16(p_tmem() + 48, pk3);
+          if (nan) blk = NAN;
           if (moved || !__any_sync(0xffffffffu, !(blk <= SUM_LIMIT))) break;
           moved = true;
           const float mb = row_max_log2();
