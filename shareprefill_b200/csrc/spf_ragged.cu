@@ -223,7 +223,7 @@ int ragged_merge(const RaggedParams& p, int max_new, int head_dim, cudaStream_t 
 // The rows of an item are the 16 rows of mma.sync m16n8k16 tiles.  A unit is 64 keys, 16 per warp; every
 // warp streams its tiles through a private ring of cp.async stages and keeps its own running maximum, sum
 // and output; the warps meet when the CTA's part of the item ends.  Bound by HBM: 64 tokens of 32 heads over 8 KV heads
-// and up to 8K keys (1.33 GB) take 207 - 217 us, 6.1 - 6.4 TB/s; one token of 28 heads over 128K keys 49 us, 5.5 TB/s, of which
+// and up to 8K keys (1.33 GB) take 216 - 228 us with the join, 5.8 - 6.1 TB/s; one token of 28 heads over 128K keys 49 us, 5.5 TB/s, of which
 // 4 us are launch and start and 3 the end.  Three stages of 16 keys per warp and two CTAs per SM keep 128 KiB of an SM in flight.
 constexpr int RR_NT = 128, RR_NW = RR_NT / 32, RR_TT = 16, RR_STAGES = 3, RR_ROWS = 16;
 
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(RR_NT, D == 64 ? 3 : 2) ragged_rows_kernel(con
   }
 }
 
-// As many CTAs as fit: at D = 128 two per SM (96 KiB of rings, 236 registers), at D = 64 three (156 registers).  A decode
+// As many CTAs as fit: at D = 128 two per SM (96 KiB of rings, 250 registers), at D = 64 three (157 registers).  A decode
 // batch of 64 requests up to 8K with D = 64 takes 145 / 129 / 173 us with 2 / 3 / 4 per SM, 133 with four of 128 registers.
 void ragged_rows_config(RaggedParams& p, bool solo) {
   p.tile_rows = RR_ROWS;
