@@ -104,9 +104,12 @@ def shareprefill_patch(model, config: SharePrefillConfig):
 
     original = model.forward.__func__
     signature = inspect.signature(original)
+    windowed = any(getattr(m, "sliding_window", None) is not None for m in (model.config, *model.modules()))
 
     def tokens_so_far(self, args, kwargs):
-        """Tokens in the cache and in this forward; None where the arguments do not say."""
+        """Tokens in the cache and in this forward; None where the arguments do not say (only layers with a window ask)."""
+        if not windowed:
+            return None
         given = signature.bind_partial(self, *args, **kwargs).arguments
         given = {**given, **given.get("kwargs", {})}
         new = given.get("input_ids") if given.get("input_ids") is not None else given.get("inputs_embeds")
@@ -120,8 +123,12 @@ def shareprefill_patch(model, config: SharePrefillConfig):
         # a kernel of the previous forward that gave up on a bounded wait left rows unwritten: say so
         # here, where a synchronisation costs nothing (the previous forward's result has been used)
         native.raise_on_device_timeouts()
-        self.reset_attention_sharing().tokens_so_far = tokens_so_far(self, args, kwargs)
-        return original(self, *args, **kwargs)
+        sharing = self.reset_attention_sharing()
+        sharing.tokens_so_far = tokens_so_far(self, args, kwargs)
+        try:
+            return original(self, *args, **kwargs)
+        finally:
+            sharing.tokens_so_far = None
 
     model.forward = forward_with_reset.__get__(model, model.__class__)
     LOGGER.info("Patched model for shareprefill.")

@@ -91,3 +91,6 @@ def test_caches_of_a_fixed_size_are_served_when_full_and_refused_before(tmp_path
         return
     err = (logits() - want).abs()
     assert err.max() < 0.15 and err.mean() < 0.01, (err.max().item(), err.mean().item())
+    assert model.attention_sharing.tokens_so_far is None          # a call of the decoder by itself is not measured by it
+    with torch.no_grad():
+        assert torch.isfinite(model.model(torch.zeros(1, 400, dtype=torch.int64, device="cuda")).last_hidden_state).all()
