@@ -4,7 +4,7 @@ import json
 import pytest
 import torch
 
-from shareprefill_b200 import SharePrefill, native
+from shareprefill_b200 import SharePrefill
 from shareprefill_b200.workloads import synthetic_lookup
 
 pytestmark = pytest.mark.gpu
@@ -64,6 +64,8 @@ def test_decoding_behind_a_sliding_cache_matches_eager(tmp_path):
 @pytest.mark.parametrize("prompt,cached,refused", [(150, "static", False), (30, "static", True), (30, "dynamic", False), (1, "static", True), (1, "dynamic", False)])
 def test_caches_of_a_fixed_size_are_served_when_full_and_refused_before(tmp_path, prompt, cached, refused):
     from transformers import DynamicCache, Qwen2Config, Qwen2ForCausalLM, StaticCache
+
+    from shareprefill_b200 import native
     cfg = Qwen2Config(vocab_size=128, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
                       num_key_value_heads=2, max_position_embeddings=4096, use_sliding_window=True, sliding_window=WINDOW,
                       max_window_layers=0, attn_implementation="eager")
